@@ -3,6 +3,6 @@ backward, elementwise chains) as hand-written sm_100a kernels behind a C ABI
 (include/c3cu.h), with a C++ mirror of C3's install-and-dispatch API."""
 from . import _lib
 from ._lib import C3CUError, device_check, fault_status, load
-from . import linear, elementwise
+from . import linear, elementwise, norm, quant
 
-__all__ = ["C3CUError", "device_check", "fault_status", "load", "linear", "elementwise", "_lib"]
+__all__ = ["C3CUError", "device_check", "fault_status", "load", "linear", "elementwise", "norm", "quant", "_lib"]

@@ -81,6 +81,16 @@ _SIGNATURES = {
     "c3cu_ew_backward_chain": ([_vp, _i, _vp, _vp, _vp, _i64, _vp], _i),
     "c3cu_softmax_ce_f32": ([_vp, _vp, _vp, _vp, _i64, _i64, _vp], _i),
     "c3cu_sgd_f32": ([_vp, _vp, _vp, _i, ctypes.c_float, _vp], _i),
+    "c3cu_quantize_rows": ([_vp, _i64, _i, _vp, _i64, _vp, _i64, _i64, _vp], _i),
+    "c3cu_rms_norm_int8": ([_vp, _i64, _vp, _i64, _i, _vp, ctypes.c_float, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64,
+                            _vp], _i),
+    "c3cu_rms_norm_bwd_workspace": ([_i64, _i64], _sz),
+    "c3cu_rms_norm_bwd": ([_vp, _i64, _vp, _i64, _vp, _i64, _i, _vp, _vp, _vp, _i64, _vp, _i64, _i64, _vp, _sz, _vp],
+                          _i),
+    "c3cu_linear_int8_fwd": ([_vp, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i, _i, _vp, _i64, _i64, _i64, _i64,
+                              _vp], _i),
+    "c3cu_gemm_dw_int8_workspace": ([_i64, _i64, _i64], _sz),
+    "c3cu_gemm_dw_int8": ([_vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _sz, _vp], _i),
     "c3cu_flash_attn_fwd": ([_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, ctypes.c_float, _i, _vp], _i),
 }
 

@@ -20,6 +20,8 @@ int c3cu_fault_get_nvls(uint32_t* out);
 int c3cu_fault_clear_nvls();
 int c3cu_fault_get_train(uint32_t* out);
 int c3cu_fault_clear_train();
+int c3cu_fault_get_int8(uint32_t* out);
+int c3cu_fault_clear_int8();
 
 namespace c3cu {
 
@@ -105,16 +107,17 @@ PFN_cuTensorMapEncodeTiled_v12000 get_encode_fn() {
 }
 }  // namespace
 
-int encode_bf16_2d_sw128(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols,
-                         uint64_t ld, uint32_t box_cols, uint32_t box_rows) {
+namespace {
+int encode_2d(CUtensorMap* map, CUtensorMapDataType type, const char* name, uint32_t esize, const void* base,
+              uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_cols, uint32_t box_rows, bool swizzle) {
   if (!aligned16(base)) {
     set_error("TMA operand base %p is not 16-byte aligned", base);
     return C3CU_ERR_ALIGN;
   }
-  if ((ld * 2u) % 16u != 0u || ld < cols) {
-    set_error("TMA operand row stride %llu elements (bf16) is not a multiple of 16 bytes or is "
+  if ((ld * esize) % 16u != 0u || ld < cols) {
+    set_error("TMA operand row stride %llu elements (%s) is not a multiple of 16 bytes or is "
               "smaller than the row length %llu",
-              (unsigned long long)ld, (unsigned long long)cols);
+              (unsigned long long)ld, name, (unsigned long long)cols);
     return C3CU_ERR_ALIGN;
   }
   auto fn = get_encode_fn();
@@ -123,11 +126,11 @@ int encode_bf16_2d_sw128(CUtensorMap* map, const void* base, uint64_t rows, uint
     return C3CU_ERR_CUDA;
   }
   const cuuint64_t dims[2] = {cols, rows};
-  const cuuint64_t strides[1] = {ld * 2u};
+  const cuuint64_t strides[1] = {ld * esize};
   const cuuint32_t box[2] = {box_cols, box_rows};
   const cuuint32_t estr[2] = {1u, 1u};
-  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides,
-                  box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+  CUresult r = fn(map, type, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
     set_error("cuTensorMapEncodeTiled failed (CUresult %d) rows=%llu cols=%llu ld=%llu box=%ux%u",
@@ -136,6 +139,17 @@ int encode_bf16_2d_sw128(CUtensorMap* map, const void* base, uint64_t rows, uint
     return C3CU_ERR_CUDA;
   }
   return C3CU_OK;
+}
+}  // namespace
+
+int encode_bf16_2d_sw128(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols,
+                         uint64_t ld, uint32_t box_cols, uint32_t box_rows) {
+  return encode_2d(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, "bf16", 2u, base, rows, cols, ld, box_cols, box_rows, true);
+}
+
+int encode_int8_2d(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_cols,
+                   uint32_t box_rows, bool swizzle) {
+  return encode_2d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, "int8", 1u, base, rows, cols, ld, box_cols, box_rows, swizzle);
 }
 
 }  // namespace c3cu
@@ -162,10 +176,10 @@ int c3cu_fault_status(uint32_t* code) {
   *code = 0u;
   int rc = c3cu::cuda_status(cudaDeviceSynchronize(), "c3cu_fault_status: synchronize");
   if (rc != C3CU_OK) return rc;
-  uint32_t words[5] = {0u, 0u, 0u, 0u, 0u};
+  uint32_t words[6] = {0u, 0u, 0u, 0u, 0u, 0u};
   if (c3cu_fault_get_gemm(&words[0]) || c3cu_fault_get_ew(&words[1]) ||
       c3cu_fault_get_attn(&words[2]) || c3cu_fault_get_nvls(&words[3]) ||
-      c3cu_fault_get_train(&words[4])) {
+      c3cu_fault_get_train(&words[4]) || c3cu_fault_get_int8(&words[5])) {
     c3cu::set_error("c3cu_fault_status: reading fault words failed");
     return C3CU_ERR_CUDA;
   }
@@ -176,6 +190,7 @@ int c3cu_fault_status(uint32_t* code) {
   c3cu_fault_clear_attn();
   c3cu_fault_clear_nvls();
   c3cu_fault_clear_train();
+  c3cu_fault_clear_int8();
   if (*code != 0u) {
     c3cu::gemm_invalidate_split_workspaces();
     c3cu::set_error("kernel fault recorded: code %u (site %u)", *code & 0xffffu, *code >> 16);

@@ -39,34 +39,6 @@ std::map<TuneKey, int> g_tune;
 // applies, without the split-K tail.
 std::atomic<int> g_variant{0};
 
-// Co-resident clusters of two CTAs for a kernel (cached per device and kernel).
-template <class Kern>
-int max_pair_clusters(Kern kern, uint32_t smem_bytes, int threads) {
-  static std::atomic<int> cached[64] = {};
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
-  const int have = cached[dev].load(std::memory_order_relaxed);
-  if (have > 0) return have;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(2 * 74, 1, 1);
-  cfg.blockDim = dim3(threads, 1, 1);
-  cfg.dynamicSmemBytes = smem_bytes;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = 2;
-  attr.val.clusterDim.y = 1;
-  attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  int n = 0;
-  if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess) {
-    cudaGetLastError();
-    return 0;
-  }
-  cached[dev].store(n, std::memory_order_relaxed);
-  return n;
-}
-
 // Split-tile workspace of the CTA-pair kernel, one per (device, stream) so that kernels on
 // different streams never share tickets: fp32 partials for `kSplitMax` shared tiles x 2 CTAs
 // x 128 x 256 (a slot per cluster boundary, at most one per cluster), then per-warp tickets
@@ -241,6 +213,8 @@ int check_common(int64_t M, int64_t N, int64_t K) {
 }
 
 }  // namespace
+
+int gemm_max_ctas() { return g_max_ctas; }
 
 void gemm_invalidate_split_workspaces() { g_split_generation.fetch_add(1u, std::memory_order_acq_rel); }
 

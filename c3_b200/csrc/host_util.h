@@ -40,6 +40,10 @@ int require_sm100();
 int encode_bf16_2d_sw128(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols,
                          uint64_t ld, uint32_t box_cols, uint32_t box_rows);
 
+// The same for a row-major int8 matrix, with 128-byte swizzle (box_cols 128) or none.
+int encode_int8_2d(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_cols,
+                   uint32_t box_rows, bool swizzle);
+
 // Called by c3cu_fault_status when a kernel recorded a fault: a split-K GEMM whose adder gave
 // up waiting may leave its ticket and ready words non-zero (its partner publishes after the
 // adder has reset them), so every pooled split workspace is cleared again on its stream before
@@ -65,6 +69,37 @@ cudaError_t launch_kernel(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t 
   cfg.attrs = attr;
   cfg.numAttrs = pdl_enabled() ? 1 : 0;
   return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
+}
+
+// The calling thread's cap on persistent GEMM CTAs (c3cu_set_gemm_max_ctas; 0 = none).
+int gemm_max_ctas();
+
+// Co-resident clusters of two CTAs for a kernel (cached per device and kernel type).
+template <class Kern>
+int max_pair_clusters(Kern kern, uint32_t smem_bytes, int threads) {
+  static std::atomic<int> cached[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+  const int have = cached[dev].load(std::memory_order_relaxed);
+  if (have > 0) return have;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2 * 74, 1, 1);
+  cfg.blockDim = dim3(threads, 1, 1);
+  cfg.dynamicSmemBytes = smem_bytes;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = 2;
+  attr.val.clusterDim.y = 1;
+  attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  cached[dev].store(n, std::memory_order_relaxed);
+  return n;
 }
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0u; }

@@ -13,6 +13,8 @@ import torch
 
 from . import _lib
 
+INT8_MAX_K = 131071  # K * 128 * 128 stays inside int32
+
 _ws_cache: dict[tuple[int, int], torch.Tensor] = {}
 
 
@@ -68,6 +70,12 @@ def _require_rows(t: torch.Tensor, name: str, dtype: torch.dtype, rows: int, col
                                        f"got strides {t.stride()}")
     if not _device_ok(t):
         raise _lib.C3CUError(-1, name, "expected a CUDA tensor")
+
+
+def _ld(t: torch.Tensor) -> int:
+    """Row stride in elements, as the C ABI takes it. That of a single row means nothing to torch
+    (it may be anything): one that keeps the 16-byte rule is given instead."""
+    return t.stride(0) if t.shape[0] > 1 else (t.shape[1] + 15) // 16 * 16
 
 
 def workspace(device: torch.device, nbytes: int) -> torch.Tensor:
@@ -226,3 +234,79 @@ def gemm(A: torch.Tensor, B: torch.Tensor, a_mn: bool, b_mn: bool, epilogue: int
                                     _stream(A.device))
     _lib.check(rc, "c3cu_gemm_bf16")
     return out
+
+
+@_lib.on_tensor_device
+def forward_int8(Xq: torch.Tensor, x_scale: torch.Tensor, Wq: torch.Tensor, w_scale: torch.Tensor,
+                 b: torch.Tensor | None = None, relu: bool = True, out_dtype: torch.dtype = torch.bfloat16,
+                 Y: torch.Tensor | None = None, mask: torch.Tensor | None = None, save_mask: bool = True):
+    """The Linear forward on int8 operands with scales (quant.quantize_rows, norm.rms_norm_int8):
+    Y = (Xq Wq^T) * x_scale[m] * w_scale[n] + b[n], through max(., 0) with `relu`.
+
+    Xq [M, K] with x_scale [M] per token, Wq [N, K] with w_scale [N] per channel; rows start on 16
+    bytes (K <= 131071). Integer products and sums are exact; z = fl32(fl32(fl32(sum) *
+    fl32(x_scale * w_scale)) + b), so the result does not depend on the kernel that ran. Returns (Y,
+    mask): Y in `out_dtype` (bf16 or fp32), and with `relu` and `save_mask` the bit-packed ReLU mask
+    of `forward` (else None), from which `relu_mask_db` starts the backward pass."""
+    if Y is not None:
+        out_dtype = Y.dtype
+    if out_dtype not in (torch.bfloat16, torch.float32):
+        raise _lib.C3CUError(-1, "Y", f"Y must be float32 or bfloat16, got {out_dtype}")
+    for t, name in ((Xq, "Xq"), (Wq, "Wq")):
+        if not isinstance(t, torch.Tensor) or t.dim() != 2:
+            raise _lib.C3CUError(-1, name, "expected a 2-D int8 tensor")
+    M, K = Xq.shape
+    N = Wq.shape[0]
+    if not 1 <= K <= INT8_MAX_K:
+        raise _lib.C3CUError(-1, "Xq", f"K = {K} outside [1, {INT8_MAX_K}]")
+    _require_rows(Xq, "Xq", torch.int8, M, K)
+    _require_rows(Wq, "Wq", torch.int8, N, K)
+    _require(x_scale, "x_scale", torch.float32, 1, (M,))
+    _require(w_scale, "w_scale", torch.float32, 1, (N,))
+    if b is not None:
+        _require(b, "b", torch.float32, 1, (N,))
+    if Y is None:
+        Y = torch.empty((M, N), dtype=out_dtype, device=Xq.device)
+    else:
+        _require_rows(Y, "Y", out_dtype, M, N)
+    if mask is not None:
+        if not (relu and save_mask):
+            raise _lib.C3CUError(-1, "mask", "a mask belongs to the ReLU output (relu and save_mask)")
+        _require_rows(mask, "mask", torch.int32, M, mask_words(N))
+    elif relu and save_mask:
+        mask = torch.empty((M, mask_words(N)), dtype=torch.int32, device=Xq.device)
+    rc = _lib.load().c3cu_linear_int8_fwd(_p(Xq), _ld(Xq), _p(x_scale), _p(Wq), _ld(Wq), _p(w_scale), _p(b), _p(Y),
+                                          _ld(Y), _lib.DTYPE_F32 if out_dtype == torch.float32 else _lib.DTYPE_BF16,
+                                          1 if relu else 0, _p(mask), 0 if mask is None else _ld(mask), M, N, K,
+                                          _stream(Xq.device))
+    _lib.check(rc, "c3cu_linear_int8_fwd")
+    return Y, mask
+
+
+@_lib.on_tensor_device
+def grad_weight_int8(dZ: torch.Tensor, Xq: torch.Tensor, x_scale: torch.Tensor, dW: torch.Tensor | None = None):
+    """dW = dZ^T (Xq * x_scale) as bf16 [N, K]: `grad_weight` ("nk") with the layer's input kept in 8
+    bits (quant.quantize_rows of a bf16 activation, or the int8 rows that went into forward_int8).
+
+    dZ [M, N] bf16 and Xq [M, K] int8, rows starting on 16 bytes. Accumulation is fp32; Xq * x_scale
+    is rounded to bf16 on its way into the tensor cores."""
+    for t, name in ((dZ, "dZ"), (Xq, "Xq")):
+        if not isinstance(t, torch.Tensor) or t.dim() != 2:
+            raise _lib.C3CUError(-1, name, "expected a 2-D tensor")
+    M, N = dZ.shape
+    K = Xq.shape[1]
+    _require_rows(dZ, "dZ", torch.bfloat16, M, N)
+    _require_rows(Xq, "Xq", torch.int8, M, K)
+    _require(x_scale, "x_scale", torch.float32, 1, (M,))
+    if dW is None:
+        dW = torch.empty((N, K), dtype=torch.bfloat16, device=dZ.device)
+    else:
+        _require_rows(dW, "dW", torch.bfloat16, N, K)
+    L = _lib.load()
+    nb = L.c3cu_gemm_dw_int8_workspace(M, N, K)
+    # of this call alone: a graph that captures it keeps its own
+    ws = torch.empty(nb, dtype=torch.uint8, device=dZ.device) if nb else None
+    rc = L.c3cu_gemm_dw_int8(_p(dZ), _ld(dZ), _p(Xq), _ld(Xq), _p(x_scale), _p(dW), _ld(dW), M, N, K, _p(ws), nb,
+                             _stream(dZ.device))
+    _lib.check(rc, "c3cu_gemm_dw_int8")
+    return dW

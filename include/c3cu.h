@@ -271,6 +271,55 @@ int c3cu_flash_attn_fwd(const void* Q, const void* K, const void* V, void* O, fl
  * the two tiles' softmax warps taking turns at their exponentials (experimental). */
 int c3cu_set_attn_variant(int variant);
 
+/* ------------------------------------------------------------------ 8-bit activations
+ * A matrix of activations (or weights) held as int8 rows with one fp32 scale each:
+ * x[m][k] ~ q[m][k] * scale[m]. No reference counterpart: the reference computes in fp32.
+ * "ld" arguments are row strides in elements (ignored by M == 1, except that the int8 and dZ
+ * operands of the two GEMMs follow the TMA rule: base and row stride multiples of 16 bytes).
+ *
+ * q[m][k] = the integer nearest to 127 x[m][k] / A, ties to even, A = max_k |x[m][k]|;
+ * scale[m] = A / 127. The rounding is that of the real quotient, whatever the launch. A row of
+ * zeros has scale 0; a row that holds an infinity or a NaN has q = 0 and scale NaN, so all that
+ * is computed from it is NaN. dtype: of X, C3CU_DTYPE_F32 or C3CU_DTYPE_BF16. K >= 1. */
+int c3cu_quantize_rows(const void* X, int64_t ldx, int dtype, int8_t* Q, int64_t ldq, float* scale, int64_t M,
+                       int64_t K, c3cu_stream_t stream);
+/* RMS norm with the residual's addition and the output in that form:
+ *   h = x + r (rounded to dtype; r and H may be NULL together: then h is x),
+ *   rstd = 1 / sqrt(mean_k h^2 + eps), y = h * rstd * weight,
+ *   q = nearest integer to 127 a / A with a = fl32(h * weight), A = max_k |a|; scale = A rstd / 127.
+ * Squares are summed in fp32 (|h| up to about 1e18). H may be X or R itself (same stride). */
+int c3cu_rms_norm_int8(const void* X, int64_t ldx, const void* R, int64_t ldr, int dtype, const float* weight,
+                       float eps, void* H, int64_t ldh, int8_t* Q, int64_t ldq, float* scale, float* rstd, int64_t M,
+                       int64_t K, c3cu_stream_t stream);
+/* The norm's gradients, the rounding to int8 taken as the identity: with g = weight dy and
+ * xhat = h rstd,  dx = rstd (g - xhat mean_k(g xhat)) + dh  (dh: the gradient that reaches h
+ * past the norm, NULL for none; dx is the gradient of x and of the residual alike) and
+ * dweight[k] = sum_m dy xhat (fp32, the same bits from every run). dY, H, dH, dX of one dtype;
+ * dX may be dY, H or dH itself (same stride). Workspace: c3cu_rms_norm_bwd_workspace(M, K)
+ * bytes of device memory (4-byte aligned) that no other call uses meanwhile. */
+size_t c3cu_rms_norm_bwd_workspace(int64_t M, int64_t K);
+int c3cu_rms_norm_bwd(const void* dY, int64_t ldy, const void* H, int64_t ldh, const void* dH, int64_t lddh, int dtype,
+                      const float* weight, const float* rstd, void* dX, int64_t lddx, float* dweight, int64_t M,
+                      int64_t K, void* workspace, size_t workspace_bytes, c3cu_stream_t stream);
+/* Linear forward on int8 rows: z = fl(fl(float(sum_k X[m][k] W[n][k]) * fl(x_scale[m] w_scale[n])) + bias[n])
+ * with the integer sum exact and each fl an fp32 rounding; Y[m][n] = z, or max(z, 0) with relu
+ * (a NaN stays), in out_dtype (C3CU_DTYPE_BF16 or C3CU_DTYPE_F32). W: [N][K]. bias may be NULL.
+ * mask (relu only, may be NULL): as in c3cu_linear_bias_relu_fwd, row stride ldm words.
+ * K <= C3CU_INT8_MAX_K, where int32 sums cannot overflow. */
+#define C3CU_INT8_MAX_K 131071
+int c3cu_linear_int8_fwd(const int8_t* X, int64_t ldx, const float* x_scale, const int8_t* W, int64_t ldw,
+                         const float* w_scale, const float* bias, void* Y, int64_t ldy, int out_dtype, int relu,
+                         uint32_t* mask, int64_t ldm, int64_t M, int64_t N, int64_t K, c3cu_stream_t stream);
+/* dW[N][K] = sum_m dZ[m][n] (X[m][k] x_scale[m]) as bf16: the weight gradient from an 8-bit
+ * checkpoint of the layer's input (fp32 accumulation; X x_scale is rounded to bf16 on its way
+ * into the tensor cores). dZ [M][N] bf16. Workspace: c3cu_gemm_dw_int8_workspace(M, N, K) bytes
+ * of device memory (16-byte aligned) that no other call uses meanwhile; the size depends on the
+ * calling thread's c3cu_set_gemm_max_ctas. */
+size_t c3cu_gemm_dw_int8_workspace(int64_t M, int64_t N, int64_t K);
+int c3cu_gemm_dw_int8(const void* dZ, int64_t lddz, const int8_t* X, int64_t ldx, const float* x_scale, void* dW,
+                      int64_t lddw, int64_t M, int64_t N, int64_t K, void* workspace, size_t workspace_bytes,
+                      c3cu_stream_t stream);
+
 /* ------------------------------------------------------------------ fused dW GEMM + all-reduce
  * The data-parallel backward's exchange step fused into the dW GEMM that produces it (replaces
  * the dW graph of MatMul backward, src/C3/C3BackwardCapture.cpp:681-723, followed by a sum over
