@@ -10,6 +10,8 @@ import re
 import threading
 from pathlib import Path
 
+import torch
+
 PKG = Path(__file__).resolve().parent
 LIB_PATH = PKG / "libc3cu.so"
 HEADERS = [PKG.parent / "include" / "c3cu.h"]
@@ -107,6 +109,8 @@ def declared_symbols() -> list[str]:
 
 def load(build_if_missing: bool = True) -> ctypes.CDLL:
     global _lib
+    if _lib is not None:  # set once, under the lock
+        return _lib
     with _lock:
         if _lib is not None:
             return _lib
@@ -147,14 +151,21 @@ def fault_status() -> int:
     return code.value
 
 
-def _cuda_devices(values, found: set) -> None:
-    import torch
+def _cuda_device(values, found: int) -> int:
+    """The CUDA device of the tensors in `values` (lists and tuples are looked into), -1 for none, -2 for
+    several; `found` is what earlier values gave."""
     for v in values:
         if isinstance(v, torch.Tensor):
-            if v.is_cuda:
-                found.add(v.device.index)
+            idx = v.get_device()  # -1 on the CPU
+            if idx != found and idx >= 0:
+                if found != -1:
+                    return -2
+                found = idx
         elif isinstance(v, (list, tuple)):
-            _cuda_devices(v, found)
+            found = _cuda_device(v, found)
+            if found == -2:
+                return -2
+    return found
 
 
 def on_tensor_device(fn):
@@ -162,18 +173,18 @@ def on_tensor_device(fn):
     launches on the current device with that device's stream, so the call is made with the
     tensors' device current (as torch ops do). Tensors on different devices are refused before
     any launch: a kernel reading another GPU's memory without peer access would fault."""
+    current = torch.cuda.current_device
+
     @functools.wraps(fn)
     def wrapper(*args, **kwargs):
-        import torch
-        found: set = set()
-        _cuda_devices(args, found)
-        _cuda_devices(kwargs.values(), found)
-        if not found:
+        idx = _cuda_device(args, -1)
+        if kwargs and idx != -2:
+            idx = _cuda_device(kwargs.values(), idx)
+        if idx == -1:
             return fn(*args, **kwargs)
-        if len(found) > 1:
-            raise C3CUError(-1, fn.__name__, f"tensors on different devices: cuda:{sorted(found)}")
-        idx = found.pop()
-        if idx == torch.cuda.current_device():  # the common case: no device switch
+        if idx == -2:
+            raise C3CUError(-1, fn.__name__, "tensors on different devices")
+        if idx == current():  # the common case: no device switch
             return fn(*args, **kwargs)
         with torch.cuda.device(idx):
             return fn(*args, **kwargs)

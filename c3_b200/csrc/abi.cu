@@ -22,6 +22,8 @@ int c3cu_fault_get_train(uint32_t* out);
 int c3cu_fault_clear_train();
 int c3cu_fault_get_int8(uint32_t* out);
 int c3cu_fault_clear_int8();
+int c3cu_fault_get_quant(uint32_t* out);
+int c3cu_fault_clear_quant();
 
 namespace c3cu {
 
@@ -176,10 +178,11 @@ int c3cu_fault_status(uint32_t* code) {
   *code = 0u;
   int rc = c3cu::cuda_status(cudaDeviceSynchronize(), "c3cu_fault_status: synchronize");
   if (rc != C3CU_OK) return rc;
-  uint32_t words[6] = {0u, 0u, 0u, 0u, 0u, 0u};
+  uint32_t words[7] = {0u, 0u, 0u, 0u, 0u, 0u, 0u};
   if (c3cu_fault_get_gemm(&words[0]) || c3cu_fault_get_ew(&words[1]) ||
       c3cu_fault_get_attn(&words[2]) || c3cu_fault_get_nvls(&words[3]) ||
-      c3cu_fault_get_train(&words[4]) || c3cu_fault_get_int8(&words[5])) {
+      c3cu_fault_get_train(&words[4]) || c3cu_fault_get_int8(&words[5]) ||
+      c3cu_fault_get_quant(&words[6])) {
     c3cu::set_error("c3cu_fault_status: reading fault words failed");
     return C3CU_ERR_CUDA;
   }
@@ -191,6 +194,7 @@ int c3cu_fault_status(uint32_t* code) {
   c3cu_fault_clear_nvls();
   c3cu_fault_clear_train();
   c3cu_fault_clear_int8();
+  c3cu_fault_clear_quant();
   if (*code != 0u) {
     c3cu::gemm_invalidate_split_workspaces();
     c3cu::set_error("kernel fault recorded: code %u (site %u)", *code & 0xffffu, *code >> 16);

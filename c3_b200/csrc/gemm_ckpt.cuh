@@ -3,16 +3,21 @@
 //   dW[N][K] = sum_m dZ[m][n] * (q[m][k] * scale[m])        (bf16 out, fp32 sums in TMEM)
 //
 // dZ is bf16, X is held as int8 rows with one fp32 scale each (c3cu_quantize_rows). The scale runs
-// along the sum, so it cannot wait for the epilogue: q * scale is formed in the kernel and rounded
-// to bf16, the tensor cores' operand type. That rounding (relative 2^-8 at most, the size of the
+// along the sum, so it cannot wait for the epilogue: q * scale is rounded to bf16, the tensor
+// cores' operand type, on its way to them. That rounding (relative 2^-8 at most, the size of the
 // output's own) is the only one besides the output's; q itself would be exact in bf16.
 //
-// The structure is gemm2_kernel's (256 x 256 tiles on CTA pairs, both operands MN-major, since dZ
-// and X are stored with the sum's index as their rows) with one more role: TMA brings X's int8
-// block into a raw buffer, and four converter warps widen it into the swizzled bf16 tile that the
-// MMA reads. So X crosses HBM and L2 at one byte per element and no bf16 copy of it exists.
+// dw_kernel has gemm2_kernel's structure (256 x 256 tiles on CTA pairs, both operands MN-major,
+// since dZ and X are stored with the sum's index as their rows), in two forms:
+//   RAW   TMA brings X's int8 block into a raw buffer and converter warps widen it into the
+//         swizzled bf16 tile that the MMA reads: X crosses HBM and L2 at one byte per element and
+//         no bf16 copy of it exists, but it is widened once for every 256 rows of dW.
+//   !RAW  X was widened once into a bf16 workspace (widen_kernel), which the kernel reads by TMA.
+// The widening in the kernel costs more than its instructions: beside the tensor cores it runs
+// into the power limit. XXX
 //
-// Warps: 0 TMA, 1 MMA (leader), 2..9 epilogue, 10..13 converters.
+// Warps: 0 TMA, 1 MMA (leader), 2..9 epilogue; RAW: 10..17 converters (two groups of four), 18 TMA
+// of X.
 #pragma once
 
 #include "ckpt_schedule.h"
@@ -33,14 +38,25 @@ using gemm2::TM;
 using gemm2::TMEM_COLS;
 using gemm2::TN;
 using gemm2::UMMA_K;
-constexpr int STAGES = 5;
-constexpr int kConvWarps = 4;
-constexpr int kThreads = 64 + 32 * (kEpiWarps + kConvWarps);
+constexpr int kConvWarps = 4;   // a group's warps
+constexpr int kConvGroups = 2;  // the groups take K blocks in turn
+constexpr int kRawWarp = 2 + kEpiWarps + kConvGroups * kConvWarps;
 constexpr uint32_t RAW_BYTES = BK * HN;  // 64 rows (m) of 128 int8 (k)
-constexpr uint32_t STAGE_BYTES = A_STAGE_BYTES + B_STAGE_BYTES + RAW_BYTES;
-constexpr uint32_t BAR_BYTES = (3 * STAGES + 5) * 8 + 8;
-constexpr uint32_t SMEM_BYTES = STAGES * STAGE_BYTES + BAR_BYTES + 1024;
-static_assert(SMEM_BYTES <= 227 * 1024, "shared memory");
+
+// Ring depths. RAW: dZ, raw int8 and widened tiles go through rings of their own, so that the
+// loads' latency and the conversion's are each hidden by as many stages as they take. !RAW: one
+// ring of both operands' stages.
+template <bool RAW>
+struct Ring {
+  static constexpr int kA = RAW ? 5 : 7;
+  static constexpr int kB = RAW ? 4 : 7;
+  static constexpr int kRaw = RAW ? 8 : 0;
+  static constexpr int kThreads = RAW ? 32 * (kRawWarp + 1) : 32 * (2 + kEpiWarps);
+  static constexpr uint32_t kBytes = kA * A_STAGE_BYTES + kB * B_STAGE_BYTES + kRaw * RAW_BYTES;
+  static constexpr uint32_t kSmem = kBytes + 2 * (kA + kB + kRaw) * 8 + 5 * 8 + 8 + 1024;
+  static_assert(kSmem <= 227 * 1024, "shared memory");
+  static_assert(kB % kConvGroups == 0 || !RAW, "a stage belongs to one group, which so sees each of its phases");
+};
 
 struct Params {
   int32_t M, N, K;     // dW is N x K, the sum runs over M
@@ -52,38 +68,76 @@ struct Params {
   Plan plan;
 };
 
-// Four int8 in a word -> fp32: the bytes, biased to unsigned, become the low mantissa bits of 2^23.
-__device__ __forceinline__ void widen4(uint32_t w, float (&f)[4]) {
-  w ^= 0x80808080u;
-  constexpr float kBias = 8388608.f + 128.f;
-  f[0] = __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440)) - kBias;
-  f[1] = __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7441)) - kBias;
-  f[2] = __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7442)) - kBias;
-  f[3] = __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7443)) - kBias;
+// A row's scale as two bf16 pairs: s = head + tail to 16 bits (both truncated).
+struct Scale2 {
+  __nv_bfloat162 head, tail;
+};
+
+__device__ __forceinline__ __nv_bfloat162 both_halves(float v) {  // v's upper 16 bits, twice
+  const uint32_t b = __byte_perm(__float_as_uint(v), 0u, 0x3232);
+  return *reinterpret_cast<const __nv_bfloat162*>(&b);
 }
 
-// Eight int8 (two words) times s, as one 16-byte piece of bf16.
-__device__ __forceinline__ uint4 scale8(uint32_t w0, uint32_t w1, float s) {
-  float a[4], b[4];
-  widen4(w0, a);
-  widen4(w1, b);
-  return make_uint4(pack_bf16x2(a[0] * s, a[1] * s), pack_bf16x2(a[2] * s, a[3] * s),
-                    pack_bf16x2(b[0] * s, b[1] * s), pack_bf16x2(b[2] * s, b[3] * s));
+__device__ __forceinline__ Scale2 split_scale(float s) {
+  const float head = __uint_as_float(__float_as_uint(s) & 0xffff0000u);
+  return {both_halves(s), both_halves(s - head)};
 }
 
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+// The two int8 in bits 0..7 and 16..23 of w, times the scale, as two bf16 (packed conversions
+// from fp32 run at a fraction of this rate). 0x4300 is 128 in bf16, with one as its last place:
+// or-ing the low seven bits gives 128 + low7, or-ing the sign bit 128 or 256, and the difference
+// is the int8, exactly. q * tail is rounded at 2^-8 of a number 2^-8 of the result, then one fused
+// multiply-add rounds the result, so it is q * s rounded to bf16 to within 2^-16; zero stays zero.
+__device__ __forceinline__ uint32_t scale_pair(uint32_t w, const Scale2& s) {
+  const uint32_t a = (w & 0x007f007fu) | 0x43004300u;
+  const uint32_t b = (w & 0x00800080u) | 0x43004300u;
+  const __nv_bfloat162 q = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a),
+                                   *reinterpret_cast<const __nv_bfloat162*>(&b));
+  const __nv_bfloat162 x = __hfma2(q, s.head, __hmul2(q, s.tail));
+  return *reinterpret_cast<const uint32_t*>(&x);
+}
+
+// Eight int8 (two words) times s, as one 16-byte piece of bf16. The middle two of each four trade
+// places (the pairs are bytes 0, 2 and 1, 3 of a word); the epilogue trades them back, where it
+// costs nothing.
+__device__ __forceinline__ uint4 scale8(uint32_t w0, uint32_t w1, const Scale2& s) {
+  return make_uint4(scale_pair(w0, s), scale_pair(w0 >> 8, s), scale_pair(w1, s), scale_pair(w1 >> 8, s));
+}
+
+__device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+
+__device__ __forceinline__ void st_shared_v4(uint32_t addr, const uint4& v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
+// Counts an arrival on a barrier of the leader CTA. The writes it publishes were made visible to
+// the async proxy, which alone reads them, by the writers' proxy fences; a release at cluster
+// scope stalled the warp for a round trip to memory (16384 x 4096 x 4096: 743 us, 527 without).
+__device__ __forceinline__ void arrive_leader(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(mapa_shared(smem_u32(bar), 0u)) : "memory");
+}
+
+template <bool RAW>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Ring<RAW>::kThreads, 1)
     dw_kernel(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CUtensorMap tmx, const Params p) {
+  constexpr int A_STAGES = Ring<RAW>::kA, B_STAGES = Ring<RAW>::kB, RAW_STAGES = Ring<RAW>::kRaw;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
   uint8_t* sA = smem;
-  uint8_t* sB = sA + STAGES * A_STAGE_BYTES;
-  uint8_t* sRaw = sB + STAGES * B_STAGE_BYTES;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE_BYTES);
-  uint64_t* full = bars;                   // A landed and B converted, in both CTAs (leader's is used)
-  uint64_t* empty = full + STAGES;
-  uint64_t* raw_full = empty + STAGES;     // this CTA's raw block landed
-  uint64_t* acc_full = raw_full + STAGES;
+  uint8_t* sB = sA + A_STAGES * A_STAGE_BYTES;
+  uint8_t* sRaw = sB + B_STAGES * B_STAGE_BYTES;
+  uint64_t* a_full = reinterpret_cast<uint64_t*>(smem + Ring<RAW>::kBytes);  // loads of both CTAs (the leader's is used)
+  uint64_t* a_empty = a_full + A_STAGES;
+  uint64_t* b_full = a_empty + A_STAGES;      // RAW: widened, in both CTAs (the leader's is used)
+  uint64_t* b_empty = b_full + B_STAGES;
+  uint64_t* raw_full = b_empty + B_STAGES;    // this CTA's int8 block landed
+  uint64_t* raw_empty = raw_full + RAW_STAGES;
+  uint64_t* acc_full = raw_empty + RAW_STAGES;
   uint64_t* acc_empty = acc_full + 2;
   uint64_t* drain = acc_empty + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
@@ -99,10 +153,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const int items = item_count(p.plan);
 
   if (warp == 0 && lane == 0) {
-    for (int s = 0; s < STAGES; ++s) {
-      mbar_init(&full[s], 1 + 2 * kConvWarps);
-      mbar_init(&empty[s], 1);
+    for (int s = 0; s < A_STAGES; ++s) {
+      mbar_init(&a_full[s], 1);
+      mbar_init(&a_empty[s], 1);
+    }
+    for (int s = 0; s < B_STAGES; ++s) {
+      mbar_init(&b_full[s], 2 * kConvWarps);
+      mbar_init(&b_empty[s], 1);
+    }
+    for (int s = 0; s < RAW_STAGES; ++s) {
       mbar_init(&raw_full[s], 1);
+      mbar_init(&raw_empty[s], kConvWarps);
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&acc_full[a], 1);
@@ -133,26 +194,56 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       for (int i = cluster; ok && i < items; i += num_clusters) {
         const Item it = item_at(p.plan, i, blocks);
         const int n0 = (it.tile / k_tiles) * TM + static_cast<int>(rank) * HM;
-        const int k0 = (it.tile % k_tiles) * TN + static_cast<int>(rank) * HN;
+        [[maybe_unused]] const int k0 = (it.tile % k_tiles) * TN + static_cast<int>(rank) * HN;
         for (int kb = it.kb0; kb < it.kb1; ++kb) {
-          if (!mbar_wait(&empty[s], ph ^ 1u, kFaultWaitEmpty)) { ok = false; break; }
-          mbar_arrive_expect_tx(&raw_full[s], RAW_BYTES);
-          tma_load_2d(sRaw + s * RAW_BYTES, &tmx, &raw_full[s], k0, kb * BK);
-          if (leader) mbar_arrive_expect_tx(&full[s], 2u * A_STAGE_BYTES);
-          const uint32_t bar_leader = mapa_shared(smem_u32(&full[s]), 0u);
+          if (!mbar_wait(&a_empty[s], ph ^ 1u, kFaultWaitEmpty)) { ok = false; break; }
+          if (leader) mbar_arrive_expect_tx(&a_full[s], 2u * (A_STAGE_BYTES + (RAW ? 0u : B_STAGE_BYTES)));
+          const uint32_t bar_leader = mapa_shared(smem_u32(&a_full[s]), 0u);
           uint8_t* sa = sA + s * A_STAGE_BYTES;
 #pragma unroll
           for (int j = 0; j < HM / 64; ++j)
             tma_load_2d_pair(sa + j * MN_CHUNK_BYTES, &tma, bar_leader, n0 + 64 * j, kb * BK);
+          if constexpr (!RAW) {
+            uint8_t* sb = sB + s * B_STAGE_BYTES;
+#pragma unroll
+            for (int j = 0; j < HN / 64; ++j)
+              tma_load_2d_pair(sb + j * MN_CHUNK_BYTES, &tmx, bar_leader, k0 + 64 * j, kb * BK);
+          }
           armed |= 1u << s;
           armed_par = (armed_par & ~(1u << s)) | (ph << s);
-          if (++s == STAGES) { s = 0; ph ^= 1u; }
+          if (++s == A_STAGES) { s = 0; ph ^= 1u; }
         }
       }
-      if (!ok) {
-        for (int t = 0; t < STAGES; ++t)
-          if (armed & (1u << t)) gemm::drain_wait(&raw_full[t], (armed_par >> t) & 1u);
+      if (!ok || fault_raised()) {
+        if (leader) {
+          for (int t = 0; t < A_STAGES; ++t)
+            if (armed & (1u << t)) gemm::drain_wait(&a_full[t], (armed_par >> t) & 1u);
+        }
         gemm2::settle_inflight_copies();
+      }
+    }
+    __syncwarp();
+  } else if (RAW && warp == kRawWarp) {
+    // ------------------------------------------------------------ TMA producer of the int8 blocks
+    if constexpr (RAW) if (lane == 0) {
+      int s = 0;
+      uint32_t ph = 0, armed = 0u, armed_par = 0u;
+      bool ok = true;
+      for (int i = cluster; ok && i < items; i += num_clusters) {
+        const Item it = item_at(p.plan, i, blocks);
+        const int k0 = (it.tile % k_tiles) * TN + static_cast<int>(rank) * HN;
+        for (int kb = it.kb0; kb < it.kb1; ++kb) {
+          if (!mbar_wait(&raw_empty[s], ph ^ 1u, kFaultWaitEmpty)) { ok = false; break; }
+          mbar_arrive_expect_tx(&raw_full[s], RAW_BYTES);
+          tma_load_2d(sRaw + s * RAW_BYTES, &tmx, &raw_full[s], k0, kb * BK);
+          armed |= 1u << s;
+          armed_par = (armed_par & ~(1u << s)) | (ph << s);
+          if (++s == RAW_STAGES) { s = 0; ph ^= 1u; }
+        }
+      }
+      if (!ok || fault_raised()) {
+        for (int t = 0; t < RAW_STAGES; ++t)
+          if (armed & (1u << t)) gemm::drain_wait(&raw_full[t], (armed_par >> t) & 1u);
       }
     }
     __syncwarp();
@@ -160,8 +251,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     // ------------------------------------------------------------ MMA issuer (leader only)
     if (leader && lane == 0) {
       constexpr uint32_t IDESC = make_idesc_bf16_f32(TM, TN, true, true);
-      int s = 0;
-      uint32_t ph = 0, acc = 0, acc_ph = 0;
+      int sa = 0, sb = 0;
+      uint32_t pa = 0, pb = 0, acc = 0, acc_ph = 0;
       bool ok = true;
       for (int i = cluster; ok && i < items; i += num_clusters) {
         const Item it = item_at(p.plan, i, blocks);
@@ -169,17 +260,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + acc * TN;
         for (int kb = it.kb0; kb < it.kb1; ++kb) {
-          if (!mbar_wait(&full[s], ph, kFaultWaitFull)) { ok = false; break; }
+          if (!mbar_wait(&a_full[sa], pa, kFaultWaitFull) ||
+              (RAW && !mbar_wait(&b_full[sb], pb, kFaultWaitFull))) {
+            ok = false;
+            break;
+          }
           tc_fence_after();
-          const uint32_t a_addr = smem_u32(sA + s * A_STAGE_BYTES);
-          const uint32_t b_addr = smem_u32(sB + s * B_STAGE_BYTES);
+          const uint32_t a_addr = smem_u32(sA + sa * A_STAGE_BYTES);
+          const uint32_t b_addr = smem_u32(sB + sb * B_STAGE_BYTES);
 #pragma unroll
           for (int kk = 0; kk < BK / UMMA_K; ++kk)
             umma_f16_ss_pair(d_tmem, make_sw128_desc(a_addr + kk * UMMA_K * 128, MN_CHUNK_BYTES, 1024),
                              make_sw128_desc(b_addr + kk * UMMA_K * 128, MN_CHUNK_BYTES, 1024), IDESC,
                              (kb != it.kb0 || kk != 0) ? 1u : 0u);
-          umma_commit_pair_mc(&empty[s], kPairMask);
-          if (++s == STAGES) { s = 0; ph ^= 1u; }
+          if constexpr (RAW) umma_commit_pair_mc(&b_empty[sb], kPairMask);
+          umma_commit_pair_mc(&a_empty[sa], kPairMask);
+          if (++sa == A_STAGES) { sa = 0; pa ^= 1u; }
+          if (++sb == B_STAGES) { sb = 0; pb ^= 1u; }
         }
         if (!ok) break;
         umma_commit_pair_mc(&acc_full[acc], kPairMask);
@@ -216,6 +313,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         uint32_t r[32];
         tmem_ld_32x32b_x32(t_row + c * 32, r);
         tmem_wait_ld();
+#pragma unroll
+        for (int j = 0; RAW && j < 32; j += 4) {  // the converters' order of columns (scale8)
+          const uint32_t t = r[j + 1];
+          r[j + 1] = r[j + 2];
+          r[j + 2] = t;
+        }
         if (it.slot < 0) {
           gemm::epilogue_chunk<kEpiStoreBf16>(g, r, row, col0);
         } else if (row < p.N) {
@@ -233,55 +336,66 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       acc ^= 1u;
       if (acc == 0u) acc_ph ^= 1u;
     }
-  } else {
-    // ------------------------------------------------------------ converters (warps 10..13)
-    // A warp takes 16 of the block's 64 rows, four at a time: lane = 8 * row + u reads the 16
-    // int8 of unit u of its row and writes two 16-byte pieces of the swizzled bf16 tile: chunk
-    // u / 4 (64 columns), pieces 2u and 2u + 1 of 8, at position piece ^ (row mod 8). Units 4..7
-    // write their odd piece first, so that the eight lanes of a row touch all banks once.
+  } else if constexpr (RAW) {
+    // ------------------------------------------------------------ converters (warps 10..17)
+    // The two groups of four warps take K blocks in turn. A warp takes 16 of the block's 64 rows,
+    // four at a time: lane = 8 * row + u reads the 16 int8 of unit u of its row and writes two
+    // 16-byte pieces of the swizzled bf16 tile: chunk u / 4 (64 columns), pieces 2u and 2u + 1 of
+    // 8, at position piece ^ (row mod 8). Units 4..7 write their odd piece first, so that the
+    // eight lanes of a row touch all banks once.
     const int cw = static_cast<int>(warp) - 2 - kEpiWarps;
+    const int group = cw / kConvWarps;
     const int u = static_cast<int>(lane & 7u);
-    const int r0 = cw * 16 + static_cast<int>(lane >> 3);
-    int s = 0;
-    uint32_t ph = 0;
+    const int r0 = (cw % kConvWarps) * 16 + static_cast<int>(lane >> 3);
+    const bool swap = u >= 4;
+    const uint32_t from = smem_u32(sRaw) + static_cast<uint32_t>(r0 * HN + u * 16);
+    const uint32_t piece = static_cast<uint32_t>(((2 * u) & 7) | (swap ? 1 : 0));
+    const uint32_t to = smem_u32(sB) + static_cast<uint32_t>((u >> 2) * MN_CHUNK_BYTES + r0 * 128);
+    // rows r0, r0 + 4, ...: the row modulo 8 alternates between lane / 8 and that plus 4
+    const uint32_t at = ((piece ^ (lane >> 3)) << 4);
+    int turn = 0;  // K blocks of earlier items, modulo the groups
+    uint32_t sr = group, sb = group, pr = 0, pb = 0;
     bool ok = true;
     for (int i = cluster; ok && i < items; i += num_clusters) {
       const Item it = item_at(p.plan, i, blocks);
+      const int first = it.kb0 + (group - turn + kConvGroups) % kConvGroups;
+      turn = (turn + it.kb1 - it.kb0) % kConvGroups;
       float next[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int m = it.kb0 * BK + r0 + 4 * j;
+        const int m = first * BK + r0 + 4 * j;
         next[j] = m < p.M ? __ldg(p.scale + m) : 0.f;
       }
-      for (int kb = it.kb0; kb < it.kb1; ++kb) {
-        float sc[4];
+      for (int kb = first; kb < it.kb1; kb += kConvGroups) {
+        if (!mbar_wait(&raw_full[sr], pr, kFaultWaitFull)) { ok = false; break; }
+        uint4 w[4], o[8];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = ld_shared_v4(from + sr * RAW_BYTES + j * (4 * HN));
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&raw_empty[sr]);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          sc[j] = next[j];
-          const int m = (kb + 1) * BK + r0 + 4 * j;
-          next[j] = kb + 1 < it.kb1 && m < p.M ? __ldg(p.scale + m) : 0.f;
+          const Scale2 sc = split_scale(next[j]);
+          const int m = (kb + kConvGroups) * BK + r0 + 4 * j;
+          next[j] = m < p.M ? __ldg(p.scale + m) : 0.f;
+          o[2 * j] = scale8(swap ? w[j].z : w[j].x, swap ? w[j].w : w[j].y, sc);
+          o[2 * j + 1] = scale8(swap ? w[j].x : w[j].z, swap ? w[j].y : w[j].w, sc);
         }
-        if (!mbar_wait(&raw_full[s], ph, kFaultWaitFull)) { ok = false; break; }
-        const uint8_t* raw = sRaw + s * RAW_BYTES;
-        uint8_t* dst = sB + s * B_STAGE_BYTES + (u >> 2) * MN_CHUNK_BYTES;
-        uint4 w[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) w[j] = *reinterpret_cast<const uint4*>(raw + (r0 + 4 * j) * HN + u * 16);
+        // only now: the conversion runs while the MMAs still read the stage's last tile
+        if (!mbar_wait(&b_empty[sb], pb ^ 1u, kFaultWaitEmpty)) { ok = false; break; }
+        const uint32_t line = to + sb * B_STAGE_BYTES;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const int r = r0 + 4 * j;
-          const uint4 even = scale8(w[j].x, w[j].y, sc[j]);
-          const uint4 odd = scale8(w[j].z, w[j].w, sc[j]);
-          uint8_t* line = dst + r * 128;
-          const int pe = ((2 * u) & 7) ^ (r & 7), po = ((2 * u + 1) & 7) ^ (r & 7);
-          const bool swap = u >= 4;
-          *reinterpret_cast<uint4*>(line + (swap ? po : pe) * 16) = swap ? odd : even;
-          *reinterpret_cast<uint4*>(line + (swap ? pe : po) * 16) = swap ? even : odd;
+          st_shared_v4(line + (at ^ ((j & 1) ? 64u : 0u)) + j * 512, o[2 * j]);
+          st_shared_v4(line + (at ^ 16u ^ ((j & 1) ? 64u : 0u)) + j * 512, o[2 * j + 1]);
         }
         fence_proxy_async_shared();  // the MMA reads the tile through the async proxy
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&full[s]), 0u));
-        if (++s == STAGES) { s = 0; ph ^= 1u; }
+        if (lane == 0) arrive_leader(&b_full[sb]);
+        sr += kConvGroups;
+        if (sr >= RAW_STAGES) { sr -= RAW_STAGES; pr ^= 1u; }
+        sb += kConvGroups;
+        if (sb >= B_STAGES) { sb -= B_STAGES; pb ^= 1u; }
       }
     }
   }
@@ -291,6 +405,39 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc_pair(tmem_base, TMEM_COLS);
+  }
+}
+
+// X in bf16: out[m][k] = bf16(q * scale), rows of `ldo` elements (a multiple of 8, columns past K
+// zero). A thread takes 16 columns of a row.
+__global__ void __launch_bounds__(256) widen_kernel(const int8_t* __restrict__ q, int64_t ldq, const float* __restrict__ scale,
+                                                    __nv_bfloat16* __restrict__ out, int64_t ldo, int M, int K) {
+  const int units = static_cast<int>((ldo + 15) / 16);
+  const int64_t total = static_cast<int64_t>(M) * units;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total;
+       i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+    const int64_t m = i / units;
+    const int k = static_cast<int>(i - m * units) * 16;
+    const int8_t* from = q + m * ldq + k;
+    uint32_t w[4] = {0u, 0u, 0u, 0u};
+    if (k + 16 <= K) {
+      const uint4 v = __ldcs(reinterpret_cast<const uint4*>(from));
+      w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        if (k + j < K) w[j / 4] |= static_cast<uint32_t>(static_cast<uint8_t>(from[j])) << (8 * (j % 4));
+    }
+    const float s = __ldg(scale + m);
+    uint32_t o[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t x = w[j / 2] >> (16 * (j % 2));
+      o[j] = pack_bf16x2(static_cast<float>(static_cast<int8_t>(x)) * s, static_cast<float>(static_cast<int8_t>(x >> 8)) * s);
+    }
+    uint4* to = reinterpret_cast<uint4*>(out + m * ldo + k);
+    to[0] = make_uint4(o[0], o[1], o[2], o[3]);
+    if (k + 8 < ldo) to[1] = make_uint4(o[4], o[5], o[6], o[7]);
   }
 }
 
@@ -305,17 +452,19 @@ __global__ void __launch_bounds__(256) add_pieces_kernel(const Params p) {
   if (row0 >= p.N || col0 >= p.K) return;
   const float* part = p.partial + static_cast<size_t>(blockIdx.y) * p.plan.pieces * (TM * TN);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int c = warp * 4 + i;
-    float sum = 0.f;
-    if (row0 + lane < p.N && col0 + c < p.K) {
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+  if (row0 + lane < p.N) {
+    const int cols = min(4, p.K - col0 - warp * 4);
 #pragma unroll 4
-      for (int s = 0; s < p.plan.pieces; ++s)
-        sum += __ldcg(part + static_cast<size_t>(s) * (TM * TN) + (bc + c) * TM + br + lane);
+    for (int s = 0; s < p.plan.pieces; ++s) {
+      const float* from = part + static_cast<size_t>(s) * (TM * TN) + (bc + warp * 4) * TM + br + lane;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (i < cols) sum[i] += __ldcg(from + i * TM);
     }
-    t[c][lane] = sum;
   }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) t[warp * 4 + i][lane] = sum[i];
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < 4; ++i) {

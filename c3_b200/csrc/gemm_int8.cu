@@ -1,6 +1,7 @@
 // C-ABI entry points of the int8 GEMMs (include/c3cu.h): the Linear forward on int8 rows with
 // scales (igemm.cuh) and the weight gradient from an 8-bit checkpoint (gemm_ckpt.cuh).
 #include <atomic>
+#include <cstdlib>
 
 #include "gemm_ckpt.cuh"
 #include "host_util.h"
@@ -114,14 +115,51 @@ int check_gemm_sizes(const char* what, int64_t M, int64_t N, int64_t K) {
   return C3CU_OK;
 }
 
-ckpt::Plan dw_plan(int64_t M, int64_t N, int64_t K, int* clusters) {
-  *clusters = pair_clusters(ckpt::dw_kernel, ckpt::SMEM_BYTES, ckpt::kThreads);
-  const int64_t tiles = ((N + ckpt::TM - 1) / ckpt::TM) * ((K + ckpt::TN - 1) / ckpt::TN);
-  return ckpt::make_plan(static_cast<int>(tiles), *clusters, static_cast<int>((M + ckpt::BK - 1) / ckpt::BK));
+// How a weight gradient runs: X widened in the kernel (raw) or once into the workspace, the tiles'
+// plan, and the workspace's parts (partial sums first, then the widened X).
+struct DwRun {
+  bool raw;
+  int clusters;
+  ckpt::Plan plan;
+  size_t partial_bytes, wide_bytes;
+  int64_t wide_ld;
+};
+
+template <bool RAW>
+int dw_clusters(int* clusters) {
+  auto kern = ckpt::dw_kernel<RAW>;
+  static std::atomic<uint64_t> smem_set{0};
+  int rc = C3CU_OK;
+  if (sm_count() > 0)  // before the occupancy query, which depends on it
+    rc = set_max_dynamic_smem(reinterpret_cast<const void*>(kern), ckpt::Ring<RAW>::kSmem, smem_set,
+                              "gemm_dw_int8: set max dynamic shared memory");
+  *clusters = pair_clusters(kern, ckpt::Ring<RAW>::kSmem, ckpt::Ring<RAW>::kThreads);
+  return rc;
 }
 
-size_t dw_workspace(const ckpt::Plan& plan) {
-  return static_cast<size_t>(plan.rest) * plan.pieces * ckpt::TM * ckpt::TN * sizeof(float);
+int dw_run(int64_t M, int64_t N, int64_t K, DwRun* r) {
+  const int64_t tiles = ((N + ckpt::TM - 1) / ckpt::TM) * ((K + ckpt::TN - 1) / ckpt::TN);
+  const int blocks = static_cast<int>((M + ckpt::BK - 1) / ckpt::BK);
+  const char* e = getenv("DEV_RAW");
+  r->raw = e && e[0] == '1';
+  const int rc = r->raw ? dw_clusters<true>(&r->clusters) : dw_clusters<false>(&r->clusters);
+  r->plan = ckpt::make_plan(static_cast<int>(tiles), r->clusters, blocks);
+  r->partial_bytes = static_cast<size_t>(r->plan.rest) * r->plan.pieces * ckpt::TM * ckpt::TN * sizeof(float);
+  r->wide_ld = (K + 7) / 8 * 8;
+  r->wide_bytes = r->raw ? 0 : static_cast<size_t>(M) * r->wide_ld * 2;
+  return rc;
+}
+
+template <bool RAW>
+int launch_dw(const CUtensorMap& ta, const CUtensorMap& tx, const ckpt::Params& p, int clusters, cudaStream_t st) {
+  const int items = ckpt::item_count(p.plan);
+  if (items < clusters) clusters = items;
+  int rc = cuda_status(launch_kernel(ckpt::dw_kernel<RAW>, dim3(2 * clusters), dim3(ckpt::Ring<RAW>::kThreads),
+                                     ckpt::Ring<RAW>::kSmem, st, ta, tx, p),
+                       "gemm_dw_int8: launch");
+  if (rc != C3CU_OK || p.plan.rest == 0) return rc;
+  ckpt::add_pieces_kernel<<<dim3(64, p.plan.rest), 256, 0, st>>>(p);
+  return cuda_status(cudaGetLastError(), "gemm_dw_int8: launch");
 }
 
 }  // namespace
@@ -186,8 +224,9 @@ extern "C" int c3cu_linear_int8_fwd(const int8_t* X, int64_t ldx, const float* x
 extern "C" size_t c3cu_gemm_dw_int8_workspace(int64_t M, int64_t N, int64_t K) {
   using namespace c3cu;
   if (M < 1 || N < 1 || K < 1 || check_gemm_sizes("gemm_dw_int8", M, N, K) != C3CU_OK) return 0;
-  int clusters = 0;
-  return dw_workspace(dw_plan(M, N, K, &clusters));
+  DwRun r;
+  dw_run(M, N, K, &r);
+  return r.partial_bytes + r.wide_bytes;
 }
 
 extern "C" int c3cu_gemm_dw_int8(const void* dZ, int64_t lddz, const int8_t* X, int64_t ldx, const float* x_scale,
@@ -228,26 +267,25 @@ extern "C" int c3cu_gemm_dw_int8(const void* dZ, int64_t lddz, const int8_t* X, 
     set_error("gemm_dw_int8: dW is too large (N %lld, K %lld)", (long long)N, (long long)K);
     return C3CU_ERR_INVALID;
   }
-  int clusters = 0;
-  p.plan = dw_plan(M, N, K, &clusters);
-  const size_t need = dw_workspace(p.plan);
+  DwRun r;
+  if ((rc = dw_run(M, N, K, &r)) != C3CU_OK) return rc;
+  p.plan = r.plan;
+  const size_t need = r.partial_bytes + r.wide_bytes;
   if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace))) {
     set_error("gemm_dw_int8: workspace of %zu bytes (16-byte aligned), %zu needed", workspace ? workspace_bytes : 0, need);
     return C3CU_ERR_WORKSPACE;
   }
   CUtensorMap ta, tx;
   if ((rc = encode_bf16_2d_sw128(&ta, dZ, M, N, lddz, 64, ckpt::BK)) != C3CU_OK) return rc;
+  // X's rows are checked by the same rule in both forms
   if ((rc = encode_int8_2d(&tx, X, M, K, ldx, ckpt::HN, ckpt::BK, false)) != C3CU_OK) return rc;
-  static std::atomic<uint64_t> smem_set{0};
-  rc = set_max_dynamic_smem(reinterpret_cast<const void*>(ckpt::dw_kernel), ckpt::SMEM_BYTES, smem_set,
-                            "gemm_dw_int8: set max dynamic shared memory");
-  if (rc != C3CU_OK) return rc;
-  const int items = ckpt::item_count(p.plan);
-  if (items < clusters) clusters = items;
-  rc = cuda_status(launch_kernel(ckpt::dw_kernel, dim3(2 * clusters), dim3(ckpt::kThreads), ckpt::SMEM_BYTES, st, ta,
-                                 tx, p),
-                   "gemm_dw_int8: launch");
-  if (rc != C3CU_OK || p.plan.rest == 0) return rc;
-  ckpt::add_pieces_kernel<<<dim3(64, p.plan.rest), 256, 0, st>>>(p);
-  return cuda_status(cudaGetLastError(), "gemm_dw_int8: launch");
+  if (r.raw) return launch_dw<true>(ta, tx, p, r.clusters, st);
+  __nv_bfloat16* wide = reinterpret_cast<__nv_bfloat16*>(static_cast<uint8_t*>(workspace) + r.partial_bytes);
+  const int64_t units = M * ((r.wide_ld + 15) / 16);
+  const int64_t want = (units + 255) / 256, most = static_cast<int64_t>(sm_count()) * 8;
+  ckpt::widen_kernel<<<static_cast<unsigned>(want < most ? want : most), 256, 0, st>>>(
+      X, ldx, x_scale, wide, r.wide_ld, static_cast<int>(M), static_cast<int>(K));
+  if ((rc = cuda_status(cudaGetLastError(), "gemm_dw_int8: launch")) != C3CU_OK) return rc;
+  if ((rc = encode_bf16_2d_sw128(&tx, wide, M, K, r.wide_ld, 64, ckpt::BK)) != C3CU_OK) return rc;
+  return launch_dw<false>(ta, tx, p, r.clusters, st);
 }

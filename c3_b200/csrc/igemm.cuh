@@ -72,6 +72,29 @@ __device__ __forceinline__ float scaled(uint32_t acc, float xs, float ws) {
   return __fmul_rn(__int2float_rn(static_cast<int>(acc)), __fmul_rn(xs, ws));
 }
 
+__device__ __forceinline__ float relu_keep_nan(float z) {  // a NaN (a row that was not finite) stays one
+  float r;
+  asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(r) : "f"(z));
+  return r;
+}
+
+// Packed fp32 arithmetic: two elements per instruction, each rounded like its scalar form.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)));
+  return d;
+}
+
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)));
+  return d;
+}
+
 // 32 columns of one row of the output (pair kernel: a thread owns a row).
 template <bool F32, bool RELU>
 __device__ __forceinline__ void store_chunk(const Params& p, const uint32_t (&r)[32], int row, int col0, float xs) {
@@ -80,23 +103,20 @@ __device__ __forceinline__ void store_chunk(const Params& p, const uint32_t (&r)
   const bool full = p.vec_ok && ncols == 32;
   float z[32];
   if (full) {
+    const float2 xs2 = make_float2(xs, xs);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const float4 w = __ldg(reinterpret_cast<const float4*>(p.ws + col0) + j);
-      z[4 * j] = scaled(r[4 * j], xs, w.x);
-      z[4 * j + 1] = scaled(r[4 * j + 1], xs, w.y);
-      z[4 * j + 2] = scaled(r[4 * j + 2], xs, w.z);
-      z[4 * j + 3] = scaled(r[4 * j + 3], xs, w.w);
-    }
-    if (p.bias) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
+      float2 lo = make_float2(__int2float_rn(static_cast<int>(r[4 * j])), __int2float_rn(static_cast<int>(r[4 * j + 1])));
+      float2 hi = make_float2(__int2float_rn(static_cast<int>(r[4 * j + 2])), __int2float_rn(static_cast<int>(r[4 * j + 3])));
+      lo = mul2(lo, mul2(xs2, make_float2(w.x, w.y)));
+      hi = mul2(hi, mul2(xs2, make_float2(w.z, w.w)));
+      if (p.bias) {
         const float4 b = __ldg(reinterpret_cast<const float4*>(p.bias + col0) + j);
-        z[4 * j] = __fadd_rn(z[4 * j], b.x);
-        z[4 * j + 1] = __fadd_rn(z[4 * j + 1], b.y);
-        z[4 * j + 2] = __fadd_rn(z[4 * j + 2], b.z);
-        z[4 * j + 3] = __fadd_rn(z[4 * j + 3], b.w);
+        lo = add2(lo, make_float2(b.x, b.y));
+        hi = add2(hi, make_float2(b.z, b.w));
       }
+      z[4 * j] = lo.x; z[4 * j + 1] = lo.y; z[4 * j + 2] = hi.x; z[4 * j + 3] = hi.y;
     }
   } else {
 #pragma unroll
@@ -109,13 +129,14 @@ __device__ __forceinline__ void store_chunk(const Params& p, const uint32_t (&r)
     }
   }
   if constexpr (RELU) {
-    uint32_t bits = 0u;
+    if (p.mask) {
+      uint32_t bits = 0u;
 #pragma unroll
-    for (int j = 0; j < 32; ++j) {
-      bits |= (z[j] > 0.f ? 1u : 0u) << j;
-      z[j] = z[j] > 0.f || z[j] != z[j] ? z[j] : 0.f;  // a NaN (a row that was not finite) stays one
+      for (int j = 0; j < 32; ++j) bits |= z[j] > 0.f ? 1u << j : 0u;
+      p.mask[static_cast<int64_t>(row) * p.ldm + (col0 >> 5)] = bits;
     }
-    if (p.mask) p.mask[static_cast<int64_t>(row) * p.ldm + (col0 >> 5)] = bits;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) z[j] = relu_keep_nan(z[j]);
   }
   if constexpr (F32) {
     float* out = static_cast<float*>(p.out) + static_cast<int64_t>(row) * p.ldo + col0;
@@ -142,6 +163,13 @@ __device__ __forceinline__ void store_chunk(const Params& p, const uint32_t (&r)
         if (j < ncols) out[j] = __float2bfloat16_rn(z[j]);
     }
   }
+}
+
+// Counts an arrival on a barrier of the leader CTA without a release at cluster scope, which would
+// wait for the warp's stores to reach memory: what the arrival reports is that the accumulator has
+// been read, and the tcgen05 fence orders that.
+__device__ __forceinline__ void arrive_leader(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(mapa_shared(smem_u32(bar), 0u)) : "memory");
 }
 
 // ================================================================ CTA pairs
@@ -289,18 +317,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::kThreads, 1)
       if (!mbar_wait(&acc_full[acc], acc_ph, kFaultWaitAccFull)) break;
       tc_fence_after();
       const uint32_t t_row = tmem_base + ((q * 32u) << 16) + acc * TN;
-#pragma unroll 1
-      for (int c = c_lo; c < c_lo + TN / 64; ++c) {
-        const int col0 = n0 + c * 32;
-        if (col0 >= p.N) break;
-        uint32_t r[32];
-        tmem_ld_32x32b_x32(t_row + c * 32, r);
+      // two chunks' accumulators in registers, so that one is on its way while the other is worked on
+      uint32_t r[2][32];
+      tmem_ld_32x32b_x32(t_row + c_lo * 32, r[0]);
+#pragma unroll
+      for (int c = 0; c < TN / 64; ++c) {
         tmem_wait_ld();
-        store_chunk<F32, RELU>(p, r, row, col0, xs);
+        if (c + 1 < TN / 64) {
+          tmem_ld_32x32b_x32(t_row + (c_lo + c + 1) * 32, r[(c + 1) & 1]);
+        } else {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) arrive_leader(&acc_empty[acc]);
+        }
+        const int col0 = n0 + (c_lo + c) * 32;
+        if (col0 < p.N) store_chunk<F32, RELU>(p, r[c & 1], row, col0, xs);
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&acc_empty[acc]), 0u));
       acc ^= 1u;
       if (acc == 0u) acc_ph ^= 1u;
     }
@@ -348,7 +380,7 @@ __device__ __forceinline__ void store_token(const Params& p, uint32_t acc, int m
   if constexpr (RELU) {
     const uint32_t bits = __ballot_sync(0xffffffffu, in && z > 0.f);
     if (p.mask && lane == 0 && in) p.mask[static_cast<int64_t>(m) * p.ldm + (n >> 5)] = bits;
-    z = z > 0.f || z != z ? z : 0.f;
+    z = relu_keep_nan(z);
   }
   if (!in) return;
   if constexpr (F32) static_cast<float*>(p.out)[static_cast<int64_t>(m) * p.ldo + n] = z;

@@ -23,7 +23,9 @@ def _p(t: torch.Tensor | None):
 
 
 def _stream(dev: torch.device):
-    return ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
+    # the raw handle: building a torch.cuda.Stream object takes as long as a launch
+    idx = dev.index
+    return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if idx is None else idx))
 
 
 def _layout(w_layout: str) -> int:
@@ -49,7 +51,7 @@ def _require(t: torch.Tensor, name: str, dtype: torch.dtype, ndim: int,
     if t.dtype != dtype or t.dim() != ndim or not t.is_contiguous():
         raise _lib.C3CUError(-1, name, f"expected contiguous {dtype} with {ndim} dims, got "
                                        f"{t.dtype} {tuple(t.shape)} contiguous={t.is_contiguous()}")
-    if shape is not None and tuple(t.shape) != tuple(shape):
+    if shape is not None and t.shape != tuple(shape):
         raise _lib.C3CUError(-1, name, f"expected shape {tuple(shape)}, got {tuple(t.shape)}")
     if not _device_ok(t):
         raise _lib.C3CUError(-1, name, "expected a CUDA tensor")
@@ -63,7 +65,7 @@ def _require_rows(t: torch.Tensor, name: str, dtype: torch.dtype, rows: int, col
         raise _lib.C3CUError(-1, name, f"expected a torch.Tensor, got {type(t).__name__}")
     if t.dtype != dtype or t.dim() != 2:
         raise _lib.C3CUError(-1, name, f"expected 2-D {dtype}, got {t.dtype} {tuple(t.shape)}")
-    if tuple(t.shape) != (rows, cols):
+    if t.shape != (rows, cols):
         raise _lib.C3CUError(-1, name, f"expected shape {(rows, cols)}, got {tuple(t.shape)}")
     if rows > 0 and cols > 0 and (t.stride(1) != 1 or (rows > 1 and t.stride(0) < (min_ld or cols))):
         raise _lib.C3CUError(-1, name, f"expected unit column stride and row stride >= {min_ld or cols}, "
@@ -266,7 +268,7 @@ def forward_int8(Xq: torch.Tensor, x_scale: torch.Tensor, Wq: torch.Tensor, w_sc
     if b is not None:
         _require(b, "b", torch.float32, 1, (N,))
     if Y is None:
-        Y = torch.empty((M, N), dtype=out_dtype, device=Xq.device)
+        Y = torch.empty(M, N, dtype=out_dtype, device=Xq.device)
     else:
         _require_rows(Y, "Y", out_dtype, M, N)
     if mask is not None:
@@ -274,7 +276,7 @@ def forward_int8(Xq: torch.Tensor, x_scale: torch.Tensor, Wq: torch.Tensor, w_sc
             raise _lib.C3CUError(-1, "mask", "a mask belongs to the ReLU output (relu and save_mask)")
         _require_rows(mask, "mask", torch.int32, M, mask_words(N))
     elif relu and save_mask:
-        mask = torch.empty((M, mask_words(N)), dtype=torch.int32, device=Xq.device)
+        mask = torch.empty(M, mask_words(N), dtype=torch.int32, device=Xq.device)
     rc = _lib.load().c3cu_linear_int8_fwd(_p(Xq), _ld(Xq), _p(x_scale), _p(Wq), _ld(Wq), _p(w_scale), _p(b), _p(Y),
                                           _ld(Y), _lib.DTYPE_F32 if out_dtype == torch.float32 else _lib.DTYPE_BF16,
                                           1 if relu else 0, _p(mask), 0 if mask is None else _ld(mask), M, N, K,
@@ -299,7 +301,7 @@ def grad_weight_int8(dZ: torch.Tensor, Xq: torch.Tensor, x_scale: torch.Tensor, 
     _require_rows(Xq, "Xq", torch.int8, M, K)
     _require(x_scale, "x_scale", torch.float32, 1, (M,))
     if dW is None:
-        dW = torch.empty((N, K), dtype=torch.bfloat16, device=dZ.device)
+        dW = torch.empty(N, K, dtype=torch.bfloat16, device=dZ.device)
     else:
         _require_rows(dW, "dW", torch.bfloat16, N, K)
     L = _lib.load()

@@ -40,7 +40,7 @@ def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, resi
     else:
         _require_rows(residual, "residual", x.dtype, M, K)
         if h is None:
-            h = torch.empty((M, K), dtype=x.dtype, device=x.device)
+            h = torch.empty(M, K, dtype=x.dtype, device=x.device)
         else:
             _require_rows(h, "h", x.dtype, M, K)
             _require_same_rows_or_apart(h, "h", ((x, "x"), (residual, "residual")))
@@ -110,7 +110,7 @@ def rms_norm_backward(dy: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, r
     _require(weight, "weight", torch.float32, 1, (K,))
     _require(rstd, "rstd", torch.float32, 1, (M,))
     if dx is None:
-        dx = torch.empty((M, K), dtype=h.dtype, device=h.device)
+        dx = torch.empty(M, K, dtype=h.dtype, device=h.device)
     else:
         _require_rows(dx, "dx", h.dtype, M, K)
         _require_same_rows_or_apart(dx, "dx", ((dy, "dy"), (h, "h"), (dh, "dh")))

@@ -26,8 +26,8 @@ def empty_rows(m: int, k: int, device) -> torch.Tensor:
     """An uninitialised int8 [m, k] whose rows start on 16 bytes (a column slice of a wider buffer
     unless k is a multiple of 16), as the int8 GEMMs read them."""
     if k % 16 == 0:
-        return torch.empty((m, k), dtype=torch.int8, device=device)
-    return torch.empty((m, (k + 15) // 16 * 16), dtype=torch.int8, device=device)[:, :k]
+        return torch.empty(m, k, dtype=torch.int8, device=device)
+    return torch.empty(m, (k + 15) // 16 * 16, dtype=torch.int8, device=device)[:, :k]
 
 
 @_lib.on_tensor_device
