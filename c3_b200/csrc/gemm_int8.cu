@@ -1,7 +1,6 @@
 // C-ABI entry points of the int8 GEMMs (include/c3cu.h): the Linear forward on int8 rows with
 // scales (igemm.cuh) and the weight gradient from an 8-bit checkpoint (gemm_ckpt.cuh).
 #include <atomic>
-#include <cstdlib>
 
 #include "gemm_ckpt.cuh"
 #include "host_util.h"
@@ -30,34 +29,76 @@ struct Operands {
 template <bool F32, bool RELU>
 int launch_igemm_pair(const Operands& o, const igemm::Params& p, cudaStream_t st) {
   CUtensorMap tx, tw;
-  int rc = encode_int8_2d(&tx, o.x, p.M, p.K, o.ldx, igemm::pair::BK, gemm2::HM, true);
-  if (rc == C3CU_OK) rc = encode_int8_2d(&tw, o.w, p.N, p.K, o.ldw, igemm::pair::BK, gemm2::HN, true);
+  int rc = encode_int8_2d(&tw, o.w, p.N, p.K, o.ldw, igemm::pair::BK, gemm2::HM, true);
+  if (rc == C3CU_OK) rc = encode_int8_2d(&tx, o.x, p.M, p.K, o.ldx, igemm::pair::BK, gemm2::HN, true);
   if (rc != C3CU_OK) return rc;
   auto kern = igemm::igemm_pair_kernel<F32, RELU>;
   static std::atomic<uint64_t> smem_set{0};
   rc = set_max_dynamic_smem(reinterpret_cast<const void*>(kern), gemm2::SMEM_BYTES, smem_set,
                             "linear_int8: set max dynamic shared memory");
   if (rc != C3CU_OK) return rc;
-  const int64_t tiles = static_cast<int64_t>((p.M + gemm2::TM - 1) / gemm2::TM) * ((p.N + gemm2::TN - 1) / gemm2::TN);
-  int clusters = pair_clusters(kern, gemm2::SMEM_BYTES, gemm2::kThreads);
+  const int64_t tiles = static_cast<int64_t>((p.N + gemm2::TM - 1) / gemm2::TM) * ((p.M + gemm2::TN - 1) / gemm2::TN);
+  int clusters = pair_clusters(kern, gemm2::SMEM_BYTES, igemm::pair::kThreads);
   if (tiles < clusters) clusters = static_cast<int>(tiles);
-  return cuda_status(launch_kernel(kern, dim3(2 * clusters), dim3(gemm2::kThreads), gemm2::SMEM_BYTES, st, tx, tw, p),
+  return cuda_status(launch_kernel(kern, dim3(2 * clusters), dim3(igemm::pair::kThreads), gemm2::SMEM_BYTES, st, tw, tx, p),
                      "linear_int8: launch");
 }
 
-struct NarrowPlan {
+// How a forward runs: T = 0 for the pair kernel, else tiles of T tokens, each split along K over a
+// cluster of `split` CTAs.
+struct ForwardPlan {
   int T, split, kb_per_cta, stages;
 };
 
+// The faster kernel by a model of both, fitted to B200 measurements (us; kb = K blocks of a CTA):
+//   narrow  3.3 + waves (kb c(T) + e(T)), e being the epilogue, or for a split tile the exchange of
+//           partial sums 0.6 + 0.034 T
+//   pair    5 + waves (3.2 + 0.265 kb)
+// Measured (us), 4096 channels x K 4096: 1 token 5.8 (T 16, split 4) against 13.4 (pair), 64 tokens
+// 7.8 (T 64, split 4) / 13.6, 512 tokens 12.5 (T 128) / 16.8, 1024 tokens 19.0 (T 256) / 17.9; 12288
+// channels x K 1024, 2048 tokens 54 (T 256) / 34.
+ForwardPlan plan_forward(int64_t M, int64_t N, int64_t K) {
+  constexpr struct {
+    int T;
+    double c, e;
+  } kinds[] = {{16, 0.18, 0.3}, {32, 0.19, 0.4}, {64, 0.21, 0.9}, {128, 0.24, 2.1}, {256, 0.37, 4.5}};
+  const int sms = sm_count() > 0 ? sm_count() : 148;
+  const auto waves = [](int64_t work, int64_t at_once) { return static_cast<double>((work + at_once - 1) / at_once); };
+  const int64_t kb_pair = (K + igemm::pair::BK - 1) / igemm::pair::BK;
+  const int64_t pairs = ((N + gemm2::TM - 1) / gemm2::TM) * ((M + gemm2::TN - 1) / gemm2::TN);
+  ForwardPlan best{0, 1, 0, 0};
+  if (gemm_max_ctas() > 0) return best;  // the persistent kernel keeps to the caller's CTAs
+  double least = 5. + waves(pairs, sms / 2) * (3.2 + 0.265 * static_cast<double>(kb_pair));
+  const int64_t kb = (K + igemm::narrow::BK - 1) / igemm::narrow::BK;
+  const int64_t n_tiles = (N + igemm::narrow::BN - 1) / igemm::narrow::BN;
+  for (const auto& kind : kinds) {
+    if (kind.T > 16 && kind.T >= 2 * M) break;  // half of it would do
+    const int64_t tiles = n_tiles * ((M + kind.T - 1) / kind.T);
+    for (int split = 1; split <= igemm::narrow::kMaxCluster && split <= kb; split *= 2) {
+      const int64_t per = (kb + split - 1) / split;
+      const double tile = static_cast<double>(per) * kind.c + (split > 1 ? 0.6 + 0.034 * kind.T : kind.e);
+      const double t = 3.3 + waves(tiles * split, sms) * tile;
+      if (t < least) {
+        least = t;
+        int stages = static_cast<int>(igemm::narrow::kMaxRing / igemm::narrow::stage_bytes(kind.T));
+        if (stages > igemm::narrow::kMaxStages) stages = igemm::narrow::kMaxStages;
+        if (stages > per) stages = static_cast<int>(per);
+        best = {kind.T, split, static_cast<int>(per), stages};
+      }
+    }
+  }
+  return best;
+}
+
 template <int T, bool F32, bool RELU>
-int launch_igemm_narrow(const Operands& o, igemm::Params p, const NarrowPlan& plan, cudaStream_t st) {
+int launch_igemm_narrow(const Operands& o, igemm::Params p, const ForwardPlan& plan, cudaStream_t st) {
   CUtensorMap tx, tw;
   int rc = encode_int8_2d(&tw, o.w, p.N, p.K, o.ldw, igemm::narrow::BK, igemm::narrow::BN, true);
   if (rc == C3CU_OK) rc = encode_int8_2d(&tx, o.x, p.M, p.K, o.ldx, igemm::narrow::BK, T, true);
   if (rc != C3CU_OK) return rc;
   auto kern = igemm::igemm_narrow_kernel<T, F32, RELU>;
   static std::atomic<uint64_t> smem_set{0};
-  rc = set_max_dynamic_smem(reinterpret_cast<const void*>(kern), 227 * 1024, smem_set,
+  rc = set_max_dynamic_smem(reinterpret_cast<const void*>(kern), igemm::narrow::kMaxSmem, smem_set,
                             "linear_int8: set max dynamic shared memory");
   if (rc != C3CU_OK) return rc;
   p.n_tiles = (p.N + igemm::narrow::BN - 1) / igemm::narrow::BN;
@@ -85,25 +126,14 @@ int launch_igemm_narrow(const Operands& o, igemm::Params p, const NarrowPlan& pl
 
 template <bool F32, bool RELU>
 int dispatch_igemm(const Operands& o, const igemm::Params& p, cudaStream_t st) {
-  const int T = p.M <= 16 ? 16 : p.M <= 32 ? 32 : p.M <= 64 ? 64 : p.M <= 128 ? 128 : 256;
-  if (p.M > 256) return launch_igemm_pair<F32, RELU>(o, p, st);
-  NarrowPlan plan;
-  plan.T = T;
-  const int kb = (p.K + 127) / 128;
-  const int64_t tiles = static_cast<int64_t>((p.N + 127) / 128) * ((p.M + T - 1) / T);
-  int split = 1;
-  while (split < igemm::narrow::kMaxCluster && split * 2 <= kb && tiles * split * 2 <= sm_count()) split *= 2;
-  plan.split = split;
-  plan.kb_per_cta = (kb + split - 1) / split;
-  int stages = static_cast<int>(igemm::narrow::kMaxRing / igemm::narrow::stage_bytes(T));
-  if (stages > igemm::narrow::kMaxStages) stages = igemm::narrow::kMaxStages;
-  plan.stages = plan.kb_per_cta < stages ? plan.kb_per_cta : stages;
-  switch (T) {
+  const ForwardPlan plan = plan_forward(p.M, p.N, p.K);
+  switch (plan.T) {
     case 16: return launch_igemm_narrow<16, F32, RELU>(o, p, plan, st);
     case 32: return launch_igemm_narrow<32, F32, RELU>(o, p, plan, st);
     case 64: return launch_igemm_narrow<64, F32, RELU>(o, p, plan, st);
     case 128: return launch_igemm_narrow<128, F32, RELU>(o, p, plan, st);
-    default: return launch_igemm_narrow<256, F32, RELU>(o, p, plan, st);
+    case 256: return launch_igemm_narrow<256, F32, RELU>(o, p, plan, st);
+    default: return launch_igemm_pair<F32, RELU>(o, p, st);
   }
 }
 
@@ -140,8 +170,14 @@ int dw_clusters(int* clusters) {
 int dw_run(int64_t M, int64_t N, int64_t K, DwRun* r) {
   const int64_t tiles = ((N + ckpt::TM - 1) / ckpt::TM) * ((K + ckpt::TN - 1) / ckpt::TN);
   const int blocks = static_cast<int>((M + ckpt::BK - 1) / ckpt::BK);
-  const char* e = getenv("DEV_RAW");
-  r->raw = e && e[0] == '1';
+  // Widening X in the kernel slows each K block from 0.4 to 0.6 us; widening it first costs a launch
+  // and three bytes per element of X at 6 TB/s. XXX
+  dw_clusters<true>(&r->clusters);
+  r->plan = ckpt::make_plan(static_cast<int>(tiles), r->clusters, blocks);
+  const double rounds = static_cast<double>(r->plan.whole / r->clusters) * blocks +
+                        (r->plan.rest > 0 ? r->plan.kb_per_piece : 0);
+  const double whole_only = r->plan.rest > 0 ? rounds : static_cast<double>((tiles + r->clusters - 1) / r->clusters) * blocks;
+  r->raw = 0.2 * whole_only < 2.5 + 3. * static_cast<double>(M) * static_cast<double>(K) / 6e6;
   const int rc = r->raw ? dw_clusters<true>(&r->clusters) : dw_clusters<false>(&r->clusters);
   r->plan = ckpt::make_plan(static_cast<int>(tiles), r->clusters, blocks);
   r->partial_bytes = static_cast<size_t>(r->plan.rest) * r->plan.pieces * ckpt::TM * ckpt::TN * sizeof(float);
@@ -213,7 +249,6 @@ extern "C" int c3cu_linear_int8_fwd(const int8_t* X, int64_t ldx, const float* x
   p.bias = bias;
   p.mask = mask;
   p.ldm = ldm;
-  p.vec_ok = aligned16(Y) && (M == 1 || ldy * e % 16 == 0) && aligned16(w_scale) && (!bias || aligned16(bias));
   const Operands o{X, W, ldx, ldw};
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (out_dtype == C3CU_DTYPE_F32)

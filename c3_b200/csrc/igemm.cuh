@@ -9,14 +9,17 @@
 // 128-deep K block of a row is one 128-byte swizzled line.
 //
 // Two kernels:
-//   igemm_pair_kernel    256 x 256 tiles on CTA pairs (cta_group::2), persistent: the structure of
-//                        gemm2_kernel with int8 K blocks. For sizes whose tiles fill the GPU.
-//   igemm_narrow_kernel  128 channels x T tokens per CTA, the channels as the MMA's rows, so that
-//                        few tokens leave no tensor-core rows empty. The K blocks of a tile are
+// In both the channels are the MMA's rows and the tokens its columns, so that few tokens leave no
+// tensor-core rows empty and a warp's stores run along a row of Y.
+//   igemm_pair_kernel    tiles of 256 channels x 256 tokens on CTA pairs (cta_group::2), persistent:
+//                        the structure of gemm2_kernel with int8 K blocks. For many tiles.
+//   igemm_narrow_kernel  128 channels x T tokens per CTA. The K blocks of a tile are
 //                        split over a cluster whose CTAs add their int32 partial sums through
 //                        distributed shared memory: with few tokens the weights are the traffic,
 //                        and the split lets all SMs read them.
 #pragma once
+
+#include <type_traits>
 
 #include "common.cuh"
 #include "gemm2_tcgen05.cuh"
@@ -33,7 +36,6 @@ struct Params {
   const float* bias;   // [N] or null
   uint32_t* mask;      // [M][ldm] (RELU), may be null
   int64_t ldm;
-  int32_t vec_ok;      // every full 32-column chunk may use 16-byte accesses
   int32_t kb_per_cta;  // narrow kernel: K blocks per CTA of a cluster
   int32_t n_tiles;     // narrow kernel: tiles of 128 channels
   int32_t stages;      // narrow kernel: ring depth
@@ -68,100 +70,58 @@ __device__ __forceinline__ void umma_i8_ss_pair(uint32_t d_tmem, uint64_t a_desc
       : "memory");
 }
 
-__device__ __forceinline__ float scaled(uint32_t acc, float xs, float ws) {
-  return __fmul_rn(__int2float_rn(static_cast<int>(acc)), __fmul_rn(xs, ws));
-}
-
 __device__ __forceinline__ float relu_keep_nan(float z) {  // a NaN (a row that was not finite) stays one
   float r;
   asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(r) : "f"(z));
   return r;
 }
 
-// Packed fp32 arithmetic: two elements per instruction, each rounded like its scalar form.
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-  float2 d;
-  asm("mul.rn.f32x2 %0, %1, %2;"
-      : "=l"(reinterpret_cast<uint64_t&>(d))
-      : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)));
-  return d;
-}
-
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  float2 d;
-  asm("add.rn.f32x2 %0, %1, %2;"
-      : "=l"(reinterpret_cast<uint64_t&>(d))
-      : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)));
-  return d;
-}
-
-// 32 columns of one row of the output (pair kernel: a thread owns a row).
-template <bool F32, bool RELU>
-__device__ __forceinline__ void store_chunk(const Params& p, const uint32_t (&r)[32], int row, int col0, float xs) {
-  if (row >= p.M) return;
-  const int ncols = min(32, p.N - col0);
-  const bool full = p.vec_ok && ncols == 32;
-  float z[32];
-  if (full) {
-    const float2 xs2 = make_float2(xs, xs);
+// The epilogue of J tokens, one channel per lane: a token's 32 lanes store 32 consecutive channels
+// (16-byte stores of a row per lane would touch 32 lines each), and the channel's scale and bias stay
+// in registers. `m` is the first token, `count` how many there are, xs(j) their scales. The J tokens'
+// arithmetic and stores are independent of one another.
+template <int J, bool F32, bool RELU, class Scale>
+__device__ __forceinline__ void store_tokens(const Params& p, const uint32_t (&acc)[J], Scale xs, int m, int count,
+                                             int n, float ws, float b, uint32_t lane) {
+  const bool in = n < p.N;
+  float z[J];
+  // Scalar intrinsics, which are never contracted: ptxas fused a packed (f32x2) multiply and add.
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float4 w = __ldg(reinterpret_cast<const float4*>(p.ws + col0) + j);
-      float2 lo = make_float2(__int2float_rn(static_cast<int>(r[4 * j])), __int2float_rn(static_cast<int>(r[4 * j + 1])));
-      float2 hi = make_float2(__int2float_rn(static_cast<int>(r[4 * j + 2])), __int2float_rn(static_cast<int>(r[4 * j + 3])));
-      lo = mul2(lo, mul2(xs2, make_float2(w.x, w.y)));
-      hi = mul2(hi, mul2(xs2, make_float2(w.z, w.w)));
-      if (p.bias) {
-        const float4 b = __ldg(reinterpret_cast<const float4*>(p.bias + col0) + j);
-        lo = add2(lo, make_float2(b.x, b.y));
-        hi = add2(hi, make_float2(b.z, b.w));
-      }
-      z[4 * j] = lo.x; z[4 * j + 1] = lo.y; z[4 * j + 2] = hi.x; z[4 * j + 3] = hi.y;
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 32; ++j) {
-      z[j] = 0.f;
-      if (j < ncols) {
-        z[j] = scaled(r[j], xs, __ldg(p.ws + col0 + j));
-        if (p.bias) z[j] = __fadd_rn(z[j], __ldg(p.bias + col0 + j));
-      }
-    }
+  for (int j = 0; j < J; ++j) {
+    z[j] = __fmul_rn(__int2float_rn(static_cast<int>(acc[j])), __fmul_rn(xs(j), ws));
+    if (p.bias) z[j] = __fadd_rn(z[j], b);
   }
   if constexpr (RELU) {
     if (p.mask) {
-      uint32_t bits = 0u;
+      uint32_t word = 0u;  // of token `lane`
 #pragma unroll
-      for (int j = 0; j < 32; ++j) bits |= z[j] > 0.f ? 1u << j : 0u;
-      p.mask[static_cast<int64_t>(row) * p.ldm + (col0 >> 5)] = bits;
+      for (int j = 0; j < J; ++j) {
+        const uint32_t bits = __ballot_sync(0xffffffffu, in && z[j] > 0.f);
+        if (lane == static_cast<uint32_t>(j)) word = bits;
+      }
+      const int n0 = n - static_cast<int>(lane);
+      if (n0 < p.N && static_cast<int>(lane) < count && lane < J)
+        p.mask[static_cast<int64_t>(m + lane) * p.ldm + (n0 >> 5)] = word;
     }
 #pragma unroll
-    for (int j = 0; j < 32; ++j) z[j] = relu_keep_nan(z[j]);
+    for (int j = 0; j < J; ++j) z[j] = relu_keep_nan(z[j]);
   }
-  if constexpr (F32) {
-    float* out = static_cast<float*>(p.out) + static_cast<int64_t>(row) * p.ldo + col0;
-    if (full) {
+  if (!in) return;
+  using Out = typename std::conditional<F32, float, __nv_bfloat16>::type;
+  Out* out = static_cast<Out*>(p.out) + static_cast<int64_t>(m) * p.ldo + n;
+  Out v[J];
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        reinterpret_cast<float4*>(out)[j] = make_float4(z[4 * j], z[4 * j + 1], z[4 * j + 2], z[4 * j + 3]);
-    } else {
+  for (int j = 0; j < J; ++j) {
+    if constexpr (F32) v[j] = z[j];
+    else v[j] = __float2bfloat16_rn(z[j]);
+  }
+  if (count >= J) {
 #pragma unroll
-      for (int j = 0; j < 32; ++j)
-        if (j < ncols) out[j] = z[j];
-    }
+    for (int j = 0; j < J; ++j, out += p.ldo) *out = v[j];
   } else {
-    __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.out) + static_cast<int64_t>(row) * p.ldo + col0;
-    if (full) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        reinterpret_cast<uint4*>(out)[j] =
-            make_uint4(pack_bf16x2(z[8 * j], z[8 * j + 1]), pack_bf16x2(z[8 * j + 2], z[8 * j + 3]),
-                       pack_bf16x2(z[8 * j + 4], z[8 * j + 5]), pack_bf16x2(z[8 * j + 6], z[8 * j + 7]));
-    } else {
-#pragma unroll
-      for (int j = 0; j < 32; ++j)
-        if (j < ncols) out[j] = __float2bfloat16_rn(z[j]);
-    }
+    for (int j = 0; j < J; ++j, out += p.ldo)
+      if (j < count) *out = v[j];
   }
 }
 
@@ -178,9 +138,7 @@ using gemm2::A_STAGE_BYTES;
 using gemm2::B_STAGE_BYTES;
 using gemm2::HM;
 using gemm2::HN;
-using gemm2::kEpiWarps;
 using gemm2::kPairMask;
-using gemm2::kThreads;
 using gemm2::SMEM_BYTES;
 using gemm2::STAGE_BYTES;
 using gemm2::STAGES;
@@ -189,11 +147,14 @@ using gemm2::TMEM_COLS;
 using gemm2::TN;
 constexpr int BK = 128;         // int8 elements: the same 128-byte lines as 64 bf16
 constexpr uint32_t KSTEP = 32;  // bytes (elements) of K per MMA
+constexpr int kEpiWarps = 8;     // sixteen measured the same
+constexpr int kThreads = 64 + 32 * kEpiWarps;
+constexpr int kWarpTokens = TN / (kEpiWarps / 4);
 }  // namespace pair
 
 template <bool F32, bool RELU>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::kThreads, 1)
-    igemm_pair_kernel(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CUtensorMap tmb,
+    igemm_pair_kernel(const __grid_constant__ CUtensorMap tmw, const __grid_constant__ CUtensorMap tmx,
                       const Params p) {
   using namespace pair;
   extern __shared__ uint8_t smem_raw[];
@@ -215,8 +176,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::kThreads, 1)
   const bool leader = rank == 0u;
   const int cluster = static_cast<int>(blockIdx.x >> 1);
   const int num_clusters = static_cast<int>(gridDim.x >> 1);
-  const int n_tiles = (p.N + TN - 1) / TN;
-  const int num_tiles = ((p.M + TM - 1) / TM) * n_tiles;
+  // a tile: 256 channels (the MMA's rows) x 256 tokens
+  const int n_tiles = (p.N + TM - 1) / TM;
+  const int num_tiles = ((p.M + TN - 1) / TN) * n_tiles;
   const int k_blocks = (p.K + BK - 1) / BK;
 
   if (warp == 0 && lane == 0) {
@@ -230,8 +192,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::kThreads, 1)
     }
     mbar_init(drain, 1);
     fence_mbarrier_init();
-    tma_prefetch_desc(&tma);
-    tma_prefetch_desc(&tmb);
+    tma_prefetch_desc(&tmw);
+    tma_prefetch_desc(&tmx);
   }
   if (warp == 1) {
     tmem_alloc_pair(tmem_slot, TMEM_COLS);
@@ -251,14 +213,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::kThreads, 1)
       uint32_t ph = 0, armed = 0u, armed_par = 0u;
       bool ok = true;
       for (int tile = cluster; ok && tile < num_tiles; tile += num_clusters) {
-        const int m0 = (tile / n_tiles) * TM + static_cast<int>(rank) * HM;
-        const int n0 = (tile % n_tiles) * TN + static_cast<int>(rank) * HN;
+        const int n0 = (tile % n_tiles) * TM + static_cast<int>(rank) * HM;
+        const int m0 = (tile / n_tiles) * TN + static_cast<int>(rank) * HN;
         for (int kb = 0; kb < k_blocks; ++kb) {
           if (!mbar_wait(&empty[s], ph ^ 1u, kFaultWaitEmpty)) { ok = false; break; }
           if (leader) mbar_arrive_expect_tx(&full[s], 2u * STAGE_BYTES);
           const uint32_t bar_leader = mapa_shared(smem_u32(&full[s]), 0u);
-          tma_load_2d_pair(sA + s * A_STAGE_BYTES, &tma, bar_leader, kb * BK, m0);
-          tma_load_2d_pair(sB + s * B_STAGE_BYTES, &tmb, bar_leader, kb * BK, n0);
+          tma_load_2d_pair(sA + s * A_STAGE_BYTES, &tmw, bar_leader, kb * BK, n0);
+          tma_load_2d_pair(sB + s * B_STAGE_BYTES, &tmx, bar_leader, kb * BK, m0);
           armed |= 1u << s;
           armed_par = (armed_par & ~(1u << s)) | (ph << s);
           if (++s == STAGES) { s = 0; ph ^= 1u; }
@@ -308,30 +270,39 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::kThreads, 1)
   } else {
     // ------------------------------------------------------------ epilogue (warps 2..9)
     const uint32_t q = warp & 3u;
-    const int c_lo = static_cast<int>((warp - 2u) >> 2) * (TN / 64);
+    const int c_lo = static_cast<int>((warp - 2u) >> 2) * kWarpTokens;  // this warp's share of the tokens
     uint32_t acc = 0, acc_ph = 0;
     for (int tile = cluster; tile < num_tiles; tile += num_clusters) {
-      const int row = (tile / n_tiles) * TM + static_cast<int>(rank) * HM + static_cast<int>(q * 32 + lane);
-      const int n0 = (tile % n_tiles) * TN;
-      const float xs = row < p.M ? __ldg(p.xs + row) : 0.f;
+      const int n = (tile % n_tiles) * TM + static_cast<int>(rank) * HM + static_cast<int>(q * 32 + lane);
+      const int m0 = (tile / n_tiles) * TN + c_lo;
+      const float ws = n < p.N ? __ldg(p.ws + n) : 0.f;
+      const float b = p.bias && n < p.N ? __ldg(p.bias + n) : 0.f;
+      float xs[kWarpTokens / 32];  // of token m0 + 32 c + lane
+#pragma unroll
+      for (int c = 0; c < kWarpTokens / 32; ++c) {
+        const int m = m0 + c * 32 + static_cast<int>(lane);
+        xs[c] = m < p.M ? __ldg(p.xs + m) : 0.f;
+      }
       if (!mbar_wait(&acc_full[acc], acc_ph, kFaultWaitAccFull)) break;
       tc_fence_after();
-      const uint32_t t_row = tmem_base + ((q * 32u) << 16) + acc * TN;
+      const uint32_t t_row = tmem_base + ((q * 32u) << 16) + acc * TN + static_cast<uint32_t>(c_lo);
       // two chunks' accumulators in registers, so that one is on its way while the other is worked on
       uint32_t r[2][32];
-      tmem_ld_32x32b_x32(t_row + c_lo * 32, r[0]);
+      tmem_ld_32x32b_x32(t_row, r[0]);
 #pragma unroll
-      for (int c = 0; c < TN / 64; ++c) {
+      for (int c = 0; c < kWarpTokens / 32; ++c) {
         tmem_wait_ld();
-        if (c + 1 < TN / 64) {
-          tmem_ld_32x32b_x32(t_row + (c_lo + c + 1) * 32, r[(c + 1) & 1]);
+        if (c + 1 < kWarpTokens / 32) {
+          tmem_ld_32x32b_x32(t_row + (c + 1) * 32, r[(c + 1) & 1]);
         } else {
           tc_fence_before();
           __syncwarp();
           if (lane == 0) arrive_leader(&acc_empty[acc]);
         }
-        const int col0 = n0 + (c_lo + c) * 32;
-        if (col0 < p.N) store_chunk<F32, RELU>(p, r[c & 1], row, col0, xs);
+        const int m = m0 + c * 32;
+        if (m < p.M)
+          store_tokens<32, F32, RELU>(
+              p, r[c & 1], [&](int j) { return __shfl_sync(0xffffffffu, xs[c], j); }, m, p.M - m, n, ws, b, lane);
       }
       acc ^= 1u;
       if (acc == 0u) acc_ph ^= 1u;
@@ -350,12 +321,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::kThreads, 1)
 namespace narrow {
 constexpr int BN = 128;          // channels per CTA: the MMA's 128 rows
 constexpr int BK = 128;
-constexpr int kThreads = 192;    // TMA, MMA, four epilogue warps
+constexpr int kThreads = 320;    // TMA, MMA, eight epilogue warps: two a scheduler, since one alone
+                                 // waits out the latency of each of its instructions
 constexpr int kMaxStages = 8;
 constexpr int kMaxCluster = 8;
 constexpr uint32_t W_BYTES = BN * BK;
 constexpr uint32_t BAR_BYTES = (2 * kMaxStages + 1) * 8 + 8;
 constexpr uint32_t kMaxRing = 200 * 1024;
+constexpr int kMaxSmem = static_cast<int>(kMaxRing) + 4096;  // barriers and alignment besides
 __host__ __device__ constexpr uint32_t stage_bytes(int T) { return W_BYTES + static_cast<uint32_t>(T) * BK; }
 __host__ __device__ constexpr uint32_t partial_bytes(int T) { return static_cast<uint32_t>(T) * BN * 4; }
 __host__ __device__ constexpr uint32_t smem_bytes(int T, int stages) {
@@ -370,23 +343,6 @@ __device__ __forceinline__ uint32_t ld_shared_cluster(uint32_t addr) {
   return v;
 }
 
-// One element per lane: 32 consecutive channels of one token.
-template <bool F32, bool RELU>
-__device__ __forceinline__ void store_token(const Params& p, uint32_t acc, int m, int n, float ws, float b,
-                                            uint32_t lane) {
-  const bool in = n < p.N;
-  float z = scaled(acc, __ldg(p.xs + m), ws);
-  if (p.bias) z = __fadd_rn(z, b);
-  if constexpr (RELU) {
-    const uint32_t bits = __ballot_sync(0xffffffffu, in && z > 0.f);
-    if (p.mask && lane == 0 && in) p.mask[static_cast<int64_t>(m) * p.ldm + (n >> 5)] = bits;
-    z = relu_keep_nan(z);
-  }
-  if (!in) return;
-  if constexpr (F32) static_cast<float*>(p.out)[static_cast<int64_t>(m) * p.ldo + n] = z;
-  else static_cast<__nv_bfloat16*>(p.out)[static_cast<int64_t>(m) * p.ldo + n] = __float2bfloat16_rn(z);
-}
-
 template <int T, bool F32, bool RELU>
 __global__ void __launch_bounds__(narrow::kThreads)
     igemm_narrow_kernel(const __grid_constant__ CUtensorMap tmw, const __grid_constant__ CUtensorMap tmx,
@@ -394,6 +350,7 @@ __global__ void __launch_bounds__(narrow::kThreads)
   using namespace narrow;
   constexpr uint32_t STAGE = stage_bytes(T);
   constexpr uint32_t COLS = T < 32 ? 32 : T;
+  __shared__ __align__(16) float s_xs[T];
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
@@ -430,6 +387,8 @@ __global__ void __launch_bounds__(narrow::kThreads)
     tmem_alloc(tmem_slot, COLS);
     tmem_relinquish();
   }
+  // the tokens' scales: fetched now, since in the epilogue every fetch would be waited for
+  for (int t = static_cast<int>(threadIdx.x); t < T; t += kThreads) s_xs[t] = m0 + t < p.M ? __ldg(p.xs + m0 + t) : 0.f;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -477,7 +436,8 @@ __global__ void __launch_bounds__(narrow::kThreads)
     __syncwarp();
   }
 
-  const uint32_t q = warp & 3u;  // the lane quarter of an epilogue warp
+  const uint32_t q = warp & 3u;                              // the lane quarter of an epilogue warp
+  const int half = warp >= 6 ? 1 : 0;                        // the two warps of a quarter share the tokens
   const int n = n0 + static_cast<int>(q * 32 + lane);
   const uint32_t t_row = tmem + ((q * 32u) << 16);
   float ws = 0.f, b = 0.f;
@@ -490,29 +450,25 @@ __global__ void __launch_bounds__(narrow::kThreads)
     ok = mbar_wait(acc_full, 0u, kFaultWaitAccFull);
     tc_fence_after();
   }
+  const int tokens = min(T, p.M - m0);
   if (size == 1u) {
     if (warp >= 2 && ok) {
 #pragma unroll 1
-      for (int c = 0; c < T; c += 16) {
-        if (m0 + c >= p.M) break;
+      for (int c = 16 * half; c < tokens; c += 32) {
         uint32_t r[16];
         tmem_ld_32x32b_x16(t_row + c, r);
         tmem_wait_ld();
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-          if (m0 + c + j < p.M) store_token<F32, RELU>(p, r[j], m0 + c + j, n, ws, b, lane);
+        store_tokens<16, F32, RELU>(p, r, [&](int j) { return s_xs[c + j]; }, m0 + c, tokens - c, n, ws, b, lane);
       }
     }
   } else {
     // The ring is free (every MMA has read its stage): it takes this CTA's partial sums
     // [token][channel], and each CTA adds up and stores its share of the tokens.
     uint32_t* part = reinterpret_cast<uint32_t*>(smem);
-    const int tokens = min(T, p.M - m0);
     const bool any = kb0 < kb1;  // the last CTAs may have no K block: their sums are zero
     if (warp >= 2) {
 #pragma unroll 1
-      for (int c = 0; c < T; c += 16) {
-        if (c >= tokens) break;
+      for (int c = 16 * half; c < tokens; c += 32) {
         uint32_t r[16];
         tmem_ld_32x32b_x16(t_row + c, r);
         tmem_wait_ld();
@@ -523,10 +479,22 @@ __global__ void __launch_bounds__(narrow::kThreads)
     cluster_sync_all();
     if (warp >= 2 && ok) {
       const uint32_t mine = smem_u32(part) + (q * 32u + lane) * 4u;
-      for (int t = static_cast<int>(rank); t < tokens; t += static_cast<int>(size)) {
-        uint32_t sum = 0u;
-        for (uint32_t r = 0; r < size; ++r) sum += ld_shared_cluster(mapa_shared(mine + t * (BN * 4), r));
-        store_token<F32, RELU>(p, sum, m0 + t, n, ws, b, lane);
+      const int share = T / static_cast<int>(size);
+      const int first = static_cast<int>(rank) * share;
+      const int last = min(first + share, tokens);
+      constexpr int J = T / kMaxCluster < 8 ? T / kMaxCluster : 8;  // divides every share
+#pragma unroll 1
+      for (int t = first + J * half; t < last; t += 2 * J) {
+        uint32_t sum[J];
+#pragma unroll
+        for (int j = 0; j < J; ++j) sum[j] = 0u;
+#pragma unroll 2
+        for (uint32_t r = 0; r < size; ++r) {
+          const uint32_t from = mapa_shared(mine + t * (BN * 4), r);
+#pragma unroll
+          for (int j = 0; j < J; ++j) sum[j] += ld_shared_cluster(from + j * (BN * 4));
+        }
+        store_tokens<J, F32, RELU>(p, sum, [&](int j) { return s_xs[t + j]; }, m0 + t, last - t, n, ws, b, lane);
       }
     }
     cluster_sync_all();  // no CTA leaves while another reads its sums

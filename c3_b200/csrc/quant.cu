@@ -9,11 +9,10 @@
 // The int8 numbers do not depend on rstd: with a = fl32(h * w) and A = max |a| the row's q is
 // round(127 a / A), so one reduction over the row yields both the sum of squares and A, and a
 // row is read once. q is the integer nearest to the real quotient, ties to even, whatever the
-// launch shape: an element whose fp32 quotient lies too near to a half-integer to be decided is
-// divided again in fp64, which decides every case (a and A have 24-bit significands, so a
-// quotient that is not a tie is at least 2^-32 of its size away from one).
+// launch shape: an element whose fp32 quotient lies too near to a half-integer is decided by the
+// sign of 254 a - (2 n + 1) A, which fp32 with fused multiply-adds gives exactly.
 #include <atomic>
-#include <cstdlib>
+#include <type_traits>
 
 #include "common.cuh"
 #include "host_util.h"
@@ -117,14 +116,20 @@ __device__ __forceinline__ void load(const T* row, int t, int i, int G, int K, R
     if (c < K) expand<T>(__ldcs(reinterpret_cast<const uint4*>(row + c)), x);
     else clear(x);
   } else {
-    float f[8];
+    using Raw = typename std::conditional<sizeof(T) == 4, uint32_t, unsigned short>::type;
+    const Raw* from = reinterpret_cast<const Raw*>(row) + t + i * 8 * SG;
+    uint32_t f[8];
+    if ((i + 1) * 8 * SG <= K) {  // the whole block's runs: no bounds
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int c = R::col(t, i, j, G);
-      f[j] = c < K ? static_cast<float>(row[c]) : 0.f;
+      for (int j = 0; j < 8; ++j) f[j] = from[j * SG];
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = R::col(t, i, j, G) < K ? from[j * SG] : Raw{0};
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x.v[j] = make_float2(f[2 * j], f[2 * j + 1]);
+    for (int j = 0; j < 8; ++j) f[j] <<= 32 - 8 * sizeof(T);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x.v[j] = make_float2(__uint_as_float(f[2 * j]), __uint_as_float(f[2 * j + 1]));
   }
 }
 
@@ -146,13 +151,29 @@ __device__ __forceinline__ void load_weight(const float* w, int t, int i, int G,
     }
   } else {
     float f[8];
+    const float* from = w + t + i * 8 * SG;
+    if ((i + 1) * 8 * SG <= K) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int c = R::col(t, i, j, G);
-      f[j] = c < K ? __ldg(w + c) : 0.f;
+      for (int j = 0; j < 8; ++j) f[j] = __ldg(from + j * SG);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = R::col(t, i, j, G) < K ? __ldg(from + j * SG) : 0.f;
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) x.v[j] = make_float2(f[2 * j], f[2 * j + 1]);
+  }
+}
+
+// Eight elements SG apart, those at columns below K (`to` is column c's address).
+template <int SG, typename T>
+__device__ __forceinline__ void store_strided(T* to, int c, int K, const T (&f)[8]) {
+  if (c + 8 * SG <= K) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) to[j * SG] = f[j];
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (c + j * SG < K) to[j * SG] = f[j];
   }
 }
 
@@ -175,19 +196,21 @@ __device__ __forceinline__ void store(T* row, int t, int i, int G, int K, Run<Ru
       expand<T>(w, x);
     }
   } else {
+    T* to = row + t + i * 8 * SG;
+    T f[8];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int c0 = R::col(t, i, 2 * j, G), c1 = R::col(t, i, 2 * j + 1, G);
       if constexpr (sizeof(T) == 4) {
-        if (c0 < K) row[c0] = x.v[j].x;
-        if (c1 < K) row[c1] = x.v[j].y;
+        f[2 * j] = x.v[j].x;
+        f[2 * j + 1] = x.v[j].y;
       } else {
         const uint32_t w = pack_bf16x2(x.v[j].x, x.v[j].y);
-        if (c0 < K) row[c0] = __ushort_as_bfloat16(static_cast<unsigned short>(w));
-        if (c1 < K) row[c1] = __ushort_as_bfloat16(static_cast<unsigned short>(w >> 16));
+        f[2 * j] = __ushort_as_bfloat16(static_cast<unsigned short>(w));
+        f[2 * j + 1] = __ushort_as_bfloat16(static_cast<unsigned short>(w >> 16));
         x.v[j] = unpack(w);
       }
     }
+    store_strided<SG>(to, t + i * 8 * SG, K, f);
   }
 }
 
@@ -203,15 +226,11 @@ __device__ __forceinline__ void store_sums(float* out, int t, int i, int G, int 
 }
 
 // ---------------------------------------------------------------- rounding to int8
-__device__ __noinline__ uint32_t quantize_exact(float a, float big) {
-  return static_cast<uint32_t>(static_cast<int>(rint(127.0 * static_cast<double>(a) / static_cast<double>(big))));
-}
-
 struct RowScale {
   float big;   // A
-  float inv;   // 127 / A
+  float inv;   // 127 / A, within 2^-24 of it
   float safe;  // largest |a inv - round(a inv)| at which a inv rounds like the real quotient
-  bool finite;
+  bool finite, tame;
 };
 
 // `bits` is the largest |a| as its bit pattern (which orders like the number, with infinities and
@@ -220,14 +239,34 @@ __device__ __forceinline__ RowScale row_scale(uint32_t bits) {
   RowScale r;
   r.big = __uint_as_float(bits);
   r.finite = bits < 0x7f800000u;
-  float rcp;  // within 2^-23 of 1 / A
+  // Beyond this range 127 / A or 254 a could leave fp32's: such rows take fp64 divisions.
+  r.tame = r.big > 1e-25f && r.big < 1e35f;
+  float rcp;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(rcp) : "f"(r.big));
-  r.inv = r.finite && bits != 0u ? 127.f * rcp : 0.f;
-  // a inv, multiplied without a rounding, is off by inv's: at most 127 * 1.5 * 2^-23 = 2.3e-5. Near
-  // the ends of fp32's range the reciprocal may overflow or vanish: there every element takes the
-  // fp64 division.
-  r.safe = (bits == 0u || (r.big > 1e-35f && r.big < 1e37f)) ? 0.5f - 4e-5f : -1.f;
+  const float inv = 127.f * rcp;
+  r.inv = r.tame ? fmaf(fmaf(-inv, r.big, 127.f), rcp, inv) : 0.f;
+  // a inv, multiplied without a rounding, is off by inv's error: at most 127 * 2^-23
+  r.safe = 0.5f - 1.6e-5f;
   return r;
+}
+
+// The nearest integer to 127 a / A, ties to even, given one of its two neighbours n = round(a inv)
+// and off = a inv - n, near +-1/2: whether the quotient is beyond the half-integer b / 2,
+// b = 2 n +- 1, is the sign of 254 a - b A. Both products are taken apart into their rounded value
+// and the rest (exact, 32 bits each); the values are so near each other that they subtract exactly.
+__device__ __forceinline__ float decide(float a, float big, float n, float off) {
+  const float way = off > 0.f ? 1.f : -1.f;
+  const float b = fmaf(2.f, n, way);
+  const float p = __fmul_rn(254.f, a), q = __fmul_rn(b, big);
+  const float rest = __fsub_rn(fmaf(254.f, a, -p), fmaf(b, big, -q));
+  const float diff = __fmul_rn(__fadd_rn(__fsub_rn(p, q), rest), way);
+  const bool odd = static_cast<int>(n) & 1;
+  return diff > 0.f || (diff == 0.f && odd) ? n + way : n;
+}
+
+// A row of extreme magnitude.
+__device__ __noinline__ float quantize_wild(float a, float big) {
+  return big > 0.f ? static_cast<float>(rint(127.0 * static_cast<double>(a) / static_cast<double>(big))) : 0.f;
 }
 
 template <typename T, int SG>
@@ -235,28 +274,30 @@ __device__ __forceinline__ void store_q(int8_t* row, int t, int i, int G, int K,
                                         const RowScale& r) {
   using R = Runs<T, SG>;
   constexpr float kMagic = 12582912.f;  // 1.5 * 2^23: adding it leaves round(a inv) in the low bits
-  uint32_t n[R::V];
-  float off[R::V];
+  float m[R::V], off[R::V];
   float worst = 0.f;
 #pragma unroll
   for (int j = 0; j < R::V / 2; ++j) {
-    const float2 m = fma2(a.v[j], both(r.inv), both(kMagic));
-    const float2 d = fma2(a.v[j], both(-r.inv), add2(m, both(-kMagic)));
-    n[2 * j] = __float_as_uint(m.x);
-    n[2 * j + 1] = __float_as_uint(m.y);
+    const float2 x = fma2(a.v[j], both(r.inv), both(kMagic));
+    const float2 d = fma2(a.v[j], both(r.inv), add2(both(kMagic), make_float2(-x.x, -x.y)));
+    m[2 * j] = x.x;
+    m[2 * j + 1] = x.y;
     off[2 * j] = d.x;
     off[2 * j + 1] = d.y;
     worst = max_magnitude(worst, d.x, d.y);
   }
-  if (!(worst <= r.safe)) {
+  if (worst > r.safe) {
 #pragma unroll
     for (int j = 0; j < R::V; ++j)
-      if (!(fabsf(off[j]) <= r.safe)) n[j] = quantize_exact(a[j], r.big);
+      if (fabsf(off[j]) > r.safe) m[j] = decide(a[j], r.big, m[j] - kMagic, off[j]) + kMagic;
   }
-  if (!r.finite) {
+  if (!r.tame) {
 #pragma unroll
-    for (int j = 0; j < R::V; ++j) n[j] = 0u;
+    for (int j = 0; j < R::V; ++j) m[j] = (r.finite ? quantize_wild(a[j], r.big) : 0.f) + kMagic;
   }
+  uint32_t n[R::V];
+#pragma unroll
+  for (int j = 0; j < R::V; ++j) n[j] = __float_as_uint(m[j]);
   if constexpr (SG == 0) {
     uint32_t w[R::V / 4];
 #pragma unroll
@@ -268,11 +309,10 @@ __device__ __forceinline__ void store_q(int8_t* row, int t, int i, int G, int K,
     if constexpr (R::V == 4) *reinterpret_cast<uint32_t*>(row + c) = w[0];
     else *reinterpret_cast<uint2*>(row + c) = make_uint2(w[0], w[1]);
   } else {
+    int8_t f[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int c = R::col(t, i, j, G);
-      if (c < K) row[c] = static_cast<int8_t>(n[j]);
-    }
+    for (int j = 0; j < 8; ++j) f[j] = static_cast<int8_t>(n[j]);
+    store_strided<SG>(row + t + i * 8 * SG, t + i * 8 * SG, K, f);
   }
 }
 
@@ -321,6 +361,33 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
 }
 
 constexpr int kMaxStages = 8;
+
+// What a bulk copy brings of a row that need not start on 16 bytes: whole 16-byte pieces around it.
+// The first and last rows' may reach past the matrix; those rows are read from global memory.
+struct Span {
+  const uint8_t* from;  // 16-byte aligned
+  uint32_t size;        // multiple of 16
+  uint32_t skip;        // bytes before the row's first
+  bool direct;
+};
+
+template <typename T>
+__device__ __forceinline__ Span row_span(const void* base, int64_t ld, int M, int64_t row, uint32_t bytes) {
+  const uint8_t* first = static_cast<const uint8_t*>(base);
+  const uint8_t* start = first + row * ld * static_cast<int64_t>(sizeof(T));
+  const uint8_t* end = first + (M - 1) * ld * static_cast<int64_t>(sizeof(T)) + bytes;
+  Span r;
+  r.skip = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(start) & 15u);
+  r.from = start - r.skip;
+  r.size = (r.skip + bytes + 15u) & ~15u;
+  r.direct = r.from < first || r.from + r.size > end;
+  return r;
+}
+
+// Bytes of a ring stage that one input's row takes.
+__host__ __device__ inline uint32_t row_pitch(uint32_t bytes, bool aligned) {
+  return aligned ? bytes : ((bytes + 15u) & ~15u) + 16u;
+}
 
 struct RowRing {
   uint64_t full[kMaxStages];
@@ -384,10 +451,9 @@ __device__ __forceinline__ void accumulate(Run<V>& a, const Run<V>& w, float2& s
 
 // One row per block (or, with 32 threads a row, per warp), held in registers between the reduction
 // and the rounding.
-template <typename T, bool NORM, bool RES, int SG, bool WARP>
+template <typename T, bool NORM, bool RES, int SG, int N, bool WARP>
 __global__ void __launch_bounds__(WARP ? 128 : 1024) rows_kernel(const FwdArgs p) {
   using R = Runs<T, SG>;
-  constexpr int N = kRowElems / R::V;
   __shared__ RowSums sums;
   const int64_t row = WARP ? static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5)
                            : static_cast<int64_t>(blockIdx.x);
@@ -438,20 +504,32 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024) rows_kernel(const FwdArgs p
   if (t == 0) row_outputs(p, row, sum, r, NORM);
 }
 
-// The same over many rows, grid-strided, through the ring (16-byte rows only).
-template <typename T, bool NORM, bool RES, int N>
+// The same over many rows, grid-strided, through the ring.
+template <typename T, bool NORM, bool RES, int SG, int N>
 __global__ void __launch_bounds__(1024) ring_rows_kernel(const FwdArgs p) {
-  constexpr int V = Runs<T, 0>::V;
+  using R = Runs<T, SG>;
+  constexpr int V = R::V;
   extern __shared__ __align__(128) uint8_t rows[];
   __shared__ RowSums sums;
   __shared__ RowRing ring;
   const int t = threadIdx.x, G = blockDim.x;
   const uint32_t bytes = static_cast<uint32_t>(p.K) * sizeof(T);
-  const uint32_t stage = (RES ? 2u : 1u) * bytes;
+  const uint32_t pitch = row_pitch(bytes, SG == 0);
+  const uint32_t stage = (RES ? 2u : 1u) * pitch;
   auto fill = [&](int s, int64_t row) {
-    mbar_arrive_expect_tx(&ring.full[s], stage);
-    bulk_load(rows + s * stage, static_cast<const T*>(p.x) + row * p.ldx, bytes, &ring.full[s]);
-    if constexpr (RES) bulk_load(rows + s * stage + bytes, static_cast<const T*>(p.res) + row * p.ldr, bytes, &ring.full[s]);
+    uint8_t* to = rows + s * stage;
+    if constexpr (SG == 0) {
+      mbar_arrive_expect_tx(&ring.full[s], stage);
+      bulk_load(to, static_cast<const T*>(p.x) + row * p.ldx, bytes, &ring.full[s]);
+      if constexpr (RES) bulk_load(to + pitch, static_cast<const T*>(p.res) + row * p.ldr, bytes, &ring.full[s]);
+    } else {
+      const Span x = row_span<T>(p.x, p.ldx, p.M, row, bytes);
+      Span r = x;
+      if constexpr (RES) r = row_span<T>(p.res, p.ldr, p.M, row, bytes);
+      mbar_arrive_expect_tx(&ring.full[s], (x.direct ? 0u : x.size) + (RES && !r.direct ? r.size : 0u));
+      if (!x.direct) bulk_load(to, x.from, x.size, &ring.full[s]);
+      if (RES && !r.direct) bulk_load(to + pitch, r.from, r.size, &ring.full[s]);
+    }
   };
   if (t == 0) {
     for (int s = 0; s < p.stages; ++s) mbar_init(&ring.full[s], 1);
@@ -468,30 +546,51 @@ __global__ void __launch_bounds__(1024) ring_rows_kernel(const FwdArgs p) {
   int64_t row = blockIdx.x;
   for (; row < p.M; row += gridDim.x) {
     if (!mbar_wait(&ring.full[s], ph, kFaultWaitFull)) break;
-    const uint4* xs = reinterpret_cast<const uint4*>(rows + s * stage);
-    [[maybe_unused]] const uint4* rs = reinterpret_cast<const uint4*>(rows + s * stage + bytes);
+    const uint8_t* at = rows + s * stage;
     Run<V> a[N];
     float2 squares = make_float2(0.f, 0.f);
     float big = 0.f;
-    constexpr bool kPackedMax = !NORM && V == 8;
+    constexpr bool kPackedMax = !NORM && SG == 0 && V == 8;
     [[maybe_unused]] __nv_bfloat162 big2 = __floats2bfloat162_rn(0.f, 0.f);
+    if constexpr (SG != 0) {
+      auto read = [&](const void* base, int64_t ld, const uint8_t* here, Run<V>(&v)[N]) {
+        const Span sp = row_span<T>(base, ld, p.M, row, bytes);
+        if (sp.direct) {
+#pragma unroll
+          for (int i = 0; i < N; ++i) load<T, SG>(static_cast<const T*>(base) + row * ld, t, i, G, p.K, v[i]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < N; ++i) load<T, SG>(reinterpret_cast<const T*>(here + sp.skip), t, i, G, p.K, v[i]);
+        }
+      };
+      read(p.x, p.ldx, at, a);
+      if constexpr (RES) {
+        Run<V> b[N];
+        read(p.res, p.ldr, at + pitch, b);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+          for (int j = 0; j < V / 2; ++j) a[i].v[j] = add2(a[i].v[j], b[i].v[j]);
+      }
+    }
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int v = t + i * G, c = v * V;
-      if (c < p.K) {
-        const uint4 raw = xs[v];
-        expand<T>(raw, a[i]);
-        if constexpr (RES) {
-          Run<V> b;
-          expand<T>(rs[v], b);
+      if (R::any(t, i, G, p.K)) {
+        if constexpr (SG == 0) {
+          const uint4 raw = reinterpret_cast<const uint4*>(at)[t + i * G];
+          expand<T>(raw, a[i]);
+          if constexpr (kPackedMax) max_magnitude8(raw, big2);
+          if constexpr (RES) {
+            Run<V> b;
+            expand<T>(reinterpret_cast<const uint4*>(at + pitch)[t + i * G], b);
 #pragma unroll
-          for (int j = 0; j < V / 2; ++j) a[i].v[j] = add2(a[i].v[j], b.v[j]);
-          store<T, 0>(static_cast<T*>(p.h) + row * p.ldh, t, i, G, p.K, a[i]);
+            for (int j = 0; j < V / 2; ++j) a[i].v[j] = add2(a[i].v[j], b.v[j]);
+          }
         }
+        if constexpr (RES) store<T, SG>(static_cast<T*>(p.h) + row * p.ldh, t, i, G, p.K, a[i]);
         Run<V> w;
-        if constexpr (NORM) load_weight<T, 0>(p.weight, t, i, G, p.K, w);
-        if constexpr (kPackedMax) max_magnitude8(raw, big2);
-        else accumulate<NORM, V>(a[i], w, squares, big);
+        if constexpr (NORM) load_weight<T, SG>(p.weight, t, i, G, p.K, w);
+        if constexpr (!kPackedMax) accumulate<NORM, V>(a[i], w, squares, big);
       }
     }
     if constexpr (kPackedMax) big = max_magnitude(0.f, __low2float(big2), __high2float(big2));
@@ -507,7 +606,7 @@ __global__ void __launch_bounds__(1024) ring_rows_kernel(const FwdArgs p) {
     int8_t* q = p.q + row * p.ldq;
 #pragma unroll
     for (int i = 0; i < N; ++i)
-      if (Runs<T, 0>::any(t, i, G, p.K)) store_q<T, 0>(q, t, i, G, p.K, a[i], r);
+      if (R::any(t, i, G, p.K)) store_q<T, SG>(q, t, i, G, p.K, a[i], r);
     if (t == 0) row_outputs(p, row, sum, r, NORM);
     if (++s == p.stages) { s = 0; ph ^= 1u; }
   }
@@ -590,13 +689,29 @@ __global__ void __launch_bounds__(512) norm_bwd_kernel(const BwdArgs p) {
   __shared__ RowRing ring;
   const int t = threadIdx.x, G = blockDim.x;
   const uint32_t bytes = static_cast<uint32_t>(p.K) * sizeof(T);
-  const uint32_t stage = (p.dh ? 3u : 2u) * bytes;
+  const uint32_t pitch = row_pitch(bytes, SG == 0);
+  const uint32_t stage = (p.dh ? 3u : 2u) * pitch;
   auto fill = [&](int s, int64_t row) {
-    mbar_arrive_expect_tx(&ring.full[s], stage);
     uint8_t* to = rows + s * stage;
-    bulk_load(to, static_cast<const T*>(p.dy) + row * p.ldy, bytes, &ring.full[s]);
-    bulk_load(to + bytes, static_cast<const T*>(p.h) + row * p.ldhh, bytes, &ring.full[s]);
-    if (p.dh) bulk_load(to + 2 * bytes, static_cast<const T*>(p.dh) + row * p.lddh, bytes, &ring.full[s]);
+    if constexpr (SG == 0) {
+      mbar_arrive_expect_tx(&ring.full[s], stage);
+      bulk_load(to, static_cast<const T*>(p.dy) + row * p.ldy, bytes, &ring.full[s]);
+      bulk_load(to + pitch, static_cast<const T*>(p.h) + row * p.ldhh, bytes, &ring.full[s]);
+      if (p.dh) bulk_load(to + 2 * pitch, static_cast<const T*>(p.dh) + row * p.lddh, bytes, &ring.full[s]);
+    } else {
+      Span sp[3];
+      sp[0] = row_span<T>(p.dy, p.ldy, p.M, row, bytes);
+      sp[1] = row_span<T>(p.h, p.ldhh, p.M, row, bytes);
+      sp[2] = row_span<T>(p.dh, p.lddh, p.M, row, bytes);
+      if (!p.dh) sp[2].direct = true;
+      uint32_t tx = 0u;
+#pragma unroll
+      for (int k = 0; k < 3; ++k) tx += sp[k].direct ? 0u : sp[k].size;
+      mbar_arrive_expect_tx(&ring.full[s], tx);
+#pragma unroll
+      for (int k = 0; k < 3; ++k)
+        if (!sp[k].direct) bulk_load(to + k * pitch, sp[k].from, sp[k].size, &ring.full[s]);
+    }
   };
   if constexpr (RING) {
     if (t == 0) {
@@ -624,26 +739,40 @@ __global__ void __launch_bounds__(512) norm_bwd_kernel(const BwdArgs p) {
   for (; row < p.M; row += gridDim.x) {
     const float rs = __ldg(p.rstd + row);
     Run<V> g[N], xh[N], d[N];
+    const T* from[3] = {static_cast<const T*>(p.dy) + row * p.ldy, static_cast<const T*>(p.h) + row * p.ldhh,
+                        p.dh ? static_cast<const T*>(p.dh) + row * p.lddh : nullptr};
     if constexpr (RING) {
       if (!mbar_wait(&ring.full[s], ph, kFaultWaitFull)) break;
     }
+    auto read = [&](int k, const void* base, int64_t ld, Run<V>(&v)[N]) {
+      bool buffered = RING;
+      uint32_t skip = 0u;
+      if constexpr (RING && SG != 0) {
+        const Span sp = row_span<T>(base, ld, p.M, row, bytes);
+        buffered = !sp.direct;
+        skip = sp.skip;
+      }
+      const uint8_t* here = rows + s * stage + k * pitch + skip;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      clear(g[i]);
-      clear(xh[i]);
-      clear(d[i]);
-      if (R::any(t, i, G, p.K)) {
-        if constexpr (RING) {
-          const uint4* from = reinterpret_cast<const uint4*>(rows + s * stage) + (t + i * G);
-          expand<T>(from[0], g[i]);
-          expand<T>(from[bytes / 16], xh[i]);
-          if (p.dh) expand<T>(from[2 * (bytes / 16)], d[i]);
-        } else {
-          load<T, SG>(static_cast<const T*>(p.dy) + row * p.ldy, t, i, G, p.K, g[i]);
-          load<T, SG>(static_cast<const T*>(p.h) + row * p.ldhh, t, i, G, p.K, xh[i]);
-          if (p.dh) load<T, SG>(static_cast<const T*>(p.dh) + row * p.lddh, t, i, G, p.K, d[i]);
+      for (int i = 0; i < N; ++i) {
+        clear(v[i]);
+        if (R::any(t, i, G, p.K)) {
+          if constexpr (RING && SG == 0) {
+            expand<T>(reinterpret_cast<const uint4*>(here)[t + i * G], v[i]);
+          } else {
+            if (buffered) load<T, SG>(reinterpret_cast<const T*>(here), t, i, G, p.K, v[i]);
+            else load<T, SG>(from[k], t, i, G, p.K, v[i]);
+          }
         }
       }
+    };
+    read(0, p.dy, p.ldy, g);
+    read(1, p.h, p.ldhh, xh);
+    if (p.dh) {
+      read(2, p.dh, p.lddh, d);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) clear(d[i]);
     }
     float2 dots = make_float2(0.f, 0.f);
 #pragma unroll
@@ -791,51 +920,79 @@ inline int ring_stages(int threads, int regs, int64_t row_bytes, int* blocks) {
   return 0;
 }
 
-template <typename T, bool NORM, bool RES, int SG>
-cudaError_t launch_rows_sg(const FwdArgs& p, int threads, cudaStream_t st) {
+template <typename T, bool NORM, bool RES, int SG, int N>
+cudaError_t launch_block_rows(const FwdArgs& p, int threads, cudaStream_t st) {
   if (threads <= 32) {
     const int per = 4;
-    rows_kernel<T, NORM, RES, SG, true><<<(p.M + per - 1) / per, 32 * per, 0, st>>>(p);
+    rows_kernel<T, NORM, RES, SG, N, true><<<(p.M + per - 1) / per, 32 * per, 0, st>>>(p);
   } else {
-    rows_kernel<T, NORM, RES, SG, false><<<p.M, threads, 0, st>>>(p);
+    rows_kernel<T, NORM, RES, SG, N, false><<<p.M, threads, 0, st>>>(p);
   }
   return cudaGetLastError();
 }
 
-// 16 elements per thread; a row over 16 * 1024 elements takes two passes.
+// Rows through the ring, if they are many enough for it: at least `times` rows a block.
+template <typename T, bool NORM, bool RES, int SG, int N>
+bool launch_ring(FwdArgs p, int threads, int times, cudaError_t* err, cudaStream_t st) {
+  int per_sm = 0;
+  const int64_t row_bytes =
+      static_cast<int64_t>(row_pitch(static_cast<uint32_t>(p.K) * sizeof(T), SG == 0)) * (RES ? 2 : 1);
+  p.stages = ring_stages(threads, 64, row_bytes, &per_sm);
+  const int64_t grid = static_cast<int64_t>(sm_count()) * per_sm;
+  if (p.stages < 2 || p.M < times * grid) return false;
+  auto kern = ring_rows_kernel<T, NORM, RES, SG, N>;
+  static std::atomic<uint64_t> smem_set{0};
+  if (set_max_dynamic_smem(reinterpret_cast<const void*>(kern), kRingSmem, smem_set, "rows: set shared memory") != C3CU_OK)
+    return false;
+  kern<<<static_cast<unsigned>(grid), threads, static_cast<size_t>(p.stages * row_bytes), st>>>(p);
+  *err = cudaGetLastError();
+  return true;
+}
+
+// Rows off the 16-byte grid: 16 or 24 single elements per thread.
+template <typename T, bool NORM, bool RES, int SG>
+cudaError_t launch_strided(const FwdArgs& p, cudaStream_t st) {
+  [[maybe_unused]] cudaError_t err;
+  // Single fp32 elements have twice the bytes of bf16 ones in flight, and gain nothing from the ring.
+  constexpr bool kRing = sizeof(T) == 2 && SG >= 128;
+  if (p.K <= 16 * SG) {
+    if constexpr (kRing)
+      if (launch_ring<T, NORM, RES, SG, 2>(p, SG, 4, &err, st)) return err;
+    return launch_block_rows<T, NORM, RES, SG, 2>(p, SG, st);
+  }
+  if constexpr (kRing)
+    if (launch_ring<T, NORM, RES, SG, 3>(p, SG, 4, &err, st)) return err;
+  return launch_block_rows<T, NORM, RES, SG, 3>(p, SG, st);
+}
+
 template <typename T, bool NORM, bool RES>
-cudaError_t launch_rows(FwdArgs p, bool vec, cudaStream_t st) {
+cudaError_t launch_rows(const FwdArgs& p, bool vec, cudaStream_t st) {
   if (p.K > kRegRow) {
     if (vec) long_rows_kernel<T, NORM, RES, 0><<<p.M, 1024, 0, st>>>(p);
     else long_rows_kernel<T, NORM, RES, 1024><<<p.M, 1024, 0, st>>>(p);
     return cudaGetLastError();
   }
   if (!vec) {
-    if (p.K <= 32 * kRowElems) return launch_rows_sg<T, NORM, RES, 32>(p, 32, st);
-    if (p.K <= 128 * kRowElems) return launch_rows_sg<T, NORM, RES, 128>(p, 128, st);
-    if (p.K <= 256 * kRowElems) return launch_rows_sg<T, NORM, RES, 256>(p, 256, st);
-    if (p.K <= 512 * kRowElems) return launch_rows_sg<T, NORM, RES, 512>(p, 512, st);
-    return launch_rows_sg<T, NORM, RES, 1024>(p, 1024, st);
+    if (p.K <= 24 * 32) return launch_strided<T, NORM, RES, 32>(p, st);
+    if (p.K <= 24 * 128) return launch_strided<T, NORM, RES, 128>(p, st);
+    if (p.K <= 24 * 256) return launch_strided<T, NORM, RES, 256>(p, st);
+    if (p.K <= 24 * 512) return launch_strided<T, NORM, RES, 512>(p, st);
+    return launch_strided<T, NORM, RES, 1024>(p, st);
   }
-  // Elements per thread: quantising alone is short of issue slots (4096 wide: 243 instructions per
-  // warp and row at 16), and twice the elements halve what a row costs besides them.
-  constexpr int E = NORM ? kRowElems : 2 * kRowElems;
-  const int ring_threads = (p.K + E * 32 - 1) / (E * 32) * 32;
-  int per_sm = 0;
-  const int64_t row_bytes = static_cast<int64_t>(p.K) * sizeof(T) * (RES ? 2 : 1);
-  const int stages = ring_stages(ring_threads, 64, row_bytes, &per_sm);
-  const int64_t grid = static_cast<int64_t>(sm_count()) * per_sm;
-  const char* e = getenv("DEV_RING");
-  if (stages >= 2 && p.M >= 2 * grid && !(e && e[0]=='0')) {
-    auto kern = ring_rows_kernel<T, NORM, RES, E / Runs<T, 0>::V>;
-    static std::atomic<uint64_t> smem_set{0};
-    if (set_max_dynamic_smem(reinterpret_cast<const void*>(kern), kRingSmem, smem_set, "rows: set shared memory") == C3CU_OK) {
-      p.stages = stages;
-      kern<<<static_cast<unsigned>(grid), ring_threads, static_cast<size_t>(stages * row_bytes), st>>>(p);
-      return cudaGetLastError();
-    }
+  constexpr int V = Runs<T, 0>::V;
+  // The ring pays where a block per row has too little in flight or too few blocks fit: wide rows
+  // (us, ring / block per row, bf16: quantise 16384 x 4096 41 / 49, 5461 x 12288 42 / 69, norm
+  // 16384 x 4096 77 / 81; but quantise 65536 x 1024 51 / 43 and fp32 8192 x 4096 33 / 25), and once
+  // its blocks have several rows each.
+  if (p.K >= (sizeof(T) == 2 ? 4096 : 8200)) {
+    // Elements per thread: quantising alone is short of issue slots, and twice the elements halve
+    // what a row costs besides them.
+    constexpr int E = NORM ? kRowElems : 2 * kRowElems;
+    const int threads = (p.K + E * 32 - 1) / (E * 32) * 32;
+    cudaError_t err;
+    if (launch_ring<T, NORM, RES, 0, E / V>(p, threads, p.K > 8192 ? 2 : 8, &err, st)) return err;
   }
-  return launch_rows_sg<T, NORM, RES, 0>(p, (p.K + kRowElems * 32 - 1) / (kRowElems * 32) * 32, st);
+  return launch_block_rows<T, NORM, RES, 0, kRowElems / V>(p, (p.K + kRowElems * 32 - 1) / (kRowElems * 32) * 32, st);
 }
 
 template <typename T>
@@ -885,24 +1042,14 @@ size_t bwd_partial_rows(int64_t M, int64_t K, bool vec, int cols) {
   return static_cast<size_t>((M + rows - 1) / rows);
 }
 
-template <typename T>
-cudaError_t launch_bwd(BwdArgs p, bool vec, int rows, int threads, cudaStream_t st) {
-  if (!vec) {
-    switch (threads) {
-      case 32: norm_bwd_kernel<T, false, 32><<<rows, 32, 0, st>>>(p); break;
-      case 64: norm_bwd_kernel<T, false, 64><<<rows, 64, 0, st>>>(p); break;
-      case 128: norm_bwd_kernel<T, false, 128><<<rows, 128, 0, st>>>(p); break;
-      case 256: norm_bwd_kernel<T, false, 256><<<rows, 256, 0, st>>>(p); break;
-      default: norm_bwd_kernel<T, false, 512><<<rows, 512, 0, st>>>(p); break;
-    }
-    return cudaGetLastError();
-  }
-  const int64_t row_bytes = static_cast<int64_t>(p.K) * sizeof(T) * (p.dh ? 3 : 2);
+template <typename T, int SG>
+cudaError_t launch_bwd(BwdArgs p, int rows, int threads, cudaStream_t st) {
+  const int64_t row_bytes =
+      static_cast<int64_t>(row_pitch(static_cast<uint32_t>(p.K) * sizeof(T), SG == 0)) * (p.dh ? 3 : 2);
   int64_t stages = (kRingSmem / bwd_blocks_per_sm(threads) - 2048) / row_bytes;
   if (stages > kMaxStages) stages = kMaxStages;
-  const char* e = getenv("DEV_RING");
-  if (stages >= 2 && p.M >= 2 * rows && !(e && e[0] == '0')) {
-    auto kern = norm_bwd_kernel<T, true, 0>;
+  if (stages >= 2 && p.M >= 2 * rows) {
+    auto kern = norm_bwd_kernel<T, true, SG>;
     static std::atomic<uint64_t> smem_set{0};
     if (set_max_dynamic_smem(reinterpret_cast<const void*>(kern), kRingSmem, smem_set,
                              "rms_norm_bwd: set shared memory") == C3CU_OK) {
@@ -911,8 +1058,20 @@ cudaError_t launch_bwd(BwdArgs p, bool vec, int rows, int threads, cudaStream_t 
       return cudaGetLastError();
     }
   }
-  norm_bwd_kernel<T, false, 0><<<rows, threads, 0, st>>>(p);
+  norm_bwd_kernel<T, false, SG><<<rows, threads, 0, st>>>(p);
   return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t launch_bwd_rows(const BwdArgs& p, bool vec, int rows, int threads, cudaStream_t st) {
+  if (vec) return launch_bwd<T, 0>(p, rows, threads, st);
+  switch (threads) {
+    case 32: return launch_bwd<T, 32>(p, rows, threads, st);
+    case 64: return launch_bwd<T, 64>(p, rows, threads, st);
+    case 128: return launch_bwd<T, 128>(p, rows, threads, st);
+    case 256: return launch_bwd<T, 256>(p, rows, threads, st);
+    default: return launch_bwd<T, 512>(p, rows, threads, st);
+  }
 }
 
 template <typename T, int SG>
@@ -931,7 +1090,7 @@ int bwd(BwdArgs p, bool vec, float* ws, cudaStream_t st) {
   cudaError_t err;
   if (p.K <= kBwdMaxK) {
     p.partial = ws;
-    err = launch_bwd<T>(p, vec, rows, bwd_threads(p.K, vec), st);
+    err = launch_bwd_rows<T>(p, vec, rows, bwd_threads(p.K, vec), st);
   } else {
     p.partial = ws + p.M;
     err = vec ? launch_bwd_strips<T, 0>(p, ws, rows, st) : launch_bwd_strips<T, kStripThreads>(p, ws, rows, st);
