@@ -1035,6 +1035,7 @@ int bwd_blocks_per_sm(int threads) { return 512 / threads < 16 ? 512 / threads :
 // Rows of partial sums, one a block; `cols`: a strip's columns.
 size_t bwd_partial_rows(int64_t M, int64_t K, bool vec, int cols) {
   if (K <= kBwdMaxK) {
+    if (M <= 4) return 1;  // one block walks over them in less time than a second launch takes
     const int64_t most = static_cast<int64_t>(sm_count() > 0 ? sm_count() : 148) * bwd_blocks_per_sm(bwd_threads(K, vec));
     return static_cast<size_t>(M < most ? M : most);
   }

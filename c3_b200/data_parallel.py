@@ -228,14 +228,24 @@ class LinearReluTrainStep:
     forward (Y bf16 + bit-packed ReLU mask) → pre-pass (dZ, db) → dW GEMM in bands, each band's
     all-reduce on `comm` → dX GEMM → the compute stream waits for the last all-reduce.
     `reserve_sms` SMs are left to the collective while the dX GEMM overlaps it. With the
-    "fused" collective: forward → pre-pass → dW GEMM that sums dW and db over the ranks → dX."""
+    "fused" collective: forward → pre-pass → dW GEMM that sums dW and db over the ranks → dX.
+
+    `x_checkpoint="int8"` keeps the layer's input between forward and dW as int8 rows with a scale
+    each (`Xq`, `x_scale`, half of X's bytes): dW then comes from them (linear.grad_weight_int8), so
+    a model of many layers can let each X go after its forward. It needs a bf16 dW that is not
+    summed by the GEMM itself."""
 
     PHASES = ("fwd", "prepass", "dw", "dx")
 
     def __init__(self, m: int, n: int, k: int, device: torch.device, grad_dtype=torch.bfloat16,
                  collective: str = "auto", group=None, chunks: int = 1, num_ctas: int = 16,
-                 reserve_sms: int = 0, overlap_dx: bool = False, peer_frac: float = 0.0, peer_ctas: int = 0):
-        from . import _lib
+                 reserve_sms: int = 0, overlap_dx: bool = False, peer_frac: float = 0.0, peer_ctas: int = 0,
+                 x_checkpoint: str = "bf16"):
+        from . import _lib, quant
+        if x_checkpoint not in ("bf16", "int8"):
+            raise ValueError(f"x_checkpoint must be 'bf16' or 'int8', got {x_checkpoint!r}")
+        if x_checkpoint == "int8" and (grad_dtype != torch.bfloat16 or collective == "fused"):
+            raise ValueError("an int8 checkpoint of X gives a bf16 dW, summed over the ranks after the GEMM")
         self.m, self.n, self.k = m, n, k
         self.device = torch.device(device)
         self.sync = GradientSync(n, k, self.device, grad_dtype, collective, group, num_ctas, peer_frac, peer_ctas)
@@ -248,6 +258,10 @@ class LinearReluTrainStep:
         self.mask = torch.empty((m, (n + 31) // 32), dtype=torch.int32, device=dev)
         self.dZ = torch.empty((m, n), dtype=torch.bfloat16, device=dev)
         self.dX = torch.empty((m, k), dtype=torch.bfloat16, device=dev)
+        self.Xq = self.x_scale = None
+        if x_checkpoint == "int8":
+            self.Xq = quant.empty_rows(m, k, dev)
+            self.x_scale = torch.empty(m, dtype=torch.float32, device=dev)
         self.comm = torch.cuda.Stream(dev)
         # overlap_dx: dX (which needs only dZ and W) runs on its own stream beside dW, so its tiles
         # fill the SMs that dW's last wave leaves idle
@@ -270,8 +284,16 @@ class LinearReluTrainStep:
     def db(self) -> torch.Tensor:
         return self.sync.db
 
+    def _grad_weight(self, dZ, X, dW):
+        """dW [rows, k] of dZ's columns, from X or its int8 checkpoint."""
+        from . import linear
+        if self.Xq is not None:
+            linear.grad_weight_int8(dZ, self.Xq, self.x_scale, dW=dW)
+        else:
+            linear.gemm(dZ, X, True, True, self.epi, dW, M=dZ.shape[1], N=self.k, K=self.m)
+
     def __call__(self, X, W, b, dY, record: bool = False) -> StepEvents | None:
-        from . import _lib, linear
+        from . import _lib, linear, quant
         comp = torch.cuda.current_stream(self.device)
         phases: dict = {}
         ar: list = []
@@ -295,6 +317,8 @@ class LinearReluTrainStep:
             return StepEvents(out, ar)
 
         mark("fwd"); linear.forward(X, W, b, "nk", self.Y, self.mask); mark("fwd")
+        if self.Xq is not None:
+            quant.quantize_rows(X, self.Xq, self.x_scale)
         mark("prepass"); linear.relu_mask_db(dY, self.mask, self.dZ, self.db); mark("prepass")
         if self.overlap_dx:
             # dW (with its sum over the ranks when fused) on the compute stream, dX beside it;
@@ -306,7 +330,7 @@ class LinearReluTrainStep:
             if self.sync.fused:
                 self.sync.gemm_dw_reduce_(self.dZ, X, comp)
             else:
-                linear.gemm(self.dZ, X, True, True, self.epi, self.dW, M=self.n, N=self.k, K=self.m)
+                self._grad_weight(self.dZ, X, self.dW)
             mark("dw")
             with torch.cuda.stream(self.side):
                 mark_on("dx", self.side)
@@ -332,7 +356,7 @@ class LinearReluTrainStep:
             # it its SMs, as for dX
             if lib is not None and i > 0:
                 lib.c3cu_set_gemm_max_ctas(self._sms - self.reserve_sms)
-            linear.gemm(self.dZ[:, r0:r1], X, True, True, self.epi, self.dW[r0:r1], M=r1 - r0, N=k, K=m)
+            self._grad_weight(self.dZ[:, r0:r1], X, self.dW[r0:r1])
             if lib is not None and i > 0:
                 lib.c3cu_set_gemm_max_ctas(0)
             if self.world > 1:

@@ -80,6 +80,55 @@ def _ld(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else (t.shape[1] + 15) // 16 * 16
 
 
+# The wrappers of the 8-bit path serve single tokens, whose kernels take a few microseconds: their
+# checks accept a well-formed operand with a handful of attribute reads, and leave saying what is
+# wrong with any other to _require and _require_rows. `dev` is the first operand's device index.
+_current_device = torch._C._cuda_getDevice
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _rows_of(t: torch.Tensor, name: str, dtype: torch.dtype, rows: int, cols: int, dev: int) -> int:
+    """Checks a 2-D operand (a column slice of a wider matrix may be one) and returns its row stride."""
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == (rows, cols) and t.get_device() == dev >= 0:
+        ld, step = t.stride()
+        if step == 1:
+            if rows <= 1:
+                return (cols + 15) // 16 * 16
+            if ld >= cols:
+                return ld
+    _require_rows(t, name, dtype, rows, cols)
+    _same_device(t, name, dev)
+    return _ld(t)
+
+
+def _vector_of(t: torch.Tensor, name: str, dtype: torch.dtype, n: int, dev: int) -> None:
+    if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == (n,) and t.get_device() == dev >= 0
+            and t.is_contiguous()):
+        _require(t, name, dtype, 1, (n,))
+        _same_device(t, name, dev)
+
+
+def _same_device(t: torch.Tensor, name: str, dev: int) -> None:
+    if t.get_device() != dev:
+        raise _lib.C3CUError(-1, name, f"on device {t.get_device()}, the first operand on {dev}")
+
+
+def _call(name: str, dev: int, *args) -> None:
+    """Calls an entry point of the C ABI, whose last argument is the stream, on device `dev`."""
+    fn = getattr(_lib.load(), name)
+    if dev == _current_device():
+        rc = fn(*args, _raw_stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, _raw_stream(dev))
+    if rc != _lib.OK:
+        _lib.check(rc, name)
+
+
+def _ptr(t: torch.Tensor | None) -> int | None:
+    return None if t is None else t.data_ptr()
+
+
 def workspace(device: torch.device, nbytes: int) -> torch.Tensor:
     """Scratch of the column-sum kernels (per-block partial sums), one buffer per (device,
     stream): launches on different streams never share partials. It is allocated while its
@@ -238,7 +287,6 @@ def gemm(A: torch.Tensor, B: torch.Tensor, a_mn: bool, b_mn: bool, epilogue: int
     return out
 
 
-@_lib.on_tensor_device
 def forward_int8(Xq: torch.Tensor, x_scale: torch.Tensor, Wq: torch.Tensor, w_scale: torch.Tensor,
                  b: torch.Tensor | None = None, relu: bool = True, out_dtype: torch.dtype = torch.bfloat16,
                  Y: torch.Tensor | None = None, mask: torch.Tensor | None = None, save_mask: bool = True):
@@ -252,7 +300,11 @@ def forward_int8(Xq: torch.Tensor, x_scale: torch.Tensor, Wq: torch.Tensor, w_sc
     of `forward` (else None), from which `relu_mask_db` starts the backward pass."""
     if Y is not None:
         out_dtype = Y.dtype
-    if out_dtype not in (torch.bfloat16, torch.float32):
+    if out_dtype is torch.bfloat16:
+        code = _lib.DTYPE_BF16
+    elif out_dtype is torch.float32:
+        code = _lib.DTYPE_F32
+    else:
         raise _lib.C3CUError(-1, "Y", f"Y must be float32 or bfloat16, got {out_dtype}")
     for t, name in ((Xq, "Xq"), (Wq, "Wq")):
         if not isinstance(t, torch.Tensor) or t.dim() != 2:
@@ -261,31 +313,30 @@ def forward_int8(Xq: torch.Tensor, x_scale: torch.Tensor, Wq: torch.Tensor, w_sc
     N = Wq.shape[0]
     if not 1 <= K <= INT8_MAX_K:
         raise _lib.C3CUError(-1, "Xq", f"K = {K} outside [1, {INT8_MAX_K}]")
-    _require_rows(Xq, "Xq", torch.int8, M, K)
-    _require_rows(Wq, "Wq", torch.int8, N, K)
-    _require(x_scale, "x_scale", torch.float32, 1, (M,))
-    _require(w_scale, "w_scale", torch.float32, 1, (N,))
+    dev = Xq.get_device()
+    ldx = _rows_of(Xq, "Xq", torch.int8, M, K, dev)
+    ldw = _rows_of(Wq, "Wq", torch.int8, N, K, dev)
+    _vector_of(x_scale, "x_scale", torch.float32, M, dev)
+    _vector_of(w_scale, "w_scale", torch.float32, N, dev)
     if b is not None:
-        _require(b, "b", torch.float32, 1, (N,))
-    if Y is None:
-        Y = torch.empty(M, N, dtype=out_dtype, device=Xq.device)
-    else:
-        _require_rows(Y, "Y", out_dtype, M, N)
+        _vector_of(b, "b", torch.float32, N, dev)
+    words = (N + 31) // 32
+    ldy, ldm = N, words
+    if Y is not None:
+        ldy = _rows_of(Y, "Y", out_dtype, M, N, dev)
     if mask is not None:
         if not (relu and save_mask):
             raise _lib.C3CUError(-1, "mask", "a mask belongs to the ReLU output (relu and save_mask)")
-        _require_rows(mask, "mask", torch.int32, M, mask_words(N))
-    elif relu and save_mask:
-        mask = torch.empty(M, mask_words(N), dtype=torch.int32, device=Xq.device)
-    rc = _lib.load().c3cu_linear_int8_fwd(_p(Xq), _ld(Xq), _p(x_scale), _p(Wq), _ld(Wq), _p(w_scale), _p(b), _p(Y),
-                                          _ld(Y), _lib.DTYPE_F32 if out_dtype == torch.float32 else _lib.DTYPE_BF16,
-                                          1 if relu else 0, _p(mask), 0 if mask is None else _ld(mask), M, N, K,
-                                          _stream(Xq.device))
-    _lib.check(rc, "c3cu_linear_int8_fwd")
+        ldm = _rows_of(mask, "mask", torch.int32, M, words, dev)
+    if Y is None:
+        Y = torch.empty(M, N, dtype=out_dtype, device=Xq.device)
+    if mask is None and relu and save_mask:
+        mask = torch.empty(M, words, dtype=torch.int32, device=Xq.device)
+    _call("c3cu_linear_int8_fwd", dev, Xq.data_ptr(), ldx, x_scale.data_ptr(), Wq.data_ptr(), ldw, w_scale.data_ptr(),
+          _ptr(b), Y.data_ptr(), ldy, code, 1 if relu else 0, _ptr(mask), ldm, M, N, K)
     return Y, mask
 
 
-@_lib.on_tensor_device
 def grad_weight_int8(dZ: torch.Tensor, Xq: torch.Tensor, x_scale: torch.Tensor, dW: torch.Tensor | None = None):
     """dW = dZ^T (Xq * x_scale) as bf16 [N, K]: `grad_weight` ("nk") with the layer's input kept in 8
     bits (quant.quantize_rows of a bf16 activation, or the int8 rows that went into forward_int8).
@@ -297,18 +348,22 @@ def grad_weight_int8(dZ: torch.Tensor, Xq: torch.Tensor, x_scale: torch.Tensor, 
             raise _lib.C3CUError(-1, name, "expected a 2-D tensor")
     M, N = dZ.shape
     K = Xq.shape[1]
-    _require_rows(dZ, "dZ", torch.bfloat16, M, N)
-    _require_rows(Xq, "Xq", torch.int8, M, K)
-    _require(x_scale, "x_scale", torch.float32, 1, (M,))
-    if dW is None:
-        dW = torch.empty(N, K, dtype=torch.bfloat16, device=dZ.device)
+    dev = dZ.get_device()
+    lddz = _rows_of(dZ, "dZ", torch.bfloat16, M, N, dev)
+    ldx = _rows_of(Xq, "Xq", torch.int8, M, K, dev)
+    _vector_of(x_scale, "x_scale", torch.float32, M, dev)
+    lddw = K
+    if dW is not None:
+        lddw = _rows_of(dW, "dW", torch.bfloat16, N, K, dev)
     else:
-        _require_rows(dW, "dW", torch.bfloat16, N, K)
-    L = _lib.load()
-    nb = L.c3cu_gemm_dw_int8_workspace(M, N, K)
-    # of this call alone: a graph that captures it keeps its own
+        dW = torch.empty(N, K, dtype=torch.bfloat16, device=dZ.device)
+    # the workspace is of this call alone: a graph that captures it keeps its own
+    if dev == _current_device():
+        nb = _lib.load().c3cu_gemm_dw_int8_workspace(M, N, K)
+    else:
+        with torch.cuda.device(dev):
+            nb = _lib.load().c3cu_gemm_dw_int8_workspace(M, N, K)
     ws = torch.empty(nb, dtype=torch.uint8, device=dZ.device) if nb else None
-    rc = L.c3cu_gemm_dw_int8(_p(dZ), _ld(dZ), _p(Xq), _ld(Xq), _p(x_scale), _p(dW), _ld(dW), M, N, K, _p(ws), nb,
-                             _stream(dZ.device))
-    _lib.check(rc, "c3cu_gemm_dw_int8")
+    _call("c3cu_gemm_dw_int8", dev, dZ.data_ptr(), lddz, Xq.data_ptr(), ldx, x_scale.data_ptr(), dW.data_ptr(), lddw, M,
+          N, K, _ptr(ws), nb)
     return dW

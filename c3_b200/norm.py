@@ -11,11 +11,10 @@ import math
 import torch
 
 from . import _lib
-from .linear import _ld, _p, _require, _require_rows, _stream
-from .quant import _dtype_code, empty_rows
+from .linear import _call, _current_device, _ptr, _rows_of, _vector_of
+from .quant import _dtype_code, empty_rows, row_stride
 
 
-@_lib.on_tensor_device
 def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual: torch.Tensor | None = None,
                   q: torch.Tensor | None = None, scale: torch.Tensor | None = None, h: torch.Tensor | None = None,
                   rstd: torch.Tensor | None = None):
@@ -29,67 +28,61 @@ def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, resi
     M, K = x.shape
     if K < 1:
         raise _lib.C3CUError(-1, "x", "rows need at least one element")
-    _require_rows(x, "x", x.dtype, M, K)
-    _require(weight, "weight", torch.float32, 1, (K,))
     eps = float(eps)
     if not 0.0 <= eps < math.inf:
         raise _lib.C3CUError(-1, "eps", f"expected a finite eps >= 0, got {eps}")
+    dev, dtype = x.get_device(), x.dtype
+    ldx = _rows_of(x, "x", dtype, M, K, dev)
+    _vector_of(weight, "weight", torch.float32, K, dev)
+    ldr = ldh = K
     if residual is None:
         if h is not None:
             raise _lib.C3CUError(-1, "h", "without a residual h is x itself")
     else:
-        _require_rows(residual, "residual", x.dtype, M, K)
-        if h is None:
-            h = torch.empty(M, K, dtype=x.dtype, device=x.device)
+        ldr = _rows_of(residual, "residual", dtype, M, K, dev)
+        if h is not None:
+            ldh = _rows_of(h, "h", dtype, M, K, dev)
+            _require_same_rows_or_apart(h, ldh, "h", ((x, ldx, "x"), (residual, ldr, "residual")))
         else:
-            _require_rows(h, "h", x.dtype, M, K)
-            _require_same_rows_or_apart(h, "h", ((x, "x"), (residual, "residual")))
+            h = torch.empty(M, K, dtype=dtype, device=x.device)
     if q is None:
-        q = empty_rows(M, K, x.device)
+        q, ldq = empty_rows(M, K, x.device), row_stride(K)
     else:
-        _require_rows(q, "q", torch.int8, M, K)
+        ldq = _rows_of(q, "q", torch.int8, M, K, dev)
     if scale is None:
         scale = torch.empty(M, dtype=torch.float32, device=x.device)
     else:
-        _require(scale, "scale", torch.float32, 1, (M,))
+        _vector_of(scale, "scale", torch.float32, M, dev)
     if rstd is None:
         rstd = torch.empty(M, dtype=torch.float32, device=x.device)
     else:
-        _require(rstd, "rstd", torch.float32, 1, (M,))
-    has = residual is not None
-    rc = _lib.load().c3cu_rms_norm_int8(_p(x), _ld(x), _p(residual), _ld(residual) if has else 0, code, _p(weight), eps,
-                                        _p(h), _ld(h) if has else 0, _p(q), _ld(q), _p(scale), _p(rstd), M, K,
-                                        _stream(x.device))
-    _lib.check(rc, "c3cu_rms_norm_int8")
-    return q, scale, h if has else x, rstd
+        _vector_of(rstd, "rstd", torch.float32, M, dev)
+    _call("c3cu_rms_norm_int8", dev, x.data_ptr(), ldx, _ptr(residual), ldr, code, weight.data_ptr(), eps, _ptr(h), ldh,
+          q.data_ptr(), ldq, scale.data_ptr(), rstd.data_ptr(), M, K)
+    return q, scale, x if h is None else h, rstd
 
 
-def _require_same_rows_or_apart(out: torch.Tensor, name: str, inputs) -> None:
+def _require_same_rows_or_apart(out: torch.Tensor, ld: int, name: str, inputs) -> None:
     """An output may be an input's own rows (each element is read before it is written, by the same
-    thread), but may not overlap one in any other way."""
-    if out.numel() == 0:
+    thread) or other columns of the same buffer, but may not overlap one in any other way. All have
+    one shape and type; `ld` and the inputs' middle entries are row strides."""
+    rows, cols = out.shape
+    if rows == 0:
         return
-    for t, other in inputs:
-        if t is None or (t.data_ptr() == out.data_ptr() and _ld(t) == _ld(out)):
+    size = out.element_size()
+    a, width = out.data_ptr(), cols * size
+    for t, ldt, other in inputs:
+        if t is None:
             continue
-        a, b = out.data_ptr(), t.data_ptr()
-        ea = a + ((out.shape[0] - 1) * out.stride(0) + out.shape[1]) * out.element_size()
-        eb = b + ((t.shape[0] - 1) * t.stride(0) + t.shape[1]) * t.element_size()
-        if a < eb and b < ea and not _disjoint_columns(out, t):
-            raise _lib.C3CUError(-1, name, f"overlaps {other} without being the same rows")
+        b = t.data_ptr()
+        if a == b and (ld == ldt or rows == 1):
+            continue
+        if a < b + ((rows - 1) * ldt + cols) * size and b < a + ((rows - 1) * ld + cols) * size:
+            off = (b - a) % (ld * size)
+            if rows == 1 or ld != ldt or off < width or off + width > ld * size:
+                raise _lib.C3CUError(-1, name, f"overlaps {other} without being the same rows")
 
 
-def _disjoint_columns(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether two matrices of one row stride are different columns of one buffer."""
-    if a.shape[0] <= 1 or a.stride(0) != b.stride(0) or a.element_size() != b.element_size():
-        return False
-    ld = a.stride(0) * a.element_size()
-    off = (b.data_ptr() - a.data_ptr()) % ld
-    width = a.shape[1] * a.element_size()
-    return off >= width and off + b.shape[1] * b.element_size() <= ld
-
-
-@_lib.on_tensor_device
 def rms_norm_backward(dy: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, rstd: torch.Tensor,
                       dh: torch.Tensor | None = None, dx: torch.Tensor | None = None,
                       dweight: torch.Tensor | None = None):
@@ -103,26 +96,30 @@ def rms_norm_backward(dy: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, r
     M, K = h.shape
     if K < 1:
         raise _lib.C3CUError(-1, "h", "rows need at least one element")
-    _require_rows(h, "h", h.dtype, M, K)
-    _require_rows(dy, "dy", h.dtype, M, K)
+    dev, dtype = h.get_device(), h.dtype
+    ldh = _rows_of(h, "h", dtype, M, K, dev)
+    ldy = _rows_of(dy, "dy", dtype, M, K, dev)
+    lddh = lddx = K
     if dh is not None:
-        _require_rows(dh, "dh", h.dtype, M, K)
-    _require(weight, "weight", torch.float32, 1, (K,))
-    _require(rstd, "rstd", torch.float32, 1, (M,))
-    if dx is None:
-        dx = torch.empty(M, K, dtype=h.dtype, device=h.device)
+        lddh = _rows_of(dh, "dh", dtype, M, K, dev)
+    _vector_of(weight, "weight", torch.float32, K, dev)
+    _vector_of(rstd, "rstd", torch.float32, M, dev)
+    if dx is not None:
+        lddx = _rows_of(dx, "dx", dtype, M, K, dev)
+        _require_same_rows_or_apart(dx, lddx, "dx", ((dy, ldy, "dy"), (h, ldh, "h"), (dh, lddh, "dh")))
     else:
-        _require_rows(dx, "dx", h.dtype, M, K)
-        _require_same_rows_or_apart(dx, "dx", ((dy, "dy"), (h, "h"), (dh, "dh")))
+        dx = torch.empty(M, K, dtype=dtype, device=h.device)
     if dweight is None:
         dweight = torch.empty(K, dtype=torch.float32, device=h.device)
     else:
-        _require(dweight, "dweight", torch.float32, 1, (K,))
-    L = _lib.load()
-    nb = L.c3cu_rms_norm_bwd_workspace(M, K)
-    # of this call alone: a graph that captures it keeps its own
+        _vector_of(dweight, "dweight", torch.float32, K, dev)
+    # the workspace is of this call alone: a graph that captures it keeps its own
+    if dev == _current_device():
+        nb = _lib.load().c3cu_rms_norm_bwd_workspace(M, K)
+    else:
+        with torch.cuda.device(dev):
+            nb = _lib.load().c3cu_rms_norm_bwd_workspace(M, K)
     ws = torch.empty(nb, dtype=torch.uint8, device=h.device) if nb else None
-    rc = L.c3cu_rms_norm_bwd(_p(dy), _ld(dy), _p(h), _ld(h), _p(dh), _ld(dh) if dh is not None else 0, code, _p(weight),
-                             _p(rstd), _p(dx), _ld(dx), _p(dweight), M, K, _p(ws), nb, _stream(h.device))
-    _lib.check(rc, "c3cu_rms_norm_bwd")
+    _call("c3cu_rms_norm_bwd", dev, dy.data_ptr(), ldy, h.data_ptr(), ldh, _ptr(dh), lddh, code, weight.data_ptr(),
+          rstd.data_ptr(), dx.data_ptr(), lddx, dweight.data_ptr(), M, K, _ptr(ws), nb)
     return dx, dweight

@@ -9,7 +9,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .linear import _ld, _p, _require, _require_rows, _stream
+from .linear import _call, _rows_of, _vector_of
 
 _DTYPES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16}
 
@@ -17,20 +17,24 @@ _DTYPES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16}
 def _dtype_code(t, name: str) -> int:
     if not isinstance(t, torch.Tensor):
         raise _lib.C3CUError(-1, name, f"expected a torch.Tensor, got {type(t).__name__}")
-    if t.dtype not in _DTYPES or t.dim() != 2:
+    code = _DTYPES.get(t.dtype)
+    if code is None or t.dim() != 2:
         raise _lib.C3CUError(-1, name, f"expected 2-D float32 or bfloat16, got {t.dtype} {tuple(t.shape)}")
-    return _DTYPES[t.dtype]
+    return code
 
 
 def empty_rows(m: int, k: int, device) -> torch.Tensor:
-    """An uninitialised int8 [m, k] whose rows start on 16 bytes (a column slice of a wider buffer
-    unless k is a multiple of 16), as the int8 GEMMs read them."""
+    """An uninitialised int8 [m, k] whose rows start on 16 bytes, as the int8 GEMMs read them: a column
+    slice of a buffer `row_stride(k)` wide, unless k is a multiple of 16."""
     if k % 16 == 0:
         return torch.empty(m, k, dtype=torch.int8, device=device)
-    return torch.empty(m, (k + 15) // 16 * 16, dtype=torch.int8, device=device)[:, :k]
+    return torch.empty(m, row_stride(k), dtype=torch.int8, device=device)[:, :k]
 
 
-@_lib.on_tensor_device
+def row_stride(k: int) -> int:
+    return (k + 15) // 16 * 16
+
+
 def quantize_rows(x: torch.Tensor, q: torch.Tensor | None = None, scale: torch.Tensor | None = None):
     """(q int8 [M, K], scale fp32 [M]) of x [M, K] (bf16 or fp32, unit column stride, any row stride).
 
@@ -40,15 +44,15 @@ def quantize_rows(x: torch.Tensor, q: torch.Tensor | None = None, scale: torch.T
     M, K = x.shape
     if K < 1:
         raise _lib.C3CUError(-1, "x", "rows need at least one element")
-    _require_rows(x, "x", x.dtype, M, K)
+    dev = x.get_device()
+    ldx = _rows_of(x, "x", x.dtype, M, K, dev)
     if q is None:
-        q = empty_rows(M, K, x.device)
+        q, ldq = empty_rows(M, K, x.device), row_stride(K)
     else:
-        _require_rows(q, "q", torch.int8, M, K)
+        ldq = _rows_of(q, "q", torch.int8, M, K, dev)
     if scale is None:
         scale = torch.empty(M, dtype=torch.float32, device=x.device)
     else:
-        _require(scale, "scale", torch.float32, 1, (M,))
-    rc = _lib.load().c3cu_quantize_rows(_p(x), _ld(x), code, _p(q), _ld(q), _p(scale), M, K, _stream(x.device))
-    _lib.check(rc, "c3cu_quantize_rows")
+        _vector_of(scale, "scale", torch.float32, M, dev)
+    _call("c3cu_quantize_rows", dev, x.data_ptr(), ldx, code, q.data_ptr(), ldq, scale.data_ptr(), M, K)
     return q, scale

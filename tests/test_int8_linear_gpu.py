@@ -320,3 +320,34 @@ def test_cap_on_ctas_changes_no_bits(cuda_device):
         L.c3cu_set_gemm_max_ctas(0)
     assert torch.equal(y, y2) and torch.equal(mask, mask2)
     assert torch.equal(dw2, want)
+
+
+@pytest.mark.parametrize("options", [{}, {"overlap_dx": True}, {"chunks": 2}])
+def test_training_step_with_an_int8_checkpoint(cuda_device, options):
+    """LinearReluTrainStep(x_checkpoint="int8"): forward, mask, db and dX are those of the bf16 step,
+    bit for bit; dW is the product with the checkpoint, and near the bf16 step's."""
+    from c3_b200.data_parallel import LinearReluTrainStep
+    dev = cuda_device
+    m, n, k = 512, 384, 328
+    X = torch.randn((m, k), generator=_gen(dev, 1), device=dev).to(BF16)
+    W = (torch.randn((n, k), generator=_gen(dev, 2), device=dev) * 0.05).to(BF16)
+    b = torch.randn(n, generator=_gen(dev, 3), device=dev) * 0.05
+    dY = (torch.randn((m, n), generator=_gen(dev, 4), device=dev) * 1e-3).to(BF16)
+    ref = LinearReluTrainStep(m, n, k, dev, **options)
+    step = LinearReluTrainStep(m, n, k, dev, x_checkpoint="int8", **options)
+    ref(X, W, b, dY)
+    step(X, W, b, dY)
+    torch.cuda.synchronize()
+    for name in ("Y", "mask", "dZ", "db", "dX"):
+        assert torch.equal(getattr(step, name), getattr(ref, name)), name
+    q, s = quant.quantize_rows(X)
+    assert torch.equal(step.Xq, q) and torch.equal(step.x_scale, s)
+    want = step.dZ.double().t() @ (q.double() * s.double()[:, None])
+    assert float((step.dW.double() - want).norm() / want.norm()) <= 2.0 ** -8
+    # a checkpoint's element is off by at most half a step, A / 254, that is about 3.5 / 254 of the
+    # rows' standard deviation at most, uniformly: 0.8 % of the norm
+    assert float((step.dW.double() - ref.dW.double()).norm() / ref.dW.double().norm()) <= 0.02
+    for bad in ({"x_checkpoint": "int4"}, {"x_checkpoint": "int8", "grad_dtype": torch.float32},
+                {"x_checkpoint": "int8", "collective": "fused"}):
+        with pytest.raises(ValueError):
+            LinearReluTrainStep(m, n, k, dev, **bad)
