@@ -128,6 +128,28 @@ def load(build_if_missing: bool = True) -> ctypes.CDLL:
         return L
 
 
+_FAST_ENTRIES = ("c3cu_quantize_rows", "c3cu_rms_norm_int8", "c3cu_rms_norm_bwd_workspace", "c3cu_rms_norm_bwd",
+                 "c3cu_linear_int8_fwd", "c3cu_gemm_dw_int8_workspace", "c3cu_gemm_dw_int8")
+_fast = None
+
+
+def fast():
+    """The module of csrc/torch/fast_calls.cpp, bound to this library's entry points."""
+    global _fast
+    if _fast is not None:
+        return _fast
+    L = load()
+    with _lock:
+        if _fast is None:
+            from . import build as _build
+            if not _build.FAST_CALLS.exists():
+                _build.build_fast_calls()
+            from . import _fast_calls
+            _fast_calls.bind(*(ctypes.cast(getattr(L, n), _vp).value for n in _FAST_ENTRIES))
+            _fast = _fast_calls
+    return _fast
+
+
 def last_error() -> str:
     msg = load().c3cu_last_error()
     return msg.decode() if msg else ""

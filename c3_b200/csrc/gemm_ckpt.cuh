@@ -8,13 +8,17 @@
 // output's own) is the only one besides the output's; q itself would be exact in bf16.
 //
 // dw_kernel has gemm2_kernel's structure (256 x 256 tiles on CTA pairs, both operands MN-major,
-// since dZ and X are stored with the sum's index as their rows), in two forms:
+// since dZ and X are stored with the sum's index as their rows). The MMA's rows are the columns of
+// dW, so that a warp's stores run along its rows whatever their alignment (2176 x 4822 over 576 rows:
+// 138 us with a row of dW per lane, 27 so). Two forms:
 //   RAW   TMA brings X's int8 block into a raw buffer and converter warps widen it into the
 //         swizzled bf16 tile that the MMA reads: X crosses HBM and L2 at one byte per element and
 //         no bf16 copy of it exists, but it is widened once for every 256 rows of dW.
 //   !RAW  X was widened once into a bf16 workspace (widen_kernel), which the kernel reads by TMA.
-// The widening in the kernel costs more than its instructions: beside the tensor cores it runs
-// into the power limit. XXX
+// Beside the tensor cores the widening runs into the power limit and the shared-memory traffic of
+// the tiles (16384 x 4096 x 4096: 505 to 548 us RAW, 424 !RAW, of which widen_kernel 33; the bf16
+// gradient from a bf16 X takes 350 to 370 in the same loop). With few K blocks RAW saves the launch
+// (128 x 256 x 784: 10.2 us against 12.3).
 //
 // Warps: 0 TMA, 1 MMA (leader), 2..9 epilogue; RAW: 10..17 converters (two groups of four), 18 TMA
 // of X.
@@ -63,8 +67,7 @@ struct Params {
   __nv_bfloat16* out;
   int64_t ldo;
   const float* scale;  // [M]
-  float* partial;      // slots of [256][256] fp32
-  int32_t vec_ok;
+  float* partial;      // slots of [256 rows][256 columns] fp32
   Plan plan;
 };
 
@@ -270,8 +273,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Ring<RAW>::kThreads,
           const uint32_t b_addr = smem_u32(sB + sb * B_STAGE_BYTES);
 #pragma unroll
           for (int kk = 0; kk < BK / UMMA_K; ++kk)
-            umma_f16_ss_pair(d_tmem, make_sw128_desc(a_addr + kk * UMMA_K * 128, MN_CHUNK_BYTES, 1024),
-                             make_sw128_desc(b_addr + kk * UMMA_K * 128, MN_CHUNK_BYTES, 1024), IDESC,
+            umma_f16_ss_pair(d_tmem, make_sw128_desc(b_addr + kk * UMMA_K * 128, MN_CHUNK_BYTES, 1024),
+                             make_sw128_desc(a_addr + kk * UMMA_K * 128, MN_CHUNK_BYTES, 1024), IDESC,
                              (kb != it.kb0 || kk != 0) ? 1u : 0u);
           if constexpr (RAW) umma_commit_pair_mc(&b_empty[sb], kPairMask);
           umma_commit_pair_mc(&a_empty[sa], kPairMask);
@@ -290,49 +293,41 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Ring<RAW>::kThreads,
   } else if (warp < 2 + kEpiWarps) {
     // ------------------------------------------------------------ epilogue (warps 2..9)
     const uint32_t q = warp & 3u;
-    const int c_lo = static_cast<int>((warp - 2u) >> 2) * (TN / 64);
-    gemm::Params g{};
-    g.M = p.N;
-    g.N = p.K;
-    g.out = p.out;
-    g.ldo = p.ldo;
-    g.vec_ok = p.vec_ok;
+    const int c_lo = static_cast<int>((warp - 2u) >> 2) * (TM / 2);  // this warp's half of the rows of dW
+    // the column within the CTA's 128: RAW tiles hold the middle two of each four swapped (scale8)
+    const uint32_t l = RAW && ((lane + 1u) & 2u) ? lane ^ 3u : lane;
+    const int in_tile = static_cast<int>(rank) * HN + static_cast<int>(q * 32u + l);
     uint32_t acc = 0, acc_ph = 0;
     for (int i = cluster; i < items; i += num_clusters) {
       const Item it = item_at(p.plan, i, blocks);
-      const int in_tile = static_cast<int>(rank) * HM + static_cast<int>(q * 32 + lane);
-      const int row = (it.tile / k_tiles) * TM + in_tile;
-      const int k0 = (it.tile % k_tiles) * TN;
+      const int n0 = (it.tile / k_tiles) * TM + c_lo;
+      const int k = (it.tile % k_tiles) * TN + in_tile;
       if (!mbar_wait(&acc_full[acc], acc_ph, kFaultWaitAccFull)) break;
       tc_fence_after();
-      const uint32_t t_row = tmem_base + ((q * 32u) << 16) + acc * TN;
+      const uint32_t t_row = tmem_base + ((q * 32u) << 16) + acc * TM + static_cast<uint32_t>(c_lo);
 #pragma unroll 1
-      for (int c = c_lo; c < c_lo + TN / 64; ++c) {
-        const int col0 = k0 + c * 32;
-        if (col0 >= p.K) break;
+      for (int c = 0; c < TM / 2; c += 32) {
+        const int rows = min(32, p.N - n0 - c);
+        if (rows <= 0) break;
         uint32_t r[32];
-        tmem_ld_32x32b_x32(t_row + c * 32, r);
+        tmem_ld_32x32b_x32(t_row + c, r);
         tmem_wait_ld();
-#pragma unroll
-        for (int j = 0; RAW && j < 32; j += 4) {  // the converters' order of columns (scale8)
-          const uint32_t t = r[j + 1];
-          r[j + 1] = r[j + 2];
-          r[j + 2] = t;
-        }
+        if (k >= p.K) continue;
         if (it.slot < 0) {
-          gemm::epilogue_chunk<kEpiStoreBf16>(g, r, row, col0);
-        } else if (row < p.N) {
-          // slot[column][row]: a warp stores 128 contiguous bytes per column
-          float* part = p.partial + static_cast<size_t>(it.slot) * (TM * TN) + in_tile;
-          const int cols = min(32, p.K - col0);
+          __nv_bfloat16* out = p.out + static_cast<int64_t>(n0 + c) * p.ldo + k;
+#pragma unroll
+          for (int j = 0; j < 32; ++j, out += p.ldo)
+            if (j < rows) *out = __float2bfloat16_rn(__uint_as_float(r[j]));
+        } else {
+          float* part = p.partial + static_cast<size_t>(it.slot) * (TM * TN) + (c_lo + c) * TN + in_tile;
 #pragma unroll
           for (int j = 0; j < 32; ++j)
-            if (j < cols) __stcg(part + (c * 32 + j) * TM, __uint_as_float(r[j]));
+            if (j < rows) __stcg(part + j * TN, __uint_as_float(r[j]));
         }
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&acc_empty[acc]), 0u));
+      if (lane == 0) arrive_leader(&acc_empty[acc]);
       acc ^= 1u;
       if (acc == 0u) acc_ph ^= 1u;
     }
@@ -409,69 +404,78 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Ring<RAW>::kThreads,
 }
 
 // X in bf16: out[m][k] = bf16(q * scale), rows of `ldo` elements (a multiple of 8, columns past K
-// zero). A thread takes 16 columns of a row.
-__global__ void __launch_bounds__(256) widen_kernel(const int8_t* __restrict__ q, int64_t ldq, const float* __restrict__ scale,
-                                                    __nv_bfloat16* __restrict__ out, int64_t ldo, int M, int K) {
-  const int units = static_cast<int>((ldo + 15) / 16);
-  const int64_t total = static_cast<int64_t>(M) * units;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total;
-       i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-    const int64_t m = i / units;
-    const int k = static_cast<int>(i - m * units) * 16;
-    const int8_t* from = q + m * ldq + k;
-    uint32_t w[4] = {0u, 0u, 0u, 0u};
-    if (k + 16 <= K) {
-      const uint4 v = __ldcs(reinterpret_cast<const uint4*>(from));
-      w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
-    } else {
-#pragma unroll
-      for (int j = 0; j < 16; ++j)
-        if (k + j < K) w[j / 4] |= static_cast<uint32_t>(static_cast<uint8_t>(from[j])) << (8 * (j % 4));
-    }
+// zero). A warp takes rows, a lane eight columns at a time (so that a warp's stores are one run of
+// 512 bytes), eight loads ahead of their use.
+constexpr int kWidenWarps = 8;
+constexpr int kWidenAhead = 8;
+
+__global__ void __launch_bounds__(32 * kWidenWarps)
+    widen_kernel(const int8_t* __restrict__ q, int64_t ldq, const float* __restrict__ scale,
+                 __nv_bfloat16* __restrict__ out, int64_t ldo, int M, int K) {
+  const int units = static_cast<int>(ldo / 8), whole = K / 8;
+  const int lane = threadIdx.x & 31;
+  const int64_t warps = static_cast<int64_t>(gridDim.x) * kWidenWarps;
+  for (int64_t m = static_cast<int64_t>(blockIdx.x) * kWidenWarps + (threadIdx.x >> 5); m < M; m += warps) {
     const float s = __ldg(scale + m);
-    uint32_t o[8];
+    const int8_t* from = q + m * ldq;
+    uint4* to = reinterpret_cast<uint4*>(out + m * ldo);
+    for (int u0 = lane; u0 < units; u0 += 32 * kWidenAhead) {
+      uint2 w[kWidenAhead];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint32_t x = w[j / 2] >> (16 * (j % 2));
-      o[j] = pack_bf16x2(static_cast<float>(static_cast<int8_t>(x)) * s, static_cast<float>(static_cast<int8_t>(x >> 8)) * s);
+      for (int i = 0; i < kWidenAhead; ++i) {
+        const int u = u0 + 32 * i;
+        w[i] = make_uint2(0u, 0u);
+        if (u < whole) {
+          w[i] = __ldcs(reinterpret_cast<const uint2*>(from) + u);
+        } else if (u < units) {
+          uint32_t x[2] = {0u, 0u};
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (u * 8 + j < K) x[j / 4] |= static_cast<uint32_t>(static_cast<uint8_t>(from[u * 8 + j])) << (8 * (j % 4));
+          w[i] = make_uint2(x[0], x[1]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kWidenAhead; ++i) {
+        const int u = u0 + 32 * i;
+        if (u >= units) break;
+        uint32_t o[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t v = (j < 2 ? w[i].x : w[i].y) >> (16 * (j % 2));
+          o[j] = pack_bf16x2(static_cast<float>(static_cast<int8_t>(v)) * s,
+                             static_cast<float>(static_cast<int8_t>(v >> 8)) * s);
+        }
+        to[u] = make_uint4(o[0], o[1], o[2], o[3]);
+      }
     }
-    uint4* to = reinterpret_cast<uint4*>(out + m * ldo + k);
-    to[0] = make_uint4(o[0], o[1], o[2], o[3]);
-    if (k + 8 < ldo) to[1] = make_uint4(o[4], o[5], o[6], o[7]);
   }
 }
 
-// Adds the pieces of the cut tiles in order, rounds once. A block takes 32 rows x 32 columns of a
-// tile: partial sums are read along rows ([column][row]) and leave along columns.
-__global__ void __launch_bounds__(256) add_pieces_kernel(const Params p) {
-  __shared__ float t[32][33];
+// Adds the pieces of the cut tiles in order, rounds once. A block takes eight rows of a tile, a thread
+// one column of them.
+constexpr int kAddRows = 8;
+
+__global__ void __launch_bounds__(TN) add_pieces_kernel(const Params p) {
   const int tile = p.plan.whole + static_cast<int>(blockIdx.y);
   const int k_tiles = (p.K + TN - 1) / TN;
-  const int br = static_cast<int>(blockIdx.x) / (TN / 32) * 32, bc = static_cast<int>(blockIdx.x) % (TN / 32) * 32;
-  const int row0 = (tile / k_tiles) * TM + br, col0 = (tile % k_tiles) * TN + bc;
-  if (row0 >= p.N || col0 >= p.K) return;
-  const float* part = p.partial + static_cast<size_t>(blockIdx.y) * p.plan.pieces * (TM * TN);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  float sum[4] = {0.f, 0.f, 0.f, 0.f};
-  if (row0 + lane < p.N) {
-    const int cols = min(4, p.K - col0 - warp * 4);
-#pragma unroll 4
-    for (int s = 0; s < p.plan.pieces; ++s) {
-      const float* from = part + static_cast<size_t>(s) * (TM * TN) + (bc + warp * 4) * TM + br + lane;
+  const int r0 = static_cast<int>(blockIdx.x) * kAddRows;
+  const int n0 = (tile / k_tiles) * TM + r0, k = (tile % k_tiles) * TN + static_cast<int>(threadIdx.x);
+  if (n0 >= p.N || k >= p.K) return;
+  const float* part = p.partial + static_cast<size_t>(blockIdx.y) * p.plan.pieces * (TM * TN) + r0 * TN + threadIdx.x;
+  float sum[kAddRows];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (i < cols) sum[i] += __ldcg(from + i * TM);
-    }
+  for (int i = 0; i < kAddRows; ++i) sum[i] = 0.f;
+#pragma unroll 2
+  for (int s = 0; s < p.plan.pieces; ++s) {
+#pragma unroll
+    for (int i = 0; i < kAddRows; ++i)
+      if (n0 + i < p.N) sum[i] += __ldcg(part + static_cast<size_t>(s) * (TM * TN) + i * TN);
   }
+  __nv_bfloat16* out = p.out + static_cast<int64_t>(n0) * p.ldo + k;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) t[warp * 4 + i][lane] = sum[i];
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = warp * 4 + i;
-    if (row0 + r < p.N && col0 + lane < p.K)
-      p.out[static_cast<int64_t>(row0 + r) * p.ldo + col0 + lane] = __float2bfloat16_rn(t[lane][r]);
-  }
+  for (int i = 0; i < kAddRows; ++i)
+    if (n0 + i < p.N) out[i * p.ldo] = __float2bfloat16_rn(sum[i]);
 }
 
 }  // namespace ckpt

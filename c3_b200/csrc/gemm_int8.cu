@@ -170,8 +170,8 @@ int dw_clusters(int* clusters) {
 int dw_run(int64_t M, int64_t N, int64_t K, DwRun* r) {
   const int64_t tiles = ((N + ckpt::TM - 1) / ckpt::TM) * ((K + ckpt::TN - 1) / ckpt::TN);
   const int blocks = static_cast<int>((M + ckpt::BK - 1) / ckpt::BK);
-  // Widening X in the kernel slows each K block from 0.4 to 0.6 us; widening it first costs a launch
-  // and three bytes per element of X at 6 TB/s. XXX
+  // Widening X in the kernel slows each K block by about 0.2 us (0.6 instead of 0.4); widening it first
+  // costs a launch, about 2.5 us, and three bytes per element of X at 6 TB/s.
   dw_clusters<true>(&r->clusters);
   r->plan = ckpt::make_plan(static_cast<int>(tiles), r->clusters, blocks);
   const double rounds = static_cast<double>(r->plan.whole / r->clusters) * blocks +
@@ -194,7 +194,7 @@ int launch_dw(const CUtensorMap& ta, const CUtensorMap& tx, const ckpt::Params& 
                                      ckpt::Ring<RAW>::kSmem, st, ta, tx, p),
                        "gemm_dw_int8: launch");
   if (rc != C3CU_OK || p.plan.rest == 0) return rc;
-  ckpt::add_pieces_kernel<<<dim3(64, p.plan.rest), 256, 0, st>>>(p);
+  ckpt::add_pieces_kernel<<<dim3(ckpt::TM / ckpt::kAddRows, p.plan.rest), ckpt::TN, 0, st>>>(p);
   return cuda_status(cudaGetLastError(), "gemm_dw_int8: launch");
 }
 
@@ -297,7 +297,6 @@ extern "C" int c3cu_gemm_dw_int8(const void* dZ, int64_t lddz, const int8_t* X, 
   p.ldo = lddw;
   p.scale = x_scale;
   p.partial = static_cast<float*>(workspace);
-  p.vec_ok = aligned16(dW) && (N == 1 || lddw % 8 == 0);
   if (((N + 255) / 256) * ((K + 255) / 256) > (1 << 24)) {
     set_error("gemm_dw_int8: dW is too large (N %lld, K %lld)", (long long)N, (long long)K);
     return C3CU_ERR_INVALID;
@@ -316,9 +315,8 @@ extern "C" int c3cu_gemm_dw_int8(const void* dZ, int64_t lddz, const int8_t* X, 
   if ((rc = encode_int8_2d(&tx, X, M, K, ldx, ckpt::HN, ckpt::BK, false)) != C3CU_OK) return rc;
   if (r.raw) return launch_dw<true>(ta, tx, p, r.clusters, st);
   __nv_bfloat16* wide = reinterpret_cast<__nv_bfloat16*>(static_cast<uint8_t*>(workspace) + r.partial_bytes);
-  const int64_t units = M * ((r.wide_ld + 15) / 16);
-  const int64_t want = (units + 255) / 256, most = static_cast<int64_t>(sm_count()) * 8;
-  ckpt::widen_kernel<<<static_cast<unsigned>(want < most ? want : most), 256, 0, st>>>(
+  const int64_t want = (M + ckpt::kWidenWarps - 1) / ckpt::kWidenWarps, most = static_cast<int64_t>(sm_count()) * 8;
+  ckpt::widen_kernel<<<static_cast<unsigned>(want < most ? want : most), 32 * ckpt::kWidenWarps, 0, st>>>(
       X, ldx, x_scale, wide, r.wide_ld, static_cast<int>(M), static_cast<int>(K));
   if ((rc = cuda_status(cudaGetLastError(), "gemm_dw_int8: launch")) != C3CU_OK) return rc;
   if ((rc = encode_bf16_2d_sw128(&tx, wide, M, K, r.wide_ld, 64, ckpt::BK)) != C3CU_OK) return rc;

@@ -11,7 +11,7 @@ import math
 import torch
 
 from . import _lib
-from .linear import _call, _current_device, _ptr, _rows_of, _vector_of
+from .linear import _call, _current_device, _fast_result, _on_gpu, _ptr, _rows_of, _vector_of
 from .quant import _dtype_code, empty_rows, row_stride
 
 
@@ -24,6 +24,10 @@ def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, resi
     the new residual stream; it may be written over either (h=residual or h=x). Without one, h is x.
     h and rstd are what `rms_norm_backward` needs. Rows may be slices of wider ones (unit column
     stride). A row of h with an infinity or a NaN gets q = 0 and scale NaN."""
+    if q is None and scale is None and h is None and rstd is None and _on_gpu(x):
+        r = _lib.fast().rms_norm_int8(x, weight, eps, residual)
+        if r is not None:
+            return _fast_result(r, "c3cu_rms_norm_int8")
     code = _dtype_code(x, "x")
     M, K = x.shape
     if K < 1:
@@ -92,6 +96,10 @@ def rms_norm_backward(dy: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, r
     stream's), added to dx. dx is the gradient of x and of the residual alike. dy, h, dh and dx have
     one type (bf16 or fp32); dx may be written over any of them. dweight has the same bits in every
     run."""
+    if dx is None and dweight is None and _on_gpu(h):
+        r = _lib.fast().rms_norm_backward(dy, h, weight, rstd, dh)
+        if r is not None:
+            return _fast_result(r, "c3cu_rms_norm_bwd")
     code = _dtype_code(h, "h")
     M, K = h.shape
     if K < 1:

@@ -9,7 +9,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .linear import _call, _rows_of, _vector_of
+from .linear import _call, _fast_result, _on_gpu, _rows_of, _vector_of
 
 _DTYPES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16}
 
@@ -40,6 +40,10 @@ def quantize_rows(x: torch.Tensor, q: torch.Tensor | None = None, scale: torch.T
 
     q is the integer nearest to 127 x / A (ties to even) with A the row's largest |x|, scale = A / 127.
     A row of zeros gets scale 0; a row with an infinity or a NaN gets q = 0 and scale NaN."""
+    if q is None and scale is None and _on_gpu(x):
+        r = _lib.fast().quantize_rows(x)
+        if r is not None:
+            return _fast_result(r, "c3cu_quantize_rows")
     code = _dtype_code(x, "x")
     M, K = x.shape
     if K < 1:
