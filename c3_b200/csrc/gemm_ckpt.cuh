@@ -302,7 +302,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Ring<RAW>::kThreads,
       const Item it = item_at(p.plan, i, blocks);
       const int n0 = (it.tile / k_tiles) * TM + c_lo;
       const int k = (it.tile % k_tiles) * TN + in_tile;
-      if (!mbar_wait(&acc_full[acc], acc_ph, kFaultWaitAccFull)) break;
+      if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[acc], acc_ph, kFaultWaitAccFull))) break;
       tc_fence_after();
       const uint32_t t_row = tmem_base + ((q * 32u) << 16) + acc * TM + static_cast<uint32_t>(c_lo);
 #pragma unroll 1
@@ -310,6 +310,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Ring<RAW>::kThreads,
         const int rows = min(32, p.N - n0 - c);
         if (rows <= 0) break;
         uint32_t r[32];
+        __syncwarp();  // lanes past the last column skip the stores
         tmem_ld_32x32b_x32(t_row + c, r);
         tmem_wait_ld();
         if (k >= p.K) continue;
@@ -362,7 +363,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Ring<RAW>::kThreads,
         next[j] = m < p.M ? __ldg(p.scale + m) : 0.f;
       }
       for (int kb = first; kb < it.kb1; kb += kConvGroups) {
-        if (!mbar_wait(&raw_full[sr], pr, kFaultWaitFull)) { ok = false; break; }
+        ok = __all_sync(0xffffffffu, mbar_wait(&raw_full[sr], pr, kFaultWaitFull));
+        if (!ok) break;
         uint4 w[4], o[8];
 #pragma unroll
         for (int j = 0; j < 4; ++j) w[j] = ld_shared_v4(from + sr * RAW_BYTES + j * (4 * HN));
@@ -377,7 +379,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Ring<RAW>::kThreads,
           o[2 * j + 1] = scale8(swap ? w[j].x : w[j].z, swap ? w[j].y : w[j].w, sc);
         }
         // only now: the conversion runs while the MMAs still read the stage's last tile
-        if (!mbar_wait(&b_empty[sb], pb ^ 1u, kFaultWaitEmpty)) { ok = false; break; }
+        ok = __all_sync(0xffffffffu, mbar_wait(&b_empty[sb], pb ^ 1u, kFaultWaitEmpty));
+        if (!ok) break;
         const uint32_t line = to + sb * B_STAGE_BYTES;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {

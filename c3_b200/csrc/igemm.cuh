@@ -283,7 +283,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::kThreads, 1)
         const int m = m0 + c * 32 + static_cast<int>(lane);
         xs[c] = m < p.M ? __ldg(p.xs + m) : 0.f;
       }
-      if (!mbar_wait(&acc_full[acc], acc_ph, kFaultWaitAccFull)) break;
+      if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[acc], acc_ph, kFaultWaitAccFull))) break;
       tc_fence_after();
       const uint32_t t_row = tmem_base + ((q * 32u) << 16) + acc * TN + static_cast<uint32_t>(c_lo);
       // two chunks' accumulators in registers, so that one is on its way while the other is worked on
@@ -291,6 +291,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::kThreads, 1)
       tmem_ld_32x32b_x32(t_row, r[0]);
 #pragma unroll
       for (int c = 0; c < kWarpTokens / 32; ++c) {
+        __syncwarp();  // lanes past the last channel skip the stores
         tmem_wait_ld();
         if (c + 1 < kWarpTokens / 32) {
           tmem_ld_32x32b_x32(t_row + (c + 1) * 32, r[(c + 1) & 1]);
@@ -304,6 +305,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::kThreads, 1)
           store_tokens<32, F32, RELU>(
               p, r[c & 1], [&](int j) { return __shfl_sync(0xffffffffu, xs[c], j); }, m, p.M - m, n, ws, b, lane);
       }
+      __syncwarp();
       acc ^= 1u;
       if (acc == 0u) acc_ph ^= 1u;
     }
@@ -447,7 +449,7 @@ __global__ void __launch_bounds__(narrow::kThreads)
       ws = __ldg(p.ws + n);
       if (p.bias) b = __ldg(p.bias + n);
     }
-    ok = mbar_wait(acc_full, 0u, kFaultWaitAccFull);
+    ok = __all_sync(0xffffffffu, mbar_wait(acc_full, 0u, kFaultWaitAccFull));
     tc_fence_after();
   }
   const int tokens = min(T, p.M - m0);
@@ -456,6 +458,7 @@ __global__ void __launch_bounds__(narrow::kThreads)
 #pragma unroll 1
       for (int c = 16 * half; c < tokens; c += 32) {
         uint32_t r[16];
+        __syncwarp();
         tmem_ld_32x32b_x16(t_row + c, r);
         tmem_wait_ld();
         store_tokens<16, F32, RELU>(p, r, [&](int j) { return s_xs[c + j]; }, m0 + c, tokens - c, n, ws, b, lane);
@@ -497,6 +500,7 @@ __global__ void __launch_bounds__(narrow::kThreads)
         store_tokens<J, F32, RELU>(p, sum, [&](int j) { return s_xs[t + j]; }, m0 + t, last - t, n, ws, b, lane);
       }
     }
+    __syncwarp();
     cluster_sync_all();  // no CTA leaves while another reads its sums
   }
 
