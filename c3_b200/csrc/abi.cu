@@ -110,8 +110,7 @@ PFN_cuTensorMapEncodeTiled_v12000 get_encode_fn() {
 }  // namespace
 
 namespace {
-int encode_2d(CUtensorMap* map, CUtensorMapDataType type, const char* name, uint32_t esize, const void* base,
-              uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_cols, uint32_t box_rows, bool swizzle) {
+int check_tma_rows(const char* name, uint32_t esize, const void* base, uint64_t cols, uint64_t ld) {
   if (!aligned16(base)) {
     set_error("TMA operand base %p is not 16-byte aligned", base);
     return C3CU_ERR_ALIGN;
@@ -122,6 +121,13 @@ int encode_2d(CUtensorMap* map, CUtensorMapDataType type, const char* name, uint
               (unsigned long long)ld, name, (unsigned long long)cols);
     return C3CU_ERR_ALIGN;
   }
+  return C3CU_OK;
+}
+
+int encode_2d(CUtensorMap* map, CUtensorMapDataType type, const char* name, uint32_t esize, const void* base,
+              uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_cols, uint32_t box_rows, bool swizzle) {
+  const int rc = check_tma_rows(name, esize, base, cols, ld);
+  if (rc != C3CU_OK) return rc;
   auto fn = get_encode_fn();
   if (!fn) {
     set_error("cuTensorMapEncodeTiled is unavailable from the CUDA driver");
@@ -148,6 +154,8 @@ int encode_bf16_2d_sw128(CUtensorMap* map, const void* base, uint64_t rows, uint
                          uint64_t ld, uint32_t box_cols, uint32_t box_rows) {
   return encode_2d(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, "bf16", 2u, base, rows, cols, ld, box_cols, box_rows, true);
 }
+
+int check_int8_rows(const void* base, uint64_t cols, uint64_t ld) { return check_tma_rows("int8", 1u, base, cols, ld); }
 
 int encode_int8_2d(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_cols,
                    uint32_t box_rows, bool swizzle) {

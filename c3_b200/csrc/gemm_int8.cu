@@ -1,10 +1,11 @@
 // C-ABI entry points of the int8 GEMMs (include/c3cu.h): the Linear forward on int8 rows with
-// scales (igemm.cuh) and the weight gradient from an 8-bit checkpoint (gemm_ckpt.cuh).
+// scales (igemm.cuh, igemv.cuh) and the weight gradient from an 8-bit checkpoint (gemm_ckpt.cuh).
 #include <atomic>
 
 #include "gemm_ckpt.cuh"
 #include "host_util.h"
 #include "igemm.cuh"
+#include "igemv.cuh"
 
 C3CU_FAULT_ACCESSORS(int8)
 
@@ -54,7 +55,7 @@ struct ForwardPlan {
 //   narrow  3.3 + waves (kb c(T) + e(T)), e being the epilogue, or for a split tile the exchange of
 //           partial sums 0.6 + 0.034 T
 //   pair    5 + waves (3.2 + 0.265 kb)
-// Measured (us), 4096 channels x K 4096: 1 token 5.8 (T 16, split 4) against 13.4 (pair), 64 tokens
+// Measured (us), 4096 channels x K 4096: 8 tokens 5.8 (T 16, split 4) against 13.4 (pair), 64 tokens
 // 7.8 (T 64, split 4) / 13.6, 512 tokens 12.5 (T 128) / 16.8, 1024 tokens 19.0 (T 256) / 17.9; 12288
 // channels x K 1024, 2048 tokens 54 (T 256) / 34.
 ForwardPlan plan_forward(int64_t M, int64_t N, int64_t K) {
@@ -124,8 +125,48 @@ int launch_igemm_narrow(const Operands& o, igemm::Params p, const ForwardPlan& p
   return cuda_status(cudaLaunchKernelEx(&cfg, kern, tw, tx, p), "linear_int8: launch");
 }
 
+// Warps per block of igemv_kernel. Few blocks: a warp for each 512 bytes of a row, so that all of W is
+// asked for at once; many: one for each 1024, so that a warp has 16 loads in flight. Measured with one
+// token (us): 512 channels x K 2048 2.3 with 4 warps, 3.2 with 1; 16 x 16384 3.2 with 16, 4.5 with 4;
+// 12288 x 1024 4.8 with 1, 5.8 with 2; 12288 x 12288 25.9 with 4, 28.1 with 8.
+int igemv_split(int64_t blocks, int64_t K) {
+  const int sms = sm_count();
+  const int most = blocks <= sms ? igemv::kMaxSplit : blocks <= 2 * sms ? 8 : 4;
+  const int64_t each = igemv::kStep * (blocks <= 2 * sms ? 1 : igemv::kAhead);
+  int split = 1;
+  while (split < most && split * each < K) split *= 2;
+  return split;
+}
+
+// Up to two tokens always, up to four while their multiplications do not outweigh a tile on the tensor
+// cores. Measured (us, igemv / narrow): one token, 4096 x 4096 5.2 / 7.3, 1397 x 777 2.4 / 4.7, 12288 x
+// 12288 26 / 34.5; two, 12288 x 4096 12.8 / 11.9; four, 4096 x 4096 7.1 / 7.7, 12288 x 4096 16 / 11.9.
+bool use_igemv(int64_t M, int64_t N, int64_t K) {
+  if (gemm_max_ctas() > 0) return false;  // the persistent kernel keeps to the caller's CTAs
+  return M <= 2 || (M <= igemv::kMaxTokens && N * K <= 20'000'000);
+}
+
+template <int T, bool F32, bool RELU>
+int launch_igemv(const Operands& o, const igemm::Params& p, cudaStream_t st) {
+  int rc = check_int8_rows(o.w, p.K, o.ldw);
+  if (rc == C3CU_OK) rc = check_int8_rows(o.x, p.K, o.ldx);
+  if (rc != C3CU_OK) return rc;
+  // a block writes a byte of the mask: those past N complete the rows' last words
+  const int64_t channels = RELU && p.mask ? (static_cast<int64_t>(p.N) + 31) / 32 * 32 : p.N;
+  const int64_t blocks = (channels + igemv::kChannels - 1) / igemv::kChannels;
+  const int split = igemv_split(blocks, p.K);
+  return cuda_status(launch_kernel(igemv::igemv_kernel<T, F32, RELU>, dim3(static_cast<unsigned>(blocks)),
+                                   dim3(32 * split), 0, st, o.x, o.ldx, o.w, o.ldw, p),
+                     "linear_int8: launch");
+}
+
 template <bool F32, bool RELU>
 int dispatch_igemm(const Operands& o, const igemm::Params& p, cudaStream_t st) {
+  if (use_igemv(p.M, p.N, p.K)) {
+    if (p.M == 1) return launch_igemv<1, F32, RELU>(o, p, st);
+    if (p.M == 2) return launch_igemv<2, F32, RELU>(o, p, st);
+    return launch_igemv<4, F32, RELU>(o, p, st);
+  }
   const ForwardPlan plan = plan_forward(p.M, p.N, p.K);
   switch (plan.T) {
     case 16: return launch_igemm_narrow<16, F32, RELU>(o, p, plan, st);

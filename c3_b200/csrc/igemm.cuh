@@ -8,9 +8,9 @@
 // kernel or tile that computed them. X and W are row-major [rows][K] (K-major operands): a
 // 128-deep K block of a row is one 128-byte swizzled line.
 //
-// Two kernels:
-// In both the channels are the MMA's rows and the tokens its columns, so that few tokens leave no
-// tensor-core rows empty and a warp's stores run along a row of Y.
+// Two kernels (igemv.cuh has a third, for a token or a few). In both the channels are the MMA's rows and
+// the tokens its columns, so that few tokens leave no tensor-core rows empty and a warp's stores run
+// along a row of Y.
 //   igemm_pair_kernel    tiles of 256 channels x 256 tokens on CTA pairs (cta_group::2), persistent:
 //                        the structure of gemm2_kernel with int8 K blocks. For many tiles.
 //   igemm_narrow_kernel  128 channels x T tokens per CTA. The K blocks of a tile are
