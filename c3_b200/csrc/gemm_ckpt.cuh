@@ -415,6 +415,8 @@ constexpr int kWidenAhead = 8;
 __global__ void __launch_bounds__(32 * kWidenWarps)
     widen_kernel(const int8_t* __restrict__ q, int64_t ldq, const float* __restrict__ scale,
                  __nv_bfloat16* __restrict__ out, int64_t ldo, int M, int K) {
+  pdl_wait();
+  pdl_launch_dependents();
   const int units = static_cast<int>(ldo / 8), whole = K / 8;
   const int lane = threadIdx.x & 31;
   const int64_t warps = static_cast<int64_t>(gridDim.x) * kWidenWarps;
@@ -460,6 +462,7 @@ __global__ void __launch_bounds__(32 * kWidenWarps)
 constexpr int kAddRows = 8;
 
 __global__ void __launch_bounds__(TN) add_pieces_kernel(const Params p) {
+  pdl_wait();
   const int tile = p.plan.whole + static_cast<int>(blockIdx.y);
   const int k_tiles = (p.K + TN - 1) / TN;
   const int r0 = static_cast<int>(blockIdx.x) * kAddRows;

@@ -231,12 +231,14 @@ template <bool RAW>
 int launch_dw(const CUtensorMap& ta, const CUtensorMap& tx, const ckpt::Params& p, int clusters, cudaStream_t st) {
   const int items = ckpt::item_count(p.plan);
   if (items < clusters) clusters = items;
-  int rc = cuda_status(launch_kernel(ckpt::dw_kernel<RAW>, dim3(2 * clusters), dim3(ckpt::Ring<RAW>::kThreads),
-                                     ckpt::Ring<RAW>::kSmem, st, ta, tx, p),
+  // not RAW: the kernel that widens X is before it
+  int rc = cuda_status(launch_serialized(!RAW || pdl_enabled(), ckpt::dw_kernel<RAW>, dim3(2 * clusters),
+                                         dim3(ckpt::Ring<RAW>::kThreads), ckpt::Ring<RAW>::kSmem, st, ta, tx, p),
                        "gemm_dw_int8: launch");
   if (rc != C3CU_OK || p.plan.rest == 0) return rc;
-  ckpt::add_pieces_kernel<<<dim3(ckpt::TM / ckpt::kAddRows, p.plan.rest), ckpt::TN, 0, st>>>(p);
-  return cuda_status(cudaGetLastError(), "gemm_dw_int8: launch");
+  return cuda_status(launch_next(ckpt::add_pieces_kernel, dim3(ckpt::TM / ckpt::kAddRows, p.plan.rest), dim3(ckpt::TN),
+                                 0, st, p),
+                     "gemm_dw_int8: launch");
 }
 
 }  // namespace
@@ -357,9 +359,11 @@ extern "C" int c3cu_gemm_dw_int8(const void* dZ, int64_t lddz, const int8_t* X, 
   if (r.raw) return launch_dw<true>(ta, tx, p, r.clusters, st);
   __nv_bfloat16* wide = reinterpret_cast<__nv_bfloat16*>(static_cast<uint8_t*>(workspace) + r.partial_bytes);
   const int64_t want = (M + ckpt::kWidenWarps - 1) / ckpt::kWidenWarps, most = static_cast<int64_t>(sm_count()) * 8;
-  ckpt::widen_kernel<<<static_cast<unsigned>(want < most ? want : most), 32 * ckpt::kWidenWarps, 0, st>>>(
-      X, ldx, x_scale, wide, r.wide_ld, static_cast<int>(M), static_cast<int>(K));
-  if ((rc = cuda_status(cudaGetLastError(), "gemm_dw_int8: launch")) != C3CU_OK) return rc;
+  rc = cuda_status(launch_kernel(ckpt::widen_kernel, dim3(static_cast<unsigned>(want < most ? want : most)),
+                                 dim3(32 * ckpt::kWidenWarps), 0, st, X, ldx, x_scale, wide, r.wide_ld,
+                                 static_cast<int>(M), static_cast<int>(K)),
+                   "gemm_dw_int8: launch");
+  if (rc != C3CU_OK) return rc;
   if ((rc = encode_bf16_2d_sw128(&tx, wide, M, K, r.wide_ld, 64, ckpt::BK)) != C3CU_OK) return rc;
   return launch_dw<false>(ta, tx, p, r.clusters, st);
 }

@@ -57,10 +57,10 @@ void gemm_invalidate_split_workspaces();
 // (c3cu_set_launch_overlap; off by default).
 bool pdl_enabled();
 
-// Launches `kern` on `stream`, with programmatic stream serialization when pdl_enabled().
+// Launches `kern` on `stream`, with programmatic stream serialization where `early` says so.
 template <typename... KArgs, typename... Args>
-cudaError_t launch_kernel(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
-                          Args&&... args) {
+cudaError_t launch_serialized(bool early, void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem,
+                              cudaStream_t stream, Args&&... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = block;
@@ -70,8 +70,25 @@ cudaError_t launch_kernel(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t 
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = pdl_enabled() ? 1 : 0;
+  cfg.numAttrs = early ? 1 : 0;
   return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
+}
+
+// ... when pdl_enabled().
+template <typename... KArgs, typename... Args>
+cudaError_t launch_kernel(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
+                          Args&&... args) {
+  return launch_serialized(pdl_enabled(), kern, grid, block, smem, stream, std::forward<Args>(args)...);
+}
+
+// Launches the second or third kernel of one call, which is scheduled while the one before it drains
+// and waits for it (pdl_wait, in every thread, before anything else), about 1 us sooner than a
+// launch of its own. The kernel before calls pdl_launch_dependents, and nothing outside the call is
+// overlapped: this one ends after that one.
+template <typename... KArgs, typename... Args>
+cudaError_t launch_next(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
+                        Args&&... args) {
+  return launch_serialized(true, kern, grid, block, smem, stream, std::forward<Args>(args)...);
 }
 
 // The calling thread's cap on persistent GEMM CTAs (c3cu_set_gemm_max_ctas; 0 = none).

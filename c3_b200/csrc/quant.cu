@@ -691,6 +691,7 @@ __global__ void __launch_bounds__(512) norm_bwd_kernel(const BwdArgs p) {
   const uint32_t bytes = static_cast<uint32_t>(p.K) * sizeof(T);
   const uint32_t pitch = row_pitch(bytes, SG == 0);
   const uint32_t stage = (p.dh ? 3u : 2u) * pitch;
+  pdl_launch_dependents();
   auto fill = [&](int s, int64_t row) {
     uint8_t* to = rows + s * stage;
     if constexpr (SG == 0) {
@@ -821,6 +822,7 @@ template <typename T, int SG>
 __global__ void __launch_bounds__(512) norm_bwd_dot_kernel(const BwdArgs p, float* __restrict__ dots) {
   constexpr int V = Runs<T, SG>::V;
   __shared__ RowSums sums;
+  pdl_launch_dependents();
   const int64_t row = blockIdx.x;
   const int t = threadIdx.x, G = blockDim.x;
   const T* dy = static_cast<const T*>(p.dy) + row * p.ldy;
@@ -848,6 +850,8 @@ template <typename T, int SG>
 __global__ void __launch_bounds__(kStripThreads) norm_bwd_strip_kernel(const BwdArgs p, const float* __restrict__ dots,
                                                                        int rows_per_block) {
   constexpr int V = Runs<T, SG>::V;
+  pdl_wait();
+  pdl_launch_dependents();
   const int t = threadIdx.x, G = blockDim.x;
   const int c0 = static_cast<int>(blockIdx.x) * (kStripThreads * V);  // the strip's first column
   const int K = p.K - c0;
@@ -880,6 +884,7 @@ __global__ void __launch_bounds__(kStripThreads) norm_bwd_strip_kernel(const Bwd
 // dweight = sum of the blocks' shares, in a fixed order.
 __global__ void __launch_bounds__(1024) sum_partials_kernel(const float* __restrict__ partial, float* __restrict__ out,
                                                             int rows, int K) {
+  pdl_wait();
   const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + (threadIdx.x & 31);
   const int warp = threadIdx.x >> 5;
   float acc = 0.f;
@@ -1079,9 +1084,10 @@ template <typename T, int SG>
 cudaError_t launch_bwd_strips(BwdArgs p, float* dots, int rows, cudaStream_t st) {
   constexpr int kCols = kStripThreads * Runs<T, SG>::V;
   norm_bwd_dot_kernel<T, SG ? 512 : 0><<<p.M, 512, 0, st>>>(p, dots);
-  norm_bwd_strip_kernel<T, SG><<<dim3((p.K + kCols - 1) / kCols, rows), kStripThreads, 0, st>>>(p, dots,
-                                                                                            strip_rows(p.M, p.K, kCols));
-  return cudaGetLastError();
+  const cudaError_t err = cudaGetLastError();
+  if (err != cudaSuccess) return err;
+  return launch_next(norm_bwd_strip_kernel<T, SG>, dim3((p.K + kCols - 1) / kCols, rows), dim3(kStripThreads), 0, st, p,
+                     static_cast<const float*>(dots), strip_rows(p.M, p.K, kCols));
 }
 
 template <typename T>
@@ -1098,8 +1104,9 @@ int bwd(BwdArgs p, bool vec, float* ws, cudaStream_t st) {
   }
   int rc = cuda_status(err, "rms_norm_bwd: launch");
   if (rc != C3CU_OK || rows <= 1) return rc;
-  sum_partials_kernel<<<(p.K + 31) / 32, 1024, 0, st>>>(p.partial, p.dweight, rows, p.K);
-  return cuda_status(cudaGetLastError(), "rms_norm_bwd: launch");
+  err = launch_next(sum_partials_kernel, dim3((p.K + 31) / 32), dim3(1024), 0, st, static_cast<const float*>(p.partial),
+                    p.dweight, rows, p.K);
+  return cuda_status(err, "rms_norm_bwd: launch");
 }
 
 int check_sizes(const char* what, int64_t M, int64_t K, int dtype) {
