@@ -18,7 +18,7 @@
 // Beside the tensor cores the widening runs into the power limit and the shared-memory traffic of
 // the tiles (16384 x 4096 x 4096: 505 to 548 us RAW, 424 !RAW, of which widen_kernel 33; the bf16
 // gradient from a bf16 X takes 350 to 370 in the same loop). With few K blocks RAW saves the launch
-// (128 x 256 x 784: 10.2 us against 12.3).
+// (in these tiles 128 x 256 x 784 took 10.2 us RAW, 12.3 else; gemm_ckpt_narrow.cuh takes 6.2).
 //
 // Warps: 0 TMA, 1 MMA (leader), 2..9 epilogue; RAW: 10..17 converters (two groups of four), 18 TMA
 // of X.
@@ -116,6 +116,43 @@ __device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {
 __device__ __forceinline__ void st_shared_v4(uint32_t addr, const uint4& v) {
   asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
+
+// One warp's part in widening a K block: 16 of the block's 64 rows, four at a time. Lane = 8 * row + u
+// reads the 16 int8 of unit u of its row and writes two 16-byte pieces of the swizzled bf16 tile:
+// chunk u / 4 (64 columns), pieces 2u and 2u + 1 of 8, at position piece ^ (row mod 8). Units 4..7
+// write their odd piece first, so that the eight lanes of a row touch all banks once.
+struct Widener {
+  int r0;             // the lane's rows are r0, r0 + 4, ...
+  uint32_t from, to;  // of the lane's first unit and piece's line in the raw block and the tile
+  uint32_t at;        // rows r0, r0 + 4, ...: the row modulo 8 alternates between lane / 8 and that plus 4
+  bool swap;
+
+  __device__ __forceinline__ Widener(int warp, int lane) {
+    const int u = lane & 7;
+    r0 = warp * 16 + (lane >> 3);
+    swap = u >= 4;
+    from = static_cast<uint32_t>(r0 * HN + u * 16);
+    const uint32_t piece = static_cast<uint32_t>(((2 * u) & 7) | (swap ? 1 : 0));
+    to = static_cast<uint32_t>((u >> 2) * MN_CHUNK_BYTES + r0 * 128);
+    at = (piece ^ static_cast<uint32_t>(lane >> 3)) << 4;
+  }
+  __device__ __forceinline__ void load(uint32_t raw, uint4 (&w)[4]) const {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = ld_shared_v4(raw + from + j * (4 * HN));
+  }
+  __device__ __forceinline__ void convert(const uint4& w, float scale, uint4* o) const {
+    const Scale2 sc = split_scale(scale);
+    o[0] = scale8(swap ? w.z : w.x, swap ? w.w : w.y, sc);
+    o[1] = scale8(swap ? w.x : w.z, swap ? w.y : w.w, sc);
+  }
+  __device__ __forceinline__ void store(uint32_t tile, const uint4 (&o)[8]) const {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      st_shared_v4(tile + to + (at ^ ((j & 1) ? 64u : 0u)) + j * 512, o[2 * j]);
+      st_shared_v4(tile + to + (at ^ 16u ^ ((j & 1) ? 64u : 0u)) + j * 512, o[2 * j + 1]);
+    }
+  }
+};
 
 // Counts an arrival on a barrier of the leader CTA. The writes it publishes were made visible to
 // the async proxy, which alone reads them, by the writers' proxy fences; a release at cluster
@@ -334,21 +371,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Ring<RAW>::kThreads,
     }
   } else if constexpr (RAW) {
     // ------------------------------------------------------------ converters (warps 10..17)
-    // The two groups of four warps take K blocks in turn. A warp takes 16 of the block's 64 rows,
-    // four at a time: lane = 8 * row + u reads the 16 int8 of unit u of its row and writes two
-    // 16-byte pieces of the swizzled bf16 tile: chunk u / 4 (64 columns), pieces 2u and 2u + 1 of
-    // 8, at position piece ^ (row mod 8). Units 4..7 write their odd piece first, so that the
-    // eight lanes of a row touch all banks once.
     const int cw = static_cast<int>(warp) - 2 - kEpiWarps;
     const int group = cw / kConvWarps;
-    const int u = static_cast<int>(lane & 7u);
-    const int r0 = (cw % kConvWarps) * 16 + static_cast<int>(lane >> 3);
-    const bool swap = u >= 4;
-    const uint32_t from = smem_u32(sRaw) + static_cast<uint32_t>(r0 * HN + u * 16);
-    const uint32_t piece = static_cast<uint32_t>(((2 * u) & 7) | (swap ? 1 : 0));
-    const uint32_t to = smem_u32(sB) + static_cast<uint32_t>((u >> 2) * MN_CHUNK_BYTES + r0 * 128);
-    // rows r0, r0 + 4, ...: the row modulo 8 alternates between lane / 8 and that plus 4
-    const uint32_t at = ((piece ^ (lane >> 3)) << 4);
+    const Widener widen(cw % kConvWarps, static_cast<int>(lane));
     int turn = 0;  // K blocks of earlier items, modulo the groups
     uint32_t sr = group, sb = group, pr = 0, pb = 0;
     bool ok = true;
@@ -359,34 +384,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Ring<RAW>::kThreads,
       float next[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int m = first * BK + r0 + 4 * j;
+        const int m = first * BK + widen.r0 + 4 * j;
         next[j] = m < p.M ? __ldg(p.scale + m) : 0.f;
       }
       for (int kb = first; kb < it.kb1; kb += kConvGroups) {
         ok = __all_sync(0xffffffffu, mbar_wait(&raw_full[sr], pr, kFaultWaitFull));
         if (!ok) break;
         uint4 w[4], o[8];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) w[j] = ld_shared_v4(from + sr * RAW_BYTES + j * (4 * HN));
+        widen.load(smem_u32(sRaw) + sr * RAW_BYTES, w);
         __syncwarp();
         if (lane == 0) mbar_arrive(&raw_empty[sr]);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const Scale2 sc = split_scale(next[j]);
-          const int m = (kb + kConvGroups) * BK + r0 + 4 * j;
+          widen.convert(w[j], next[j], &o[2 * j]);
+          const int m = (kb + kConvGroups) * BK + widen.r0 + 4 * j;
           next[j] = m < p.M ? __ldg(p.scale + m) : 0.f;
-          o[2 * j] = scale8(swap ? w[j].z : w[j].x, swap ? w[j].w : w[j].y, sc);
-          o[2 * j + 1] = scale8(swap ? w[j].x : w[j].z, swap ? w[j].y : w[j].w, sc);
         }
         // only now: the conversion runs while the MMAs still read the stage's last tile
         ok = __all_sync(0xffffffffu, mbar_wait(&b_empty[sb], pb ^ 1u, kFaultWaitEmpty));
         if (!ok) break;
-        const uint32_t line = to + sb * B_STAGE_BYTES;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          st_shared_v4(line + (at ^ ((j & 1) ? 64u : 0u)) + j * 512, o[2 * j]);
-          st_shared_v4(line + (at ^ 16u ^ ((j & 1) ? 64u : 0u)) + j * 512, o[2 * j + 1]);
-        }
+        widen.store(smem_u32(sB) + sb * B_STAGE_BYTES, o);
         fence_proxy_async_shared();  // the MMA reads the tile through the async proxy
         __syncwarp();
         if (lane == 0) arrive_leader(&b_full[sb]);

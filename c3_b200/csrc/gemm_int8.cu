@@ -3,6 +3,7 @@
 #include <atomic>
 
 #include "gemm_ckpt.cuh"
+#include "gemm_ckpt_narrow.cuh"
 #include "host_util.h"
 #include "igemm.cuh"
 #include "igemv.cuh"
@@ -45,6 +46,56 @@ int launch_igemm_pair(const Operands& o, const igemm::Params& p, cudaStream_t st
                      "linear_int8: launch");
 }
 
+// Clusters of 1, 2, 4 and 8 CTAs of the small-tile kernels that run at once. Each such CTA takes an SM
+// for itself, and a cluster stays within one group of SMs, which need not hold a whole number of them:
+// a B200 ran 74 clusters of two, but 33 of four and 15 of eight.
+struct AtOnce {
+  int of[4];
+  int operator()(int split) const { return of[split >= 8 ? 3 : split >= 4 ? 2 : split - 1]; }
+};
+
+int query_clusters(int split) {
+  auto kern = ckpt_narrow::dw_narrow_kernel<32>;
+  constexpr int kSmem = static_cast<int>(ckpt_narrow::Ring<32>::kSmem);
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(split) * 64);
+  cfg.blockDim = dim3(ckpt_narrow::kThreads);
+  cfg.dynamicSmemBytes = kSmem;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = static_cast<unsigned>(split);
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  return n;
+}
+
+AtOnce clusters_at_once() {  // asked once per device
+  static std::atomic<int> cached[64][4] = {};
+  AtOnce r;
+  const int sms = sm_count() > 0 ? sm_count() : 148;
+  int dev = 0;
+  const bool known = sm_count() > 0 && cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 64;
+  for (int i = 0; i < 4; ++i) {
+    const int split = 1 << i;
+    r.of[i] = split == 1 || !known ? 0 : cached[dev][i].load(std::memory_order_relaxed);
+    if (r.of[i] > 0) continue;
+    const int n = split == 1 || !known ? 0 : query_clusters(split);
+    r.of[i] = n > 0 ? n : sms / split > 0 ? sms / split : 1;
+    if (n > 0) cached[dev][i].store(n, std::memory_order_relaxed);
+  }
+  return r;
+}
+
 // How a forward runs: T = 0 for the pair kernel, else tiles of T tokens, each split along K over a
 // cluster of `split` CTAs.
 struct ForwardPlan {
@@ -71,6 +122,7 @@ ForwardPlan plan_forward(int64_t M, int64_t N, int64_t K) {
   if (gemm_max_ctas() > 0) return best;  // the persistent kernel keeps to the caller's CTAs
   double least = 5. + waves(pairs, sms / 2) * (3.2 + 0.265 * static_cast<double>(kb_pair));
   const int64_t kb = (K + igemm::narrow::BK - 1) / igemm::narrow::BK;
+  const AtOnce at_once = clusters_at_once();
   const int64_t n_tiles = (N + igemm::narrow::BN - 1) / igemm::narrow::BN;
   for (const auto& kind : kinds) {
     if (kind.T > 16 && kind.T >= 2 * M) break;  // half of it would do
@@ -78,7 +130,7 @@ ForwardPlan plan_forward(int64_t M, int64_t N, int64_t K) {
     for (int split = 1; split <= igemm::narrow::kMaxCluster && split <= kb; split *= 2) {
       const int64_t per = (kb + split - 1) / split;
       const double tile = static_cast<double>(per) * kind.c + (split > 1 ? 0.6 + 0.034 * kind.T : kind.e);
-      const double t = 3.3 + waves(tiles * split, sms) * tile;
+      const double t = 3.3 + waves(tiles, at_once(split)) * tile;
       if (t < least) {
         least = t;
         int stages = static_cast<int>(igemm::narrow::kMaxRing / igemm::narrow::stage_bytes(kind.T));
@@ -186,9 +238,11 @@ int check_gemm_sizes(const char* what, int64_t M, int64_t N, int64_t K) {
   return C3CU_OK;
 }
 
-// How a weight gradient runs: X widened in the kernel (raw) or once into the workspace, the tiles'
-// plan, and the workspace's parts (partial sums first, then the widened X).
+// How a weight gradient runs: in small tiles (T > 0) of T rows, each split over a cluster of `split`
+// CTAs, or in large ones: X widened in the kernel (raw) or once into the workspace, the tiles' plan,
+// and the workspace's parts (partial sums first, then the widened X).
 struct DwRun {
+  int T, split, kb_per_cta;
   bool raw;
   int clusters;
   ckpt::Plan plan;
@@ -218,7 +272,45 @@ int dw_run(int64_t M, int64_t N, int64_t K, DwRun* r) {
   const double rounds = static_cast<double>(r->plan.whole / r->clusters) * blocks +
                         (r->plan.rest > 0 ? r->plan.kb_per_piece : 0);
   const double whole_only = r->plan.rest > 0 ? rounds : static_cast<double>((tiles + r->clusters - 1) / r->clusters) * blocks;
-  r->raw = 0.2 * whole_only < 2.5 + 3. * static_cast<double>(M) * static_cast<double>(K) / 6e6;
+  const double widening = 3. * static_cast<double>(M) * static_cast<double>(K) / 6e6;
+  r->raw = 0.2 * whole_only < 2.5 + widening;
+  // The faster kernel by a model of both, fitted to B200 measurements (us; K blocks of 64 rows of X):
+  //   large  3.3 + waves * 2.6 + blocks (0.43 RAW, 0.36 else) + cut tiles 2.8 + 0.09 pieces + widening
+  //   small  1.3 + waves (blocks c(T) + e(T)), e for a split tile 3.5 + 0.021 T
+  // Over 57 random sizes it misses the fastest form by 0.8 % on average, large tiles alone by 29 %.
+  // Measured, small / large: 256 x 784 over 128 rows 4.1 / 6.5, 32 x 25 over 2908 6.9 / 11.1, 1024 x
+  // 1024 over 2048 13.8 / 15.9, 2176 x 4822 over 576 37 / 21.
+  r->T = 0;
+  if (gemm_max_ctas() == 0) {  // else the persistent kernel keeps to the caller's CTAs
+    const double turns = static_cast<double>((tiles + r->clusters - 1) / r->clusters);
+    double least = 3.3 + 2.6 * turns + (r->raw ? 0.43 : 0.36) * whole_only +
+                   (r->plan.rest > 0 ? 2.8 + 0.09 * r->plan.rest * r->plan.pieces : 0.) + (r->raw ? 0. : 1. + widening);
+    constexpr struct {
+      int T;
+      double c, e;
+    } kinds[] = {{32, 0.37, 2.6}, {64, 0.40, 2.9}, {128, 0.44, 3.8}};
+    const int64_t k_tiles = (K + ckpt_narrow::COLS - 1) / ckpt_narrow::COLS;
+    const AtOnce at_once = clusters_at_once();
+    for (const auto& kind : kinds) {
+      if (kind.T > 32 && kind.T >= 2 * N) break;  // half of it would do
+      const int64_t small = k_tiles * ((N + kind.T - 1) / kind.T);
+      for (int split = 1; split <= ckpt_narrow::kMaxCluster && split <= blocks; split *= 2) {
+        const int per = (blocks + split - 1) / split;
+        const double t = 1.3 + static_cast<double>((small + at_once(split) - 1) / at_once(split)) *
+                                   (per * kind.c + (split > 1 ? 3.5 + 0.021 * kind.T : kind.e));
+        if (t < least) {
+          least = t;
+          r->T = kind.T;
+          r->split = split;
+          r->kb_per_cta = per;
+        }
+      }
+    }
+  }
+  if (r->T > 0) {
+    r->partial_bytes = r->wide_bytes = 0;
+    return C3CU_OK;
+  }
   const int rc = r->raw ? dw_clusters<true>(&r->clusters) : dw_clusters<false>(&r->clusters);
   r->plan = ckpt::make_plan(static_cast<int>(tiles), r->clusters, blocks);
   r->partial_bytes = static_cast<size_t>(r->plan.rest) * r->plan.pieces * ckpt::TM * ckpt::TN * sizeof(float);
@@ -239,6 +331,30 @@ int launch_dw(const CUtensorMap& ta, const CUtensorMap& tx, const ckpt::Params& 
   return cuda_status(launch_next(ckpt::add_pieces_kernel, dim3(ckpt::TM / ckpt::kAddRows, p.plan.rest), dim3(ckpt::TN),
                                  0, st, p),
                      "gemm_dw_int8: launch");
+}
+
+template <int T>
+int launch_dw_narrow(const CUtensorMap& tz, const CUtensorMap& tx, const ckpt_narrow::Params& p, int split,
+                     cudaStream_t st) {
+  auto kern = ckpt_narrow::dw_narrow_kernel<T>;
+  static std::atomic<uint64_t> smem_set{0};
+  const int rc = set_max_dynamic_smem(reinterpret_cast<const void*>(kern), ckpt_narrow::Ring<T>::kSmem, smem_set,
+                            "gemm_dw_int8: set max dynamic shared memory");
+  if (rc != C3CU_OK) return rc;
+  const int64_t grid = static_cast<int64_t>(p.k_tiles) * ((p.N + T - 1) / T) * split;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.blockDim = dim3(ckpt_narrow::kThreads);
+  cfg.dynamicSmemBytes = ckpt_narrow::Ring<T>::kSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = static_cast<unsigned>(split);
+  attr.val.clusterDim.y = 1;
+  attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cuda_status(cudaLaunchKernelEx(&cfg, kern, tz, tx, p), "gemm_dw_int8: launch");
 }
 
 }  // namespace
@@ -356,6 +472,15 @@ extern "C" int c3cu_gemm_dw_int8(const void* dZ, int64_t lddz, const int8_t* X, 
   if ((rc = encode_bf16_2d_sw128(&ta, dZ, M, N, lddz, 64, ckpt::BK)) != C3CU_OK) return rc;
   // X's rows are checked by the same rule in both forms
   if ((rc = encode_int8_2d(&tx, X, M, K, ldx, ckpt::HN, ckpt::BK, false)) != C3CU_OK) return rc;
+  if (r.T > 0) {
+    const ckpt_narrow::Params q{p.M, p.N, p.K, p.out, p.ldo, p.scale, r.kb_per_cta,
+                                (p.K + ckpt_narrow::COLS - 1) / ckpt_narrow::COLS};
+    switch (r.T) {
+      case 32: return launch_dw_narrow<32>(ta, tx, q, r.split, st);
+      case 64: return launch_dw_narrow<64>(ta, tx, q, r.split, st);
+      default: return launch_dw_narrow<128>(ta, tx, q, r.split, st);
+    }
+  }
   if (r.raw) return launch_dw<true>(ta, tx, p, r.clusters, st);
   __nv_bfloat16* wide = reinterpret_cast<__nv_bfloat16*>(static_cast<uint8_t*>(workspace) + r.partial_bytes);
   const int64_t want = (M + ckpt::kWidenWarps - 1) / ckpt::kWidenWarps, most = static_cast<int64_t>(sm_count()) * 8;
