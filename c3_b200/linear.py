@@ -110,6 +110,21 @@ def _vector_of(t: torch.Tensor, name: str, dtype: torch.dtype, n: int, dev: int)
         _same_device(t, name, dev)
 
 
+def _require_apart(out: torch.Tensor, name: str, *inputs) -> None:
+    """Refuses a given output (2-D, unit column stride) whose memory reaches into an input's: other
+    rows of that input may still be read when it is written. `inputs` are (tensor, name) pairs."""
+    if out.numel() == 0:
+        return
+    a = out.data_ptr()
+    end = a + ((out.shape[0] - 1) * out.stride(0) + out.shape[1]) * out.element_size()
+    for t, other in inputs:
+        if t is None or t.numel() == 0:
+            continue
+        b = t.data_ptr()
+        if a < b + ((t.shape[0] - 1) * t.stride(0) + t.shape[1]) * t.element_size() and b < end:
+            raise _lib.C3CUError(-1, name, f"overlaps {other}")
+
+
 def _same_device(t: torch.Tensor, name: str, dev: int) -> None:
     if t.get_device() != dev:
         raise _lib.C3CUError(-1, name, f"on device {t.get_device()}, the first operand on {dev}")
@@ -342,6 +357,7 @@ def forward_int8(Xq: torch.Tensor, x_scale: torch.Tensor, Wq: torch.Tensor, w_sc
     ldy, ldm = N, words
     if Y is not None:
         ldy = _rows_of(Y, "Y", out_dtype, M, N, dev)
+        _require_apart(Y, "Y", (Xq, "Xq"), (Wq, "Wq"))
     if mask is not None:
         if not (relu and save_mask):
             raise _lib.C3CUError(-1, "mask", "a mask belongs to the ReLU output (relu and save_mask)")
@@ -377,6 +393,7 @@ def grad_weight_int8(dZ: torch.Tensor, Xq: torch.Tensor, x_scale: torch.Tensor, 
     lddw = K
     if dW is not None:
         lddw = _rows_of(dW, "dW", torch.bfloat16, N, K, dev)
+        _require_apart(dW, "dW", (dZ, "dZ"), (Xq, "Xq"))
     else:
         dW = torch.empty(N, K, dtype=torch.bfloat16, device=dZ.device)
     # the workspace is of this call alone: a graph that captures it keeps its own

@@ -11,7 +11,8 @@ import math
 import torch
 
 from . import _lib
-from .linear import _call, _current_device, _fast_result, _on_gpu, _ptr, _rows_of, _vector_of
+from .linear import (_call, _current_device, _fast_result, _on_gpu, _ptr, _require_apart, _rows_of,
+                     _vector_of)
 from .quant import _dtype_code, empty_rows, row_stride
 
 
@@ -53,6 +54,7 @@ def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, resi
         q, ldq = empty_rows(M, K, x.device), row_stride(K)
     else:
         ldq = _rows_of(q, "q", torch.int8, M, K, dev)
+        _require_apart(q, "q", (x, "x"), (residual, "residual"), (h, "h"))
     if scale is None:
         scale = torch.empty(M, dtype=torch.float32, device=x.device)
     else:

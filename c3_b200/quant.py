@@ -9,7 +9,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .linear import _call, _fast_result, _on_gpu, _rows_of, _vector_of
+from .linear import _call, _fast_result, _on_gpu, _require_apart, _rows_of, _vector_of
 
 _DTYPES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16}
 
@@ -54,6 +54,7 @@ def quantize_rows(x: torch.Tensor, q: torch.Tensor | None = None, scale: torch.T
         q, ldq = empty_rows(M, K, x.device), row_stride(K)
     else:
         ldq = _rows_of(q, "q", torch.int8, M, K, dev)
+        _require_apart(q, "q", (x, "x"))
     if scale is None:
         scale = torch.empty(M, dtype=torch.float32, device=x.device)
     else:
