@@ -815,7 +815,108 @@ __global__ void __launch_bounds__(512) norm_bwd_kernel(const BwdArgs p) {
     if (R::any(t, i, G, p.K)) store_sums<T, SG>(out, t, i, G, p.K, acc[i]);
 }
 
-// Long rows: the rows' dot products first, then dx and dweight by strips of columns.
+// Rows of up to twice that length, on the 16-byte grid: 32 columns a thread, of which only dweight's
+// shares and the weights fit in registers. So each row is read twice from its buffer, for the dot
+// product and for dx, and the buffer is filled again behind the next row's reduction. Against strips,
+// which read dy and h twice from HBM, 5461 x 12288 bf16 took 96 us instead of 148 (83 at the copy rate).
+constexpr int kWideElems = 2 * kRowElems;
+constexpr int kWideThreads = 512;
+
+template <typename T>
+__global__ void __launch_bounds__(kWideThreads) norm_bwd_wide_kernel(const BwdArgs p) {
+  using R = Runs<T, 0>;
+  constexpr int V = R::V, N = kWideElems / V;
+  extern __shared__ __align__(128) uint8_t rows[];
+  __shared__ RowSums sums;
+  __shared__ RowRing ring;
+  const int t = threadIdx.x, G = kWideThreads;
+  const uint32_t bytes = static_cast<uint32_t>(p.K) * sizeof(T);
+  const uint32_t stage = (p.dh ? 3u : 2u) * bytes;
+  pdl_launch_dependents();
+  auto fill = [&](int s, int64_t row) {
+    uint8_t* to = rows + s * stage;
+    mbar_arrive_expect_tx(&ring.full[s], stage);
+    bulk_load(to, static_cast<const T*>(p.dy) + row * p.ldy, bytes, &ring.full[s]);
+    bulk_load(to + bytes, static_cast<const T*>(p.h) + row * p.ldhh, bytes, &ring.full[s]);
+    if (p.dh) bulk_load(to + 2 * bytes, static_cast<const T*>(p.dh) + row * p.lddh, bytes, &ring.full[s]);
+  };
+  if (t == 0) {
+    for (int s = 0; s < p.stages; ++s) mbar_init(&ring.full[s], 1);
+    fence_mbarrier_init();
+    fence_proxy_async_shared();
+    for (int s = 0; s < p.stages; ++s) {
+      const int64_t row = blockIdx.x + static_cast<int64_t>(s) * gridDim.x;
+      if (row < p.M) fill(s, row);
+    }
+  }
+  Run<V> w[N], acc[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    clear(acc[i]);
+    if (R::any(t, i, G, p.K)) load_weight<T, 0>(p.weight, t, i, G, p.K, w[i]);
+    else clear(w[i]);
+  }
+  const float inv_k = __fdiv_rn(1.f, static_cast<float>(p.K));
+  __syncthreads();
+  int s = 0, flip = 0, last = -1;  // last: the buffer of the row before
+  uint32_t ph = 0;
+  int64_t row = blockIdx.x;
+  for (; row < p.M; row += gridDim.x) {
+    const float rs = __ldg(p.rstd + row);
+    if (!mbar_wait(&ring.full[s], ph, kFaultWaitFull)) break;
+    const uint4* dy = reinterpret_cast<const uint4*>(rows + s * stage);
+    const uint4* h = reinterpret_cast<const uint4*>(rows + s * stage + bytes);
+    const uint4* dh = reinterpret_cast<const uint4*>(rows + s * stage + 2u * bytes);
+    float2 dots = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (!R::any(t, i, G, p.K)) continue;
+      Run<V> g, xh;
+      expand<T>(dy[t + i * G], g);
+      expand<T>(h[t + i * G], xh);
+#pragma unroll
+      for (int j = 0; j < V / 2; ++j) {
+        xh.v[j] = mul2(xh.v[j], both(rs));
+        acc[i].v[j] = fma2(g.v[j], xh.v[j], acc[i].v[j]);
+        dots = fma2(mul2(g.v[j], w[i].v[j]), xh.v[j], dots);
+      }
+    }
+    float dot = dots.x + dots.y;
+    uint32_t unused = 0u;
+    row_reduce<true, false>(dot, unused, &sums, flip);
+    flip ^= 1;
+    if (t == 0 && last >= 0) {
+      const int64_t next = row + static_cast<int64_t>(p.stages - 1) * gridDim.x;
+      if (next < p.M) fill(last, next);
+    }
+    dot *= -inv_k;
+    T* dx = static_cast<T*>(p.dx) + row * p.lddx;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (!R::any(t, i, G, p.K)) continue;
+      Run<V> g, xh, d;
+      expand<T>(dy[t + i * G], g);
+      expand<T>(h[t + i * G], xh);
+      clear(d);
+      if (p.dh) expand<T>(dh[t + i * G], d);
+#pragma unroll
+      for (int j = 0; j < V / 2; ++j) {
+        xh.v[j] = mul2(xh.v[j], both(rs));
+        d.v[j] = fma2(both(rs), fma2(xh.v[j], both(dot), mul2(g.v[j], w[i].v[j])), d.v[j]);
+      }
+      store<T, 0>(dx, t, i, G, p.K, d);
+    }
+    last = s;
+    if (++s == p.stages) { s = 0; ph ^= 1u; }
+  }
+  if (row < p.M && t == 0) settle_rows(ring, p.stages, s, ph, row, p.M);
+  float* out = p.partial + static_cast<int64_t>(blockIdx.x) * p.K;
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (R::any(t, i, G, p.K)) store_sums<T, 0>(out, t, i, G, p.K, acc[i]);
+}
+
+// Longer rows, and those off the 16-byte grid: the rows' dot products first, then dx and dweight by strips of columns.
 constexpr int kStripThreads = 128;
 
 template <typename T, int SG>
@@ -1012,7 +1113,7 @@ int fwd(const FwdArgs& p, bool norm, cudaStream_t st, const char* what) {
   return cuda_status(err, what);
 }
 
-constexpr int kBwdMaxK = 512 * kRowElems;  // beyond: strips
+constexpr int kBwdMaxK = 512 * kRowElems;  // beyond: two reads of a buffer, or strips
 
 // Rows of a strip block: enough blocks for every SM to have eight, at least 16 rows, and a grid
 // whose y dimension keeps its limit.
@@ -1080,6 +1181,26 @@ cudaError_t launch_bwd_rows(const BwdArgs& p, bool vec, int rows, int threads, c
   }
 }
 
+// Buffers of norm_bwd_wide_kernel's ring, or 0 for strips: rows of which not two fit, or too few rows for
+// a block on each SM (3 x 12288 bf16: 7.8 us in strips, 14 in this kernel; 40 rows: 14.4 both).
+int wide_stages(int64_t M, int64_t K, int esize, bool dh) {
+  if (K > kWideThreads * kWideElems || M < sm_count()) return 0;
+  const int64_t stages = (kRingSmem - 2048) / (K * esize * (dh ? 3 : 2));
+  return stages < 2 ? 0 : static_cast<int>(stages < kMaxStages ? stages : kMaxStages);
+}
+
+template <typename T>
+cudaError_t launch_bwd_wide(BwdArgs p, int blocks, int stages, cudaStream_t st) {
+  auto kern = norm_bwd_wide_kernel<T>;
+  static std::atomic<uint64_t> smem_set{0};
+  if (set_max_dynamic_smem(reinterpret_cast<const void*>(kern), kRingSmem, smem_set,
+                           "rms_norm_bwd: set shared memory") != C3CU_OK)
+    return cudaErrorInvalidValue;
+  p.stages = stages;
+  kern<<<blocks, kWideThreads, static_cast<size_t>(stages) * p.K * sizeof(T) * (p.dh ? 3 : 2), st>>>(p);
+  return cudaGetLastError();
+}
+
 template <typename T, int SG>
 cudaError_t launch_bwd_strips(BwdArgs p, float* dots, int rows, cudaStream_t st) {
   constexpr int kCols = kStripThreads * Runs<T, SG>::V;
@@ -1093,11 +1214,16 @@ cudaError_t launch_bwd_strips(BwdArgs p, float* dots, int rows, cudaStream_t st)
 template <typename T>
 int bwd(BwdArgs p, bool vec, float* ws, cudaStream_t st) {
   const int cols = kStripThreads * (vec ? Runs<T, 0>::V : 8);
-  const int rows = static_cast<int>(bwd_partial_rows(p.M, p.K, vec, cols));
+  int rows = static_cast<int>(bwd_partial_rows(p.M, p.K, vec, cols));
+  const int stages = vec && p.K > kBwdMaxK ? wide_stages(p.M, p.K, sizeof(T), p.dh != nullptr) : 0;
   cudaError_t err;
   if (p.K <= kBwdMaxK) {
     p.partial = ws;
     err = launch_bwd_rows<T>(p, vec, rows, bwd_threads(p.K, vec), st);
+  } else if (stages > 0) {
+    rows = sm_count();  // a block on each
+    p.partial = ws;
+    err = launch_bwd_wide<T>(p, rows, stages, st);
   } else {
     p.partial = ws + p.M;
     err = vec ? launch_bwd_strips<T, 0>(p, ws, rows, st) : launch_bwd_strips<T, kStripThreads>(p, ws, rows, st);
@@ -1211,6 +1337,7 @@ extern "C" size_t c3cu_rms_norm_bwd_workspace(int64_t M, int64_t K) {
       if (n > rows) rows = n;
     }
   }
+  if (K > quant::kBwdMaxK && M >= sm_count() && static_cast<size_t>(sm_count()) > rows) rows = sm_count();
   const size_t dots = K <= quant::kBwdMaxK ? 0 : static_cast<size_t>(M);
   return (dots + (rows > 1 ? rows * static_cast<size_t>(K) : 0)) * sizeof(float);
 }

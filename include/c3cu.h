@@ -280,11 +280,12 @@ int c3cu_set_attn_variant(int variant);
  * q[m][k] = the integer nearest to 127 x[m][k] / A, ties to even, A = max_k |x[m][k]|;
  * scale[m] = A / 127. The rounding is that of the real quotient, whatever the launch. A row of
  * zeros has scale 0; a row that holds an infinity or a NaN has q = 0 and scale NaN, so all that
- * is computed from it is NaN. dtype: of X, C3CU_DTYPE_F32 or C3CU_DTYPE_BF16. K >= 1. */
+ * is computed from it is NaN. Outputs may not reach into inputs but where it is said. A capped
+ * caller (c3cu_set_gemm_max_ctas) gets the persistent kernels of the two GEMMs. dtype: of X, C3CU_DTYPE_F32 or C3CU_DTYPE_BF16. K >= 1. */
 int c3cu_quantize_rows(const void* X, int64_t ldx, int dtype, int8_t* Q, int64_t ldq, float* scale, int64_t M,
                        int64_t K, c3cu_stream_t stream);
 /* RMS norm with the residual's addition and the output in that form:
- *   h = x + r (rounded to dtype; r and H may be NULL together: then h is x),
+ *   h = x + r (rounded to dtype; R and H may be NULL together: then h is x),
  *   rstd = 1 / sqrt(mean_k h^2 + eps), y = h * rstd * weight,
  *   q = nearest integer to 127 a / A with a = fl32(h * weight), A = max_k |a|; scale = A rstd / 127.
  * Squares are summed in fp32 (|h| up to about 1e18). H may be X or R itself (same stride). */
