@@ -157,6 +157,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::kThreads, 1)
     igemm_pair_kernel(const __grid_constant__ CUtensorMap tmw, const __grid_constant__ CUtensorMap tmx,
                       const Params p) {
   using namespace pair;
+  __shared__ __align__(16) float s_xs[kEpiWarps][32];  // each warp's own: the scales of the tokens it works on
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
@@ -270,6 +271,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::kThreads, 1)
   } else {
     // ------------------------------------------------------------ epilogue (warps 2..9)
     const uint32_t q = warp & 3u;
+    float* my_xs = s_xs[warp - 2u];
     const int c_lo = static_cast<int>((warp - 2u) >> 2) * kWarpTokens;  // this warp's share of the tokens
     uint32_t acc = 0, acc_ph = 0;
     for (int tile = cluster; tile < num_tiles; tile += num_clusters) {
@@ -301,9 +303,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::kThreads, 1)
           if (lane == 0) arrive_leader(&acc_empty[acc]);
         }
         const int m = m0 + c * 32;
+        my_xs[lane] = xs[c];
+        __syncwarp();
         if (m < p.M)
           store_tokens<32, F32, RELU>(
-              p, r[c & 1], [&](int j) { return __shfl_sync(0xffffffffu, xs[c], j); }, m, p.M - m, n, ws, b, lane);
+              p, r[c & 1], [&](int j) { return my_xs[j]; }, m, p.M - m, n, ws, b, lane);
+        __syncwarp();
       }
       __syncwarp();
       acc ^= 1u;
