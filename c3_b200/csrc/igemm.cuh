@@ -12,8 +12,12 @@
 // the tokens its columns, so that few tokens leave no tensor-core rows empty and a warp's stores run
 // along a row of Y.
 //   igemm_pair_kernel    tiles of 256 channels x 256 tokens on CTA pairs (cta_group::2), persistent:
-//                        the structure of gemm2_kernel with int8 K blocks. For many tiles.
-//   igemm_narrow_kernel  128 channels x T tokens per CTA. The K blocks of a tile are
+//                        the structure of gemm2_kernel with int8 K blocks. For many tiles. 8192 x
+//                        4096 x 4096: 92 us (3.0 POP/s) on a cool chip, 112 at the power limit. A tile
+//                        costs 2.4 us beside its MMAs, at K 16384 as at 256: the epilogue's
+//                        arithmetic, mask and stores slow the MMAs that they overlap (78 us without).
+//   igemm_narrow_kernel  128 channels x T tokens per CTA (40 x 4096 x 4096: 7.0 us in a graph, of
+//                        which reading W once is 2.6). The K blocks of a tile are
 //                        split over a cluster whose CTAs add their int32 partial sums through
 //                        distributed shared memory: with few tokens the weights are the traffic,
 //                        and the split lets all SMs read them.

@@ -451,7 +451,8 @@ __device__ __forceinline__ void accumulate(Run<V>& a, const Run<V>& w, float2& s
 }
 
 // One row per block (or, with 32 threads a row, per warp), held in registers between the reduction
-// and the rounding.
+// and the rounding. For few rows, where the launch is most of the time (a token of 4096 with the norm:
+// 2.2 us in a graph, an empty kernel 2.1).
 template <typename T, bool NORM, bool RES, int SG, int N, bool WARP>
 __global__ void __launch_bounds__(WARP ? 128 : 1024) rows_kernel(const FwdArgs p) {
   using R = Runs<T, SG>;
@@ -505,7 +506,9 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024) rows_kernel(const FwdArgs p
   if (t == 0) row_outputs(p, row, sum, r, NORM);
 }
 
-// The same over many rows, grid-strided, through the ring.
+// The same over many rows, grid-strided, through the ring. 16384 x 4096 bf16: norm with residual 76.5
+// us (6.1 TB/s; a block a row 88), quantising alone 41 us (4.9 TB/s, a block a row 57), which the issue
+// slots bound: the rounding costs about fifteen instructions an element.
 template <typename T, bool NORM, bool RES, int SG, int N>
 __global__ void __launch_bounds__(1024) ring_rows_kernel(const FwdArgs p) {
   using R = Runs<T, SG>;
@@ -680,7 +683,8 @@ struct BwdArgs {
 // g = w dy, xhat = h rstd: dx = rstd (g - xhat mean(g xhat)) + dh, dweight = sum_rows dy xhat.
 // A block walks over rows (grid-strided); a thread owns the same N runs of columns in each, so
 // dweight's share of the block stays in registers until the end. RING: rows come through the ring
-// of buffers (16-byte rows only); else straight from global memory.
+// of buffers; else straight from global memory. 16384 x 4096 bf16 with dh: 88.5 us with the sum of the
+// shares (6.1 TB/s), 124 without the ring.
 template <typename T, bool RING, int SG>
 __global__ void __launch_bounds__(512) norm_bwd_kernel(const BwdArgs p) {
   using R = Runs<T, SG>;
@@ -917,7 +921,8 @@ __global__ void __launch_bounds__(kWideThreads) norm_bwd_wide_kernel(const BwdAr
     if (R::any(t, i, G, p.K)) store_sums<T, 0>(out, t, i, G, p.K, acc[i]);
 }
 
-// Longer rows, and those off the 16-byte grid: the rows' dot products first, then dx and dweight by strips of columns.
+// Longer rows, and those off the 16-byte grid: the rows' dot products first, then dx and dweight by
+// strips of columns, so that dy and h are read twice. Off the grid 5461 x 12287 bf16 takes 293 us.
 constexpr int kStripThreads = 128;
 
 template <typename T, int SG>
