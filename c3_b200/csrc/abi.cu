@@ -4,7 +4,6 @@
 #include <cudaTypedefs.h>
 
 #include <mutex>
-#include <vector>
 
 #include "common.cuh"
 #include "host_util.h"
@@ -62,18 +61,15 @@ int set_max_dynamic_smem(const void* kernel, int bytes, std::atomic<uint64_t>& d
 }
 
 int sm_count() {
-  static std::mutex mu;
-  static std::vector<int> cache;
+  static std::atomic<int> cache[64] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return 0;
-  std::lock_guard<std::mutex> lock(mu);
-  if (static_cast<int>(cache.size()) <= dev) cache.resize(dev + 1, 0);
-  if (cache[dev] == 0) {
-    int n = 0;
-    cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-    cache[dev] = n;
-  }
-  return cache[dev];
+  const bool cached = dev >= 0 && dev < 64;
+  int n = cached ? cache[dev].load(std::memory_order_relaxed) : 0;
+  if (n > 0) return n;
+  cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+  if (cached) cache[dev].store(n, std::memory_order_relaxed);
+  return n;
 }
 
 int require_sm100() {

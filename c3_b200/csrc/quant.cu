@@ -1159,7 +1159,8 @@ int bwd_blocks_per_sm(int threads) { return 512 / threads < 16 ? 512 / threads :
 size_t bwd_partial_rows(int64_t M, int64_t K, bool vec, int cols) {
   if (K <= kBwdMaxK) {
     if (M <= 4) return 1;  // one block walks over them in less time than a second launch takes
-    const int64_t most = static_cast<int64_t>(sm_count() > 0 ? sm_count() : 148) * bwd_blocks_per_sm(bwd_threads(K, vec));
+    const int sms = sm_count();
+    const int64_t most = static_cast<int64_t>(sms > 0 ? sms : 148) * bwd_blocks_per_sm(bwd_threads(K, vec));
     // A row more for a block costs about 0.65 us; a block's share of dweight, written and added up, 1.3 us
     // per MB. Measured (us) with 1, 2, 3, 4 rows a block: 1000 x 1024 bf16 9.4, 7.9, 7.4, 8.1; 333 x 2048
     // 8.6, 7.5, 6.9, 7.7; 333 x 512 4.3, 4.8, 6.3, 7.0.
@@ -1357,6 +1358,7 @@ extern "C" size_t c3cu_rms_norm_bwd_workspace(int64_t M, int64_t K) {
     for (int v : {4, 8}) {
       const size_t n = quant::bwd_partial_rows(M, K, vec, quant::kStripThreads * v);
       if (n > rows) rows = n;
+      if (K <= quant::kBwdMaxK) break;  // only strips depend on v
     }
   }
   if (K > quant::kBwdMaxK && M >= sm_count() && static_cast<size_t>(sm_count()) > rows) rows = sm_count();
