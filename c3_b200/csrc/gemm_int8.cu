@@ -103,9 +103,10 @@ struct ForwardPlan {
 };
 
 // The faster kernel by a model of both, fitted to B200 measurements (us; kb = K blocks of a CTA):
-//   narrow  3.3 + waves (kb c(T) + e(T)), e being the epilogue, or for a split tile the exchange of
-//           partial sums 0.6 + 0.034 T
-//   pair    5 + waves (3.2 + 0.265 kb)
+//   narrow  3.2 + waves (kb c(T) + e(T)), e being the epilogue, or for a split tile the exchange of
+//           partial sums 1.2 + 0.028 tokens
+//   pair    2.5 + waves (4.0 + 0.27 kb)
+// Over 196 random sizes its choice takes 1.4 % longer than the fastest form on average.
 // Measured (us), 4096 channels x K 4096: 8 tokens 5.8 (T 16, split 4) against 13.4 (pair), 64 tokens
 // 7.8 (T 64, split 4) / 13.6, 512 tokens 12.5 (T 128) / 16.8, 1024 tokens 19.0 (T 256) / 17.9; 12288
 // channels x K 1024, 2048 tokens 54 (T 256) / 34.
@@ -113,14 +114,14 @@ ForwardPlan plan_forward(int64_t M, int64_t N, int64_t K) {
   constexpr struct {
     int T;
     double c, e;
-  } kinds[] = {{16, 0.18, 0.3}, {32, 0.19, 0.4}, {64, 0.21, 0.9}, {128, 0.24, 2.1}, {256, 0.37, 4.5}};
+  } kinds[] = {{16, 0.21, 0.6}, {32, 0.22, 0.8}, {64, 0.23, 1.3}, {128, 0.27, 2.1}, {256, 0.40, 4.8}};
   const int sms = sm_count() > 0 ? sm_count() : 148;
   const auto waves = [](int64_t work, int64_t at_once) { return static_cast<double>((work + at_once - 1) / at_once); };
   const int64_t kb_pair = (K + igemm::pair::BK - 1) / igemm::pair::BK;
   const int64_t pairs = ((N + gemm2::TM - 1) / gemm2::TM) * ((M + gemm2::TN - 1) / gemm2::TN);
   ForwardPlan best{0, 1, 0, 0};
   if (gemm_max_ctas() > 0) return best;  // the persistent kernel keeps to the caller's CTAs
-  double least = 5. + waves(pairs, sms / 2) * (3.2 + 0.265 * static_cast<double>(kb_pair));
+  double least = 2.5 + waves(pairs, sms / 2) * (4.0 + 0.27 * static_cast<double>(kb_pair));
   const int64_t kb = (K + igemm::narrow::BK - 1) / igemm::narrow::BK;
   const AtOnce at_once = clusters_at_once();
   const int64_t n_tiles = (N + igemm::narrow::BN - 1) / igemm::narrow::BN;
@@ -129,8 +130,9 @@ ForwardPlan plan_forward(int64_t M, int64_t N, int64_t K) {
     const int64_t tiles = n_tiles * ((M + kind.T - 1) / kind.T);
     for (int split = 1; split <= igemm::narrow::kMaxCluster && split <= kb; split *= 2) {
       const int64_t per = (kb + split - 1) / split;
-      const double tile = static_cast<double>(per) * kind.c + (split > 1 ? 0.6 + 0.034 * kind.T : kind.e);
-      const double t = 3.3 + waves(tiles, at_once(split)) * tile;
+      const double exchange = 1.2 + 0.028 * static_cast<double>(M < kind.T ? M : kind.T);
+      const double tile = static_cast<double>(per) * kind.c + (split > 1 ? exchange : kind.e);
+      const double t = 3.2 + waves(tiles, at_once(split)) * tile;
       if (t < least) {
         least = t;
         int stages = static_cast<int>(igemm::narrow::kMaxRing / igemm::narrow::stage_bytes(kind.T));
