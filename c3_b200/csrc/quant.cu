@@ -820,30 +820,47 @@ __global__ void __launch_bounds__(512) norm_bwd_kernel(const BwdArgs p) {
     if (R::any(t, i, G, p.K)) store_sums<T, SG>(out, t, i, G, p.K, acc[i]);
 }
 
-// Rows of up to twice that length, on the 16-byte grid: 32 columns a thread, of which only dweight's
+// Rows of up to twice that length: 32 columns a thread, of which only dweight's
 // shares and the weights fit in registers. So each row is read twice from its buffer, for the dot
 // product and for dx, and the buffer is filled again behind the next row's reduction. Against strips,
-// which read dy and h twice from HBM, 5461 x 12288 bf16 took 96 us instead of 148 (83 at the copy rate).
+// which read dy and h twice from HBM, 5461 x 12288 bf16 took 96 us instead of 148 (83 at the copy rate),
+// and off the 16-byte grid 5461 x 12287 130 instead of 293.
 constexpr int kWideElems = 2 * kRowElems;
 constexpr int kWideThreads = 512;
 
-template <typename T>
+template <typename T, int SG>
 __global__ void __launch_bounds__(kWideThreads) norm_bwd_wide_kernel(const BwdArgs p) {
-  using R = Runs<T, 0>;
+  using R = Runs<T, SG>;
   constexpr int V = R::V, N = kWideElems / V;
   extern __shared__ __align__(128) uint8_t rows[];
   __shared__ RowSums sums;
   __shared__ RowRing ring;
   const int t = threadIdx.x, G = kWideThreads;
   const uint32_t bytes = static_cast<uint32_t>(p.K) * sizeof(T);
-  const uint32_t stage = (p.dh ? 3u : 2u) * bytes;
+  const uint32_t pitch = row_pitch(bytes, SG == 0);
+  const uint32_t stage = (p.dh ? 3u : 2u) * pitch;
   pdl_launch_dependents();
   auto fill = [&](int s, int64_t row) {
     uint8_t* to = rows + s * stage;
-    mbar_arrive_expect_tx(&ring.full[s], stage);
-    bulk_load(to, static_cast<const T*>(p.dy) + row * p.ldy, bytes, &ring.full[s]);
-    bulk_load(to + bytes, static_cast<const T*>(p.h) + row * p.ldhh, bytes, &ring.full[s]);
-    if (p.dh) bulk_load(to + 2 * bytes, static_cast<const T*>(p.dh) + row * p.lddh, bytes, &ring.full[s]);
+    if constexpr (SG == 0) {
+      mbar_arrive_expect_tx(&ring.full[s], stage);
+      bulk_load(to, static_cast<const T*>(p.dy) + row * p.ldy, bytes, &ring.full[s]);
+      bulk_load(to + pitch, static_cast<const T*>(p.h) + row * p.ldhh, bytes, &ring.full[s]);
+      if (p.dh) bulk_load(to + 2 * pitch, static_cast<const T*>(p.dh) + row * p.lddh, bytes, &ring.full[s]);
+    } else {
+      Span sp[3];
+      sp[0] = row_span<T>(p.dy, p.ldy, p.M, row, bytes);
+      sp[1] = row_span<T>(p.h, p.ldhh, p.M, row, bytes);
+      sp[2] = row_span<T>(p.dh, p.lddh, p.M, row, bytes);
+      if (!p.dh) sp[2].direct = true;
+      uint32_t tx = 0u;
+#pragma unroll
+      for (int k = 0; k < 3; ++k) tx += sp[k].direct ? 0u : sp[k].size;
+      mbar_arrive_expect_tx(&ring.full[s], tx);
+#pragma unroll
+      for (int k = 0; k < 3; ++k)
+        if (!sp[k].direct) bulk_load(to + k * pitch, sp[k].from, sp[k].size, &ring.full[s]);
+    }
   };
   if (t == 0) {
     for (int s = 0; s < p.stages; ++s) mbar_init(&ring.full[s], 1);
@@ -858,7 +875,7 @@ __global__ void __launch_bounds__(kWideThreads) norm_bwd_wide_kernel(const BwdAr
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     clear(acc[i]);
-    if (R::any(t, i, G, p.K)) load_weight<T, 0>(p.weight, t, i, G, p.K, w[i]);
+    if (R::any(t, i, G, p.K)) load_weight<T, SG>(p.weight, t, i, G, p.K, w[i]);
     else clear(w[i]);
   }
   const float inv_k = __fdiv_rn(1.f, static_cast<float>(p.K));
@@ -869,16 +886,30 @@ __global__ void __launch_bounds__(kWideThreads) norm_bwd_wide_kernel(const BwdAr
   for (; row < p.M; row += gridDim.x) {
     const float rs = __ldg(p.rstd + row);
     if (!mbar_wait(&ring.full[s], ph, kFaultWaitFull)) break;
-    const uint4* dy = reinterpret_cast<const uint4*>(rows + s * stage);
-    const uint4* h = reinterpret_cast<const uint4*>(rows + s * stage + bytes);
-    const uint4* dh = reinterpret_cast<const uint4*>(rows + s * stage + 2u * bytes);
+    // where the k-th input's row is: in its buffer, or (off the grid, the first and last) where it was
+    auto source = [&](int k, const void* base, int64_t ld) {
+      const uint8_t* at = rows + s * stage + k * pitch;
+      if constexpr (SG == 0) {
+        return reinterpret_cast<const T*>(at);
+      } else {
+        const Span sp = row_span<T>(base, ld, p.M, row, bytes);
+        return sp.direct ? static_cast<const T*>(base) + row * ld : reinterpret_cast<const T*>(at + sp.skip);
+      }
+    };
+    auto read = [&](const T* from, int i, Run<V>& v) {
+      if constexpr (SG == 0) expand<T>(reinterpret_cast<const uint4*>(from)[t + i * G], v);
+      else load<T, SG>(from, t, i, G, p.K, v);
+    };
+    const T* dy = source(0, p.dy, p.ldy);
+    const T* h = source(1, p.h, p.ldhh);
+    const T* dh = p.dh ? source(2, p.dh, p.lddh) : nullptr;
     float2 dots = make_float2(0.f, 0.f);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       if (!R::any(t, i, G, p.K)) continue;
       Run<V> g, xh;
-      expand<T>(dy[t + i * G], g);
-      expand<T>(h[t + i * G], xh);
+      read(dy, i, g);
+      read(h, i, xh);
 #pragma unroll
       for (int j = 0; j < V / 2; ++j) {
         xh.v[j] = mul2(xh.v[j], both(rs));
@@ -900,16 +931,16 @@ __global__ void __launch_bounds__(kWideThreads) norm_bwd_wide_kernel(const BwdAr
     for (int i = 0; i < N; ++i) {
       if (!R::any(t, i, G, p.K)) continue;
       Run<V> g, xh, d;
-      expand<T>(dy[t + i * G], g);
-      expand<T>(h[t + i * G], xh);
+      read(dy, i, g);
+      read(h, i, xh);
       clear(d);
-      if (p.dh) expand<T>(dh[t + i * G], d);
+      if (p.dh) read(dh, i, d);
 #pragma unroll
       for (int j = 0; j < V / 2; ++j) {
         xh.v[j] = mul2(xh.v[j], both(rs));
         d.v[j] = fma2(both(rs), fma2(xh.v[j], both(dot), mul2(g.v[j], w[i].v[j])), d.v[j]);
       }
-      store<T, 0>(dx, t, i, G, p.K, d);
+      store<T, SG>(dx, t, i, G, p.K, d);
     }
     last = s;
     if (++s == p.stages) { s = 0; ph ^= 1u; }
@@ -918,11 +949,11 @@ __global__ void __launch_bounds__(kWideThreads) norm_bwd_wide_kernel(const BwdAr
   float* out = p.partial + static_cast<int64_t>(blockIdx.x) * p.K;
 #pragma unroll
   for (int i = 0; i < N; ++i)
-    if (R::any(t, i, G, p.K)) store_sums<T, 0>(out, t, i, G, p.K, acc[i]);
+    if (R::any(t, i, G, p.K)) store_sums<T, SG>(out, t, i, G, p.K, acc[i]);
 }
 
-// Longer rows, and those off the 16-byte grid: the rows' dot products first, then dx and dweight by
-// strips of columns, so that dy and h are read twice. Off the grid 5461 x 12287 bf16 takes 293 us.
+// Longer rows, and few: the rows' dot products first, then dx and dweight by strips of columns, so that dy
+// and h are read twice.
 constexpr int kStripThreads = 128;
 
 template <typename T, int SG>
@@ -1206,21 +1237,22 @@ cudaError_t launch_bwd_rows(const BwdArgs& p, bool vec, int rows, int threads, c
 
 // Buffers of norm_bwd_wide_kernel's ring, or 0 for strips: rows of which not two fit, or too few rows for
 // a block on each SM (3 x 12288 bf16: 7.8 us in strips, 14 in this kernel; 40 rows: 14.4 both).
-int wide_stages(int64_t M, int64_t K, int esize, bool dh) {
+int wide_stages(int64_t M, int64_t K, int esize, bool vec, bool dh) {
   if (K > kWideThreads * kWideElems || M < sm_count()) return 0;
-  const int64_t stages = (kRingSmem - 2048) / (K * esize * (dh ? 3 : 2));
+  const int64_t stages = (kRingSmem - 2048) / (row_pitch(static_cast<uint32_t>(K * esize), vec) * (dh ? 3 : 2));
   return stages < 2 ? 0 : static_cast<int>(stages < kMaxStages ? stages : kMaxStages);
 }
 
-template <typename T>
+template <typename T, int SG>
 cudaError_t launch_bwd_wide(BwdArgs p, int blocks, int stages, cudaStream_t st) {
-  auto kern = norm_bwd_wide_kernel<T>;
+  auto kern = norm_bwd_wide_kernel<T, SG>;
   static std::atomic<uint64_t> smem_set{0};
   if (set_max_dynamic_smem(reinterpret_cast<const void*>(kern), kRingSmem, smem_set,
                            "rms_norm_bwd: set shared memory") != C3CU_OK)
     return cudaErrorInvalidValue;
   p.stages = stages;
-  kern<<<blocks, kWideThreads, static_cast<size_t>(stages) * p.K * sizeof(T) * (p.dh ? 3 : 2), st>>>(p);
+  kern<<<blocks, kWideThreads,
+         static_cast<size_t>(stages) * row_pitch(static_cast<uint32_t>(p.K) * sizeof(T), SG == 0) * (p.dh ? 3 : 2), st>>>(p);
   return cudaGetLastError();
 }
 
@@ -1238,7 +1270,7 @@ template <typename T>
 int bwd(BwdArgs p, bool vec, float* ws, cudaStream_t st) {
   const int cols = kStripThreads * (vec ? Runs<T, 0>::V : 8);
   int rows = static_cast<int>(bwd_partial_rows(p.M, p.K, vec, cols));
-  const int stages = vec && p.K > kBwdMaxK ? wide_stages(p.M, p.K, sizeof(T), p.dh != nullptr) : 0;
+  const int stages = p.K > kBwdMaxK ? wide_stages(p.M, p.K, sizeof(T), vec, p.dh != nullptr) : 0;
   cudaError_t err;
   if (p.K <= kBwdMaxK) {
     p.partial = ws;
@@ -1246,7 +1278,7 @@ int bwd(BwdArgs p, bool vec, float* ws, cudaStream_t st) {
   } else if (stages > 0) {
     rows = sm_count();  // a block on each
     p.partial = ws;
-    err = launch_bwd_wide<T>(p, rows, stages, st);
+    err = vec ? launch_bwd_wide<T, 0>(p, rows, stages, st) : launch_bwd_wide<T, kWideThreads>(p, rows, stages, st);
   } else {
     p.partial = ws + p.M;
     err = vec ? launch_bwd_strips<T, 0>(p, ws, rows, st) : launch_bwd_strips<T, kStripThreads>(p, ws, rows, st);

@@ -49,3 +49,24 @@ def test_wide_row_that_is_not_finite(cuda_device):
     rstd[7] = 0
     dx, dw = norm.rms_norm_backward(dy, h, w, rstd, dh=d)
     assert bool(torch.isnan(dx[7, 100])) and bool(torch.isfinite(dx[[6, 8]]).all()) and bool(torch.isnan(dw[100]))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("dh", [False, True])
+@pytest.mark.parametrize("m,k", [(148, 8193), (300, 9001), (400, 12287), (149, 16383), (150, 16385)])
+def test_wide_rows_off_the_16_byte_grid(cuda_device, m, k, dh, dtype):
+    dev = cuda_device
+    dy, h, w, rstd, d = _bwd_inputs(m, k, dtype, dh, dev, m + k)
+    want = norm.rms_norm_backward(dy, h, w, rstd, dh=d)
+    _check_bwd(dy, h, w, rstd, d, *want)
+    # rows that start anywhere, with other values around them, and dx over one of the inputs
+    wide = [torch.full((m, k + 13), 7.0, dtype=dtype, device=dev) for _ in range(3)]
+    views = [b[:, c:c + k] for b, c in zip(wide, (5, 1, 9))]
+    for v, t in zip(views, (dy, h, d)):
+        if t is not None:
+            v.copy_(t)
+    dx, dw = norm.rms_norm_backward(views[0], views[1], w, rstd, dh=views[2] if dh else None, dx=views[0])
+    assert torch.equal(dx, want[0]) and torch.equal(dw, want[1])
+    assert torch.equal(views[1], h) and (not dh or torch.equal(views[2], d))
+    views[0].fill_(7.0)
+    assert bool((wide[0] == 7).all())
