@@ -91,6 +91,7 @@ _SIGNATURES = {
                           _i),
     "c3cu_linear_int8_fwd": ([_vp, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i, _i, _vp, _i64, _i64, _i64, _i64,
                               _vp], _i),
+    "c3cu_set_int8_form": ([_i, _i, _i], _i),
     "c3cu_gemm_dw_int8_workspace": ([_i64, _i64, _i64], _sz),
     "c3cu_gemm_dw_int8": ([_vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _sz, _vp], _i),
     "c3cu_flash_attn_fwd": ([_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, ctypes.c_float, _i, _vp], _i),

@@ -153,6 +153,8 @@ int encode_bf16_2d_sw128(CUtensorMap* map, const void* base, uint64_t rows, uint
 
 int check_int8_rows(const void* base, uint64_t cols, uint64_t ld) { return check_tma_rows("int8", 1u, base, cols, ld); }
 
+int check_bf16_rows(const void* base, uint64_t cols, uint64_t ld) { return check_tma_rows("bf16", 2u, base, cols, ld); }
+
 int encode_int8_2d(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_cols,
                    uint32_t box_rows, bool swizzle) {
   return encode_2d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, "int8", 1u, base, rows, cols, ld, box_cols, box_rows, swizzle);

@@ -2,27 +2,33 @@
 //
 //   dW[N][K] = sum_m dZ[m][n] * (q[m][k] * scale[m])        (bf16 out, fp32 sums in TMEM)
 //
-// dZ is bf16, X is held as int8 rows with one fp32 scale each (c3cu_quantize_rows). The scale runs
-// along the sum, so it cannot wait for the epilogue: q * scale is rounded to bf16, the tensor
-// cores' operand type, on its way to them. That rounding (relative 2^-8 at most, the size of the
-// output's own) is the only one besides the output's; q itself would be exact in bf16.
+// dZ is bf16, X is held as int8 rows with one fp32 scale each (c3cu_quantize_rows). The scale runs along
+// the sum, so it cannot wait for the epilogue: it goes to an operand. q is exact in the tensor cores' 16-bit
+// types, so the scale goes to dZ, and the operand rounding is that of dZ * scale alone. In bf16 that
+// rounding (2^-8) would be as large as the output's own; so it is fp16 here (2^-11), and two bf16 terms
+// (2^-14) in the small tiles of gemm_ckpt_narrow.cuh. Against fp64 the error of dW is then the output
+// rounding's (0.0017 of the norm; 0.0024 with operands in bf16).
 //
-// dw_kernel has gemm2_kernel's structure (256 x 256 tiles on CTA pairs, both operands MN-major,
-// since dZ and X are stored with the sum's index as their rows). The MMA's rows are the columns of
-// dW, so that a warp's stores run along its rows whatever their alignment (2176 x 4822 over 576 rows:
-// 138 us with a row of dW per lane, 27 so). Two forms:
-//   RAW   TMA brings X's int8 block into a raw buffer and converter warps widen it into the
-//         swizzled bf16 tile that the MMA reads: X crosses HBM and L2 at one byte per element and
-//         no bf16 copy of it exists, but it is widened once for every 256 rows of dW.
-//   !RAW  X was widened once into a bf16 workspace (widen_kernel), which the kernel reads by TMA.
-// Beside the tensor cores the widening runs into the power limit and the shared-memory traffic of
-// the tiles (16384 x 4096 x 4096: 505 to 548 us RAW, 424 !RAW, of which widen_kernel 33; the bf16
-// gradient from a bf16 X takes 350 to 370 in the same loop). With few K blocks RAW saves the launch
-// (in these tiles 128 x 256 x 784 took 10.2 us RAW, 12.3 else; gemm_ckpt_narrow.cuh takes 6.2).
+// fp16 has five bits of exponent where bf16 has eight, so each column of dZ * scale, i.e. each row of dW,
+// is brought into its range by a power of two of its own:
+//   column_top_kernel  the largest finite |dZ * scale| of each column (in bands of rows)
+//   operands_kernel    dZ * scale * 2^(14 - e) in fp16, e the exponent of the column's largest, and q in
+//                      fp16, both into the workspace
+//   dw_kernel          the product, gemm2_kernel's structure (256 x 256 tiles on CTA pairs, both operands
+//                      MN-major, since dZ and X are stored with the sum's index as their rows); its epilogue
+//                      multiplies by 2^(e - 14), exactly
+// 16384 x 4096 x 4096: 480 to 500 us, of which the product takes 340 and the first two, which read dZ twice,
+// about 110. Operands rounded to bf16, for which X alone was rewritten, took 433 to 450.
+// An element is rounded by 2^-11 of itself or, from 2^-28 of its column's largest down, by 2^-39 of that
+// largest, which is below what fp32 sums over the column lose. What is not finite stays so.
 //
-// Warps: 0 TMA, 1 MMA (leader), 2..9 epilogue; RAW: 10..17 converters (two groups of four), 18 TMA
-// of X.
+// The MMA's rows are the columns of dW, so that a warp's stores run along its rows whatever their
+// alignment (2176 x 4822 over 576 rows: 138 us with a row of dW per lane, 27 so).
+//
+// Warps of dw_kernel: 0 TMA, 1 MMA (leader), 2..9 epilogue.
 #pragma once
+
+#include <cuda_fp16.h>
 
 #include "ckpt_schedule.h"
 #include "gemm2_tcgen05.cuh"
@@ -37,147 +43,36 @@ using gemm2::HM;
 using gemm2::HN;
 using gemm2::kEpiWarps;
 using gemm2::kPairMask;
+using gemm2::kThreads;
 using gemm2::MN_CHUNK_BYTES;
+using gemm2::SMEM_BYTES;
+using gemm2::STAGE_BYTES;
+using gemm2::STAGES;
 using gemm2::TM;
 using gemm2::TMEM_COLS;
 using gemm2::TN;
 using gemm2::UMMA_K;
-constexpr int kConvWarps = 4;   // a group's warps
-constexpr int kConvGroups = 2;  // the groups take K blocks in turn
-constexpr int kRawWarp = 2 + kEpiWarps + kConvGroups * kConvWarps;
-constexpr uint32_t RAW_BYTES = BK * HN;  // 64 rows (m) of 128 int8 (k)
-
-// Ring depths. RAW: dZ, raw int8 and widened tiles go through rings of their own, so that the
-// loads' latency and the conversion's are each hidden by as many stages as they take. !RAW: one
-// ring of both operands' stages.
-template <bool RAW>
-struct Ring {
-  static constexpr int kA = RAW ? 5 : 7;
-  static constexpr int kB = RAW ? 4 : 7;
-  static constexpr int kRaw = RAW ? 8 : 0;
-  static constexpr int kThreads = RAW ? 32 * (kRawWarp + 1) : 32 * (2 + kEpiWarps);
-  static constexpr uint32_t kBytes = kA * A_STAGE_BYTES + kB * B_STAGE_BYTES + kRaw * RAW_BYTES;
-  static constexpr uint32_t kSmem = kBytes + 2 * (kA + kB + kRaw) * 8 + 5 * 8 + 8 + 1024;
-  static_assert(kSmem <= 227 * 1024, "shared memory");
-  static_assert(kB % kConvGroups == 0 || !RAW, "a stage belongs to one group, which so sees each of its phases");
-};
 
 struct Params {
   int32_t M, N, K;     // dW is N x K, the sum runs over M
   __nv_bfloat16* out;
   int64_t ldo;
-  const float* scale;  // [M]
-  float* partial;      // slots of [256 rows][256 columns] fp32
+  const float* back;   // [N, padded to 64]: 2^(e - 14) of each row of dW
+  float* partial;      // slots of [256 rows][256 columns] fp32, not yet multiplied by it
   Plan plan;
 };
 
-// A row's scale as two bf16 pairs: s = head + tail to 16 bits (both truncated).
-struct Scale2 {
-  __nv_bfloat162 head, tail;
-};
-
-__device__ __forceinline__ __nv_bfloat162 both_halves(float v) {  // v's upper 16 bits, twice
-  const uint32_t b = __byte_perm(__float_as_uint(v), 0u, 0x3232);
-  return *reinterpret_cast<const __nv_bfloat162*>(&b);
-}
-
-__device__ __forceinline__ Scale2 split_scale(float s) {
-  const float head = __uint_as_float(__float_as_uint(s) & 0xffff0000u);
-  return {both_halves(s), both_halves(s - head)};
-}
-
-// The two int8 in bits 0..7 and 16..23 of w, times the scale, as two bf16 (packed conversions
-// from fp32 run at a fraction of this rate). 0x4300 is 128 in bf16, with one as its last place:
-// or-ing the low seven bits gives 128 + low7, or-ing the sign bit 128 or 256, and the difference
-// is the int8, exactly. q * tail is rounded at 2^-8 of a number 2^-8 of the result, then one fused
-// multiply-add rounds the result, so it is q * s rounded to bf16 to within 2^-16; zero stays zero.
-__device__ __forceinline__ uint32_t scale_pair(uint32_t w, const Scale2& s) {
-  const uint32_t a = (w & 0x007f007fu) | 0x43004300u;
-  const uint32_t b = (w & 0x00800080u) | 0x43004300u;
-  const __nv_bfloat162 q = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a),
-                                   *reinterpret_cast<const __nv_bfloat162*>(&b));
-  const __nv_bfloat162 x = __hfma2(q, s.head, __hmul2(q, s.tail));
-  return *reinterpret_cast<const uint32_t*>(&x);
-}
-
-// Eight int8 (two words) times s, as one 16-byte piece of bf16. The middle two of each four trade
-// places (the pairs are bytes 0, 2 and 1, 3 of a word); the epilogue trades them back, where it
-// costs nothing.
-__device__ __forceinline__ uint4 scale8(uint32_t w0, uint32_t w1, const Scale2& s) {
-  return make_uint4(scale_pair(w0, s), scale_pair(w0 >> 8, s), scale_pair(w1, s), scale_pair(w1 >> 8, s));
-}
-
-__device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
-  return v;
-}
-
-__device__ __forceinline__ void st_shared_v4(uint32_t addr, const uint4& v) {
-  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
-}
-
-// One warp's part in widening a K block: 16 of the block's 64 rows, four at a time. Lane = 8 * row + u
-// reads the 16 int8 of unit u of its row and writes two 16-byte pieces of the swizzled bf16 tile:
-// chunk u / 4 (64 columns), pieces 2u and 2u + 1 of 8, at position piece ^ (row mod 8). Units 4..7
-// write their odd piece first, so that the eight lanes of a row touch all banks once.
-struct Widener {
-  int r0;             // the lane's rows are r0, r0 + 4, ...
-  uint32_t from, to;  // of the lane's first unit and piece's line in the raw block and the tile
-  uint32_t at;        // rows r0, r0 + 4, ...: the row modulo 8 alternates between lane / 8 and that plus 4
-  bool swap;
-
-  __device__ __forceinline__ Widener(int warp, int lane) {
-    const int u = lane & 7;
-    r0 = warp * 16 + (lane >> 3);
-    swap = u >= 4;
-    from = static_cast<uint32_t>(r0 * HN + u * 16);
-    const uint32_t piece = static_cast<uint32_t>(((2 * u) & 7) | (swap ? 1 : 0));
-    to = static_cast<uint32_t>((u >> 2) * MN_CHUNK_BYTES + r0 * 128);
-    at = (piece ^ static_cast<uint32_t>(lane >> 3)) << 4;
-  }
-  __device__ __forceinline__ void load(uint32_t raw, uint4 (&w)[4]) const {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) w[j] = ld_shared_v4(raw + from + j * (4 * HN));
-  }
-  __device__ __forceinline__ void convert(const uint4& w, float scale, uint4* o) const {
-    const Scale2 sc = split_scale(scale);
-    o[0] = scale8(swap ? w.z : w.x, swap ? w.w : w.y, sc);
-    o[1] = scale8(swap ? w.x : w.z, swap ? w.y : w.w, sc);
-  }
-  __device__ __forceinline__ void store(uint32_t tile, const uint4 (&o)[8]) const {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      st_shared_v4(tile + to + (at ^ ((j & 1) ? 64u : 0u)) + j * 512, o[2 * j]);
-      st_shared_v4(tile + to + (at ^ 16u ^ ((j & 1) ? 64u : 0u)) + j * 512, o[2 * j + 1]);
-    }
-  }
-};
-
-// Counts an arrival on a barrier of the leader CTA. The writes it publishes were made visible to
-// the async proxy, which alone reads them, by the writers' proxy fences; a release at cluster
-// scope stalled the warp for a round trip to memory (16384 x 4096 x 4096: 743 us, 527 without).
-__device__ __forceinline__ void arrive_leader(uint64_t* bar) {
-  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(mapa_shared(smem_u32(bar), 0u)) : "memory");
-}
-
-template <bool RAW>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Ring<RAW>::kThreads, 1)
-    dw_kernel(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CUtensorMap tmx, const Params p) {
-  constexpr int A_STAGES = Ring<RAW>::kA, B_STAGES = Ring<RAW>::kB, RAW_STAGES = Ring<RAW>::kRaw;
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+    dw_kernel(const __grid_constant__ CUtensorMap tmz, const __grid_constant__ CUtensorMap tmx, const Params p) {
+  __shared__ float4 s_back[kEpiWarps][8];  // each warp's own: of the 32 rows it works on
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
-  uint8_t* sA = smem;
-  uint8_t* sB = sA + A_STAGES * A_STAGE_BYTES;
-  uint8_t* sRaw = sB + B_STAGES * B_STAGE_BYTES;
-  uint64_t* a_full = reinterpret_cast<uint64_t*>(smem + Ring<RAW>::kBytes);  // loads of both CTAs (the leader's is used)
-  uint64_t* a_empty = a_full + A_STAGES;
-  uint64_t* b_full = a_empty + A_STAGES;      // RAW: widened, in both CTAs (the leader's is used)
-  uint64_t* b_empty = b_full + B_STAGES;
-  uint64_t* raw_full = b_empty + B_STAGES;    // this CTA's int8 block landed
-  uint64_t* raw_empty = raw_full + RAW_STAGES;
-  uint64_t* acc_full = raw_empty + RAW_STAGES;
+  uint8_t* sZ = smem;
+  uint8_t* sX = smem + STAGES * A_STAGE_BYTES;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE_BYTES);  // loads of both CTAs (the leader's is used)
+  uint64_t* empty = full + STAGES;
+  uint64_t* acc_full = empty + STAGES;
   uint64_t* acc_empty = acc_full + 2;
   uint64_t* drain = acc_empty + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
@@ -193,17 +88,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Ring<RAW>::kThreads,
   const int items = item_count(p.plan);
 
   if (warp == 0 && lane == 0) {
-    for (int s = 0; s < A_STAGES; ++s) {
-      mbar_init(&a_full[s], 1);
-      mbar_init(&a_empty[s], 1);
-    }
-    for (int s = 0; s < B_STAGES; ++s) {
-      mbar_init(&b_full[s], 2 * kConvWarps);
-      mbar_init(&b_empty[s], 1);
-    }
-    for (int s = 0; s < RAW_STAGES; ++s) {
-      mbar_init(&raw_full[s], 1);
-      mbar_init(&raw_empty[s], kConvWarps);
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&acc_full[a], 1);
@@ -211,7 +98,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Ring<RAW>::kThreads,
     }
     mbar_init(drain, 1);
     fence_mbarrier_init();
-    tma_prefetch_desc(&tma);
+    tma_prefetch_desc(&tmz);
     tma_prefetch_desc(&tmx);
   }
   if (warp == 1) {
@@ -234,65 +121,39 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Ring<RAW>::kThreads,
       for (int i = cluster; ok && i < items; i += num_clusters) {
         const Item it = item_at(p.plan, i, blocks);
         const int n0 = (it.tile / k_tiles) * TM + static_cast<int>(rank) * HM;
-        [[maybe_unused]] const int k0 = (it.tile % k_tiles) * TN + static_cast<int>(rank) * HN;
-        for (int kb = it.kb0; kb < it.kb1; ++kb) {
-          if (!mbar_wait(&a_empty[s], ph ^ 1u, kFaultWaitEmpty)) { ok = false; break; }
-          if (leader) mbar_arrive_expect_tx(&a_full[s], 2u * (A_STAGE_BYTES + (RAW ? 0u : B_STAGE_BYTES)));
-          const uint32_t bar_leader = mapa_shared(smem_u32(&a_full[s]), 0u);
-          uint8_t* sa = sA + s * A_STAGE_BYTES;
-#pragma unroll
-          for (int j = 0; j < HM / 64; ++j)
-            tma_load_2d_pair(sa + j * MN_CHUNK_BYTES, &tma, bar_leader, n0 + 64 * j, kb * BK);
-          if constexpr (!RAW) {
-            uint8_t* sb = sB + s * B_STAGE_BYTES;
-#pragma unroll
-            for (int j = 0; j < HN / 64; ++j)
-              tma_load_2d_pair(sb + j * MN_CHUNK_BYTES, &tmx, bar_leader, k0 + 64 * j, kb * BK);
-          }
-          armed |= 1u << s;
-          armed_par = (armed_par & ~(1u << s)) | (ph << s);
-          if (++s == A_STAGES) { s = 0; ph ^= 1u; }
-        }
-      }
-      if (!ok || fault_raised()) {
-        if (leader) {
-          for (int t = 0; t < A_STAGES; ++t)
-            if (armed & (1u << t)) gemm::drain_wait(&a_full[t], (armed_par >> t) & 1u);
-        }
-        gemm2::settle_inflight_copies();
-      }
-    }
-    __syncwarp();
-  } else if (RAW && warp == kRawWarp) {
-    // ------------------------------------------------------------ TMA producer of the int8 blocks
-    if constexpr (RAW) if (lane == 0) {
-      int s = 0;
-      uint32_t ph = 0, armed = 0u, armed_par = 0u;
-      bool ok = true;
-      for (int i = cluster; ok && i < items; i += num_clusters) {
-        const Item it = item_at(p.plan, i, blocks);
         const int k0 = (it.tile % k_tiles) * TN + static_cast<int>(rank) * HN;
         for (int kb = it.kb0; kb < it.kb1; ++kb) {
-          if (!mbar_wait(&raw_empty[s], ph ^ 1u, kFaultWaitEmpty)) { ok = false; break; }
-          mbar_arrive_expect_tx(&raw_full[s], RAW_BYTES);
-          tma_load_2d(sRaw + s * RAW_BYTES, &tmx, &raw_full[s], k0, kb * BK);
+          if (!mbar_wait(&empty[s], ph ^ 1u, kFaultWaitEmpty)) { ok = false; break; }
+          if (leader) mbar_arrive_expect_tx(&full[s], 2u * STAGE_BYTES);
+          const uint32_t bar_leader = mapa_shared(smem_u32(&full[s]), 0u);
+          uint8_t* sz = sZ + s * A_STAGE_BYTES;
+          uint8_t* sx = sX + s * B_STAGE_BYTES;
+#pragma unroll
+          for (int j = 0; j < HM / 64; ++j)
+            tma_load_2d_pair(sz + j * MN_CHUNK_BYTES, &tmz, bar_leader, n0 + 64 * j, kb * BK);
+#pragma unroll
+          for (int j = 0; j < HN / 64; ++j)
+            tma_load_2d_pair(sx + j * MN_CHUNK_BYTES, &tmx, bar_leader, k0 + 64 * j, kb * BK);
           armed |= 1u << s;
           armed_par = (armed_par & ~(1u << s)) | (ph << s);
-          if (++s == RAW_STAGES) { s = 0; ph ^= 1u; }
+          if (++s == STAGES) { s = 0; ph ^= 1u; }
         }
       }
-      if (!ok || fault_raised()) {
-        for (int t = 0; t < RAW_STAGES; ++t)
-          if (armed & (1u << t)) gemm::drain_wait(&raw_full[t], (armed_par >> t) & 1u);
+      // No copy outlives the CTA, also where the MMA issuer gave up on a late one after this lane was done
+      // (the leader's barriers count both CTAs' copies, and the pair leaves together).
+      if (leader) {
+        for (int t = 0; t < STAGES; ++t)
+          if (armed & (1u << t)) gemm::drain_wait(&full[t], (armed_par >> t) & 1u);
       }
+      if (!ok) gemm2::settle_inflight_copies();
     }
     __syncwarp();
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer (leader only)
     if (leader && lane == 0) {
-      constexpr uint32_t IDESC = make_idesc_bf16_f32(TM, TN, true, true);
-      int sa = 0, sb = 0;
-      uint32_t pa = 0, pb = 0, acc = 0, acc_ph = 0;
+      constexpr uint32_t IDESC = make_idesc_f16_f32(TM, TN, true, true);
+      int s = 0;
+      uint32_t ph = 0, acc = 0, acc_ph = 0;
       bool ok = true;
       for (int i = cluster; ok && i < items; i += num_clusters) {
         const Item it = item_at(p.plan, i, blocks);
@@ -300,23 +161,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Ring<RAW>::kThreads,
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + acc * TN;
         for (int kb = it.kb0; kb < it.kb1; ++kb) {
-          if (!mbar_wait(&a_full[sa], pa, kFaultWaitFull) ||
-              (RAW && !mbar_wait(&b_full[sb], pb, kFaultWaitFull))) {
-            ok = false;
-            break;
-          }
+          if (!mbar_wait(&full[s], ph, kFaultWaitFull)) { ok = false; break; }
           tc_fence_after();
-          const uint32_t a_addr = smem_u32(sA + sa * A_STAGE_BYTES);
-          const uint32_t b_addr = smem_u32(sB + sb * B_STAGE_BYTES);
+          const uint32_t z_addr = smem_u32(sZ + s * A_STAGE_BYTES);
+          const uint32_t x_addr = smem_u32(sX + s * B_STAGE_BYTES);
 #pragma unroll
           for (int kk = 0; kk < BK / UMMA_K; ++kk)
-            umma_f16_ss_pair(d_tmem, make_sw128_desc(b_addr + kk * UMMA_K * 128, MN_CHUNK_BYTES, 1024),
-                             make_sw128_desc(a_addr + kk * UMMA_K * 128, MN_CHUNK_BYTES, 1024), IDESC,
+            umma_f16_ss_pair(d_tmem, make_sw128_desc(x_addr + kk * UMMA_K * 128, MN_CHUNK_BYTES, 1024),
+                             make_sw128_desc(z_addr + kk * UMMA_K * 128, MN_CHUNK_BYTES, 1024), IDESC,
                              (kb != it.kb0 || kk != 0) ? 1u : 0u);
-          if constexpr (RAW) umma_commit_pair_mc(&b_empty[sb], kPairMask);
-          umma_commit_pair_mc(&a_empty[sa], kPairMask);
-          if (++sa == A_STAGES) { sa = 0; pa ^= 1u; }
-          if (++sb == B_STAGES) { sb = 0; pb ^= 1u; }
+          umma_commit_pair_mc(&empty[s], kPairMask);
+          if (++s == STAGES) { s = 0; ph ^= 1u; }
         }
         if (!ok) break;
         umma_commit_pair_mc(&acc_full[acc], kPairMask);
@@ -327,18 +182,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Ring<RAW>::kThreads,
       gemm::drain_wait(drain, 0u);
     }
     __syncwarp();
-  } else if (warp < 2 + kEpiWarps) {
+  } else {
     // ------------------------------------------------------------ epilogue (warps 2..9)
     const uint32_t q = warp & 3u;
     const int c_lo = static_cast<int>((warp - 2u) >> 2) * (TM / 2);  // this warp's half of the rows of dW
-    // the column within the CTA's 128: RAW tiles hold the middle two of each four swapped (scale8)
-    const uint32_t l = RAW && ((lane + 1u) & 2u) ? lane ^ 3u : lane;
-    const int in_tile = static_cast<int>(rank) * HN + static_cast<int>(q * 32u + l);
+    const int in_tile = static_cast<int>(rank) * HN + static_cast<int>(q * 32u + lane);
+    float4* back = s_back[warp - 2u];
     uint32_t acc = 0, acc_ph = 0;
     for (int i = cluster; i < items; i += num_clusters) {
       const Item it = item_at(p.plan, i, blocks);
       const int n0 = (it.tile / k_tiles) * TM + c_lo;
       const int k = (it.tile % k_tiles) * TN + in_tile;
+      // asked for while the MMAs run: in the loop below each would be waited for
+      const int at = n0 + 4 * static_cast<int>(lane);
+      const float4 mine = at < p.N ? __ldg(reinterpret_cast<const float4*>(p.back + at)) : make_float4(0.f, 0.f, 0.f, 0.f);
       if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[acc], acc_ph, kFaultWaitAccFull))) break;
       tc_fence_after();
       const uint32_t t_row = tmem_base + ((q * 32u) << 16) + acc * TM + static_cast<uint32_t>(c_lo);
@@ -348,14 +205,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Ring<RAW>::kThreads,
         if (rows <= 0) break;
         uint32_t r[32];
         __syncwarp();  // lanes past the last column skip the stores
+        if (static_cast<int>(lane >> 3) == c / 32) back[lane & 7u] = mine;
         tmem_ld_32x32b_x32(t_row + c, r);
         tmem_wait_ld();
+        __syncwarp();
         if (k >= p.K) continue;
         if (it.slot < 0) {
           __nv_bfloat16* out = p.out + static_cast<int64_t>(n0 + c) * p.ldo + k;
 #pragma unroll
-          for (int j = 0; j < 32; ++j, out += p.ldo)
-            if (j < rows) *out = __float2bfloat16_rn(__uint_as_float(r[j]));
+          for (int j = 0; j < 32; j += 4) {
+            const float4 f = back[j / 4];
+            const float v[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+            for (int i4 = 0; i4 < 4; ++i4, out += p.ldo)
+              if (j + i4 < rows) *out = __float2bfloat16_rn(__uint_as_float(r[j + i4]) * v[i4]);
+          }
         } else {
           float* part = p.partial + static_cast<size_t>(it.slot) * (TM * TN) + (c_lo + c) * TN + in_tile;
 #pragma unroll
@@ -365,53 +229,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Ring<RAW>::kThreads,
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) arrive_leader(&acc_empty[acc]);
+      if (lane == 0) mbar_arrive_leader(&acc_empty[acc]);
       acc ^= 1u;
       if (acc == 0u) acc_ph ^= 1u;
-    }
-  } else if constexpr (RAW) {
-    // ------------------------------------------------------------ converters (warps 10..17)
-    const int cw = static_cast<int>(warp) - 2 - kEpiWarps;
-    const int group = cw / kConvWarps;
-    const Widener widen(cw % kConvWarps, static_cast<int>(lane));
-    int turn = 0;  // K blocks of earlier items, modulo the groups
-    uint32_t sr = group, sb = group, pr = 0, pb = 0;
-    bool ok = true;
-    for (int i = cluster; ok && i < items; i += num_clusters) {
-      const Item it = item_at(p.plan, i, blocks);
-      const int first = it.kb0 + (group - turn + kConvGroups) % kConvGroups;
-      turn = (turn + it.kb1 - it.kb0) % kConvGroups;
-      float next[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int m = first * BK + widen.r0 + 4 * j;
-        next[j] = m < p.M ? __ldg(p.scale + m) : 0.f;
-      }
-      for (int kb = first; kb < it.kb1; kb += kConvGroups) {
-        ok = __all_sync(0xffffffffu, mbar_wait(&raw_full[sr], pr, kFaultWaitFull));
-        if (!ok) break;
-        uint4 w[4], o[8];
-        widen.load(smem_u32(sRaw) + sr * RAW_BYTES, w);
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&raw_empty[sr]);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          widen.convert(w[j], next[j], &o[2 * j]);
-          const int m = (kb + kConvGroups) * BK + widen.r0 + 4 * j;
-          next[j] = m < p.M ? __ldg(p.scale + m) : 0.f;
-        }
-        // only now: the conversion runs while the MMAs still read the stage's last tile
-        ok = __all_sync(0xffffffffu, mbar_wait(&b_empty[sb], pb ^ 1u, kFaultWaitEmpty));
-        if (!ok) break;
-        widen.store(smem_u32(sB) + sb * B_STAGE_BYTES, o);
-        fence_proxy_async_shared();  // the MMA reads the tile through the async proxy
-        __syncwarp();
-        if (lane == 0) arrive_leader(&b_full[sb]);
-        sr += kConvGroups;
-        if (sr >= RAW_STAGES) { sr -= RAW_STAGES; pr ^= 1u; }
-        sb += kConvGroups;
-        if (sb >= B_STAGES) { sb -= B_STAGES; pb ^= 1u; }
-      }
     }
   }
 
@@ -423,54 +243,236 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Ring<RAW>::kThreads,
   }
 }
 
-// X in bf16: out[m][k] = bf16(q * scale), rows of `ldo` elements (a multiple of 8, columns past K
-// zero). A warp takes rows, a lane eight columns at a time (so that a warp's stores are one run of
-// 512 bytes), eight loads ahead of their use.
-constexpr int kWidenWarps = 8;
-constexpr int kWidenAhead = 8;
+// ---------------------------------------------------------------- fp16 operands
+// dZ is walked in items of 64 columns (a 128-byte line of a row: eight lanes, 16 bytes each) by a band of
+// rows; bands are few, so that their column maxima are soon put together again.
+constexpr int kPrepThreads = 256;
+constexpr int kMaxBands = 32;
+constexpr int kPrepRows = kPrepThreads / 8;  // rows of an item that a block has at a time
 
-__global__ void __launch_bounds__(32 * kWidenWarps)
-    widen_kernel(const int8_t* __restrict__ q, int64_t ldq, const float* __restrict__ scale,
-                 __nv_bfloat16* __restrict__ out, int64_t ldo, int M, int K) {
+struct Prep {
+  const __nv_bfloat16* dz;
+  const int8_t* q;
+  const float* scale;
+  float* top;     // [bands][tiles * 64]
+  float* back;    // [tiles * 64]
+  __half* z16;    // [M][ldz]
+  __half* x16;    // [M][ldx16]
+  int64_t lddz, ldq, ldz, ldx16;
+  int32_t M, N, K;
+  int32_t tiles, bands, band_rows;
+};
+
+// Eight columns of a row of dZ from column n on, zeros past N.
+__device__ __forceinline__ uint4 load_ragged_dz(const Prep& p, int64_t m, int n) {
+  const __nv_bfloat16* at = p.dz + m * p.lddz + n;
+  uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (n + j < p.N) w[j / 2] |= static_cast<uint32_t>(__ldg(reinterpret_cast<const unsigned short*>(at) + j)) << (16 * (j & 1));
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// f(row, dZ's eight columns from n on, scale) for the thread's rows of a band, eight loads ahead of their use.
+template <class F>
+__device__ __forceinline__ void for_rows(const Prep& p, int64_t m0, int64_t m1, int n, F f) {
+  constexpr int A = 8;
+  int64_t m = m0;
+  if (n + 8 <= p.N) {
+    for (; m + (A - 1) * kPrepRows < m1; m += A * kPrepRows) {
+      uint4 w[A];
+      float s[A];
+#pragma unroll
+      for (int a = 0; a < A; ++a) {
+        w[a] = __ldg(reinterpret_cast<const uint4*>(p.dz + (m + a * kPrepRows) * p.lddz + n));
+        s[a] = __ldg(p.scale + m + a * kPrepRows);
+      }
+#pragma unroll
+      for (int a = 0; a < A; ++a) f(m + a * kPrepRows, w[a], s[a]);
+    }
+#pragma unroll 4
+    for (; m < m1; m += kPrepRows)
+      f(m, __ldg(reinterpret_cast<const uint4*>(p.dz + m * p.lddz + n)), __ldg(p.scale + m));
+  } else {
+    for (; m < m1; m += kPrepRows) f(m, load_ragged_dz(p, m, n), __ldg(p.scale + m));
+  }
+}
+
+// dZ * scale, the product that both kernels take.
+__device__ __forceinline__ void scaled8(const uint4& w, float s, float2 (&v)[4]) {
+  const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    v[j] = mul2(make_float2(__uint_as_float(x[j] << 16), __uint_as_float(x[j] & 0xffff0000u)), make_float2(s, s));
+}
+
+// The larger magnitude; a NaN counts for nothing.
+__device__ __forceinline__ float larger(float top, float v) { return fmaxf(top, fabsf(v)); }
+__device__ __forceinline__ float larger_finite(float top, float v) {
+  return fabsf(v) < __builtin_huge_valf() ? larger(top, v) : top;
+}
+
+__global__ void __launch_bounds__(kPrepThreads) column_top_kernel(const Prep p) {
+  __shared__ float s_top[kPrepThreads / 32][64];
   pdl_wait();
   pdl_launch_dependents();
-  const int units = static_cast<int>(ldo / 8), whole = K / 8;
-  const int lane = threadIdx.x & 31;
-  const int64_t warps = static_cast<int64_t>(gridDim.x) * kWidenWarps;
-  for (int64_t m = static_cast<int64_t>(blockIdx.x) * kWidenWarps + (threadIdx.x >> 5); m < M; m += warps) {
-    const float s = __ldg(scale + m);
-    const int8_t* from = q + m * ldq;
-    uint4* to = reinterpret_cast<uint4*>(out + m * ldo);
-    for (int u0 = lane; u0 < units; u0 += 32 * kWidenAhead) {
-      uint2 w[kWidenAhead];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int piece = lane & 7;
+  for (int item = blockIdx.x; item < p.tiles * p.bands; item += gridDim.x) {
+    const int tile = item % p.tiles, band = item / p.tiles;
+    const int n = tile * 64 + piece * 8;
+    const int64_t m1 = min(static_cast<int64_t>(p.M), static_cast<int64_t>(band + 1) * p.band_rows);
+    const int64_t m0 = static_cast<int64_t>(band) * p.band_rows + (threadIdx.x >> 3);
+    float top[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (n < p.N) {
+      const auto walk = [&](auto pick) {
+        for_rows(p, m0, m1, n, [&](int64_t, const uint4& w, float s) {
+          float2 v[4];
+          scaled8(w, s, v);
 #pragma unroll
-      for (int i = 0; i < kWidenAhead; ++i) {
-        const int u = u0 + 32 * i;
-        w[i] = make_uint2(0u, 0u);
-        if (u < whole) {
-          w[i] = __ldcs(reinterpret_cast<const uint2*>(from) + u);
-        } else if (u < units) {
-          uint32_t x[2] = {0u, 0u};
+          for (int j = 0; j < 4; ++j) {
+            top[2 * j] = pick(top[2 * j], v[j].x);
+            top[2 * j + 1] = pick(top[2 * j + 1], v[j].y);
+          }
+        });
+      };
+      walk([](float t, float v) { return larger(t, v); });
+      bool infinite = false;
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (u * 8 + j < K) x[j / 4] |= static_cast<uint32_t>(static_cast<uint8_t>(from[u * 8 + j])) << (8 * (j % 4));
-          w[i] = make_uint2(x[0], x[1]);
-        }
-      }
+      for (int j = 0; j < 8; ++j) infinite = infinite || top[j] == __builtin_huge_valf();
+      if (infinite) {  // again without what is infinite
 #pragma unroll
-      for (int i = 0; i < kWidenAhead; ++i) {
-        const int u = u0 + 32 * i;
-        if (u >= units) break;
-        uint32_t o[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t v = (j < 2 ? w[i].x : w[i].y) >> (16 * (j % 2));
-          o[j] = pack_bf16x2(static_cast<float>(static_cast<int8_t>(v)) * s,
-                             static_cast<float>(static_cast<int8_t>(v >> 8)) * s);
-        }
-        to[u] = make_uint4(o[0], o[1], o[2], o[3]);
+        for (int j = 0; j < 8; ++j) top[j] = 0.f;
+        walk([](float t, float v) { return larger_finite(t, v); });
       }
     }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      top[j] = fmaxf(top[j], __shfl_xor_sync(0xffffffffu, top[j], 8));
+      top[j] = fmaxf(top[j], __shfl_xor_sync(0xffffffffu, top[j], 16));
+    }
+    if (lane < 8) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s_top[warp][piece * 8 + j] = top[j];
+    }
+    __syncthreads();
+    if (threadIdx.x < 64) {
+      float t = 0.f;
+#pragma unroll
+      for (int w = 0; w < kPrepThreads / 32; ++w) t = fmaxf(t, s_top[w][threadIdx.x]);
+      p.top[(static_cast<int64_t>(band) * p.tiles + tile) * 64 + threadIdx.x] = t;
+    }
+    __syncthreads();
+  }
+}
+
+// Four int8 in fp16, exactly: 0x6400 is 1024 with one as its last place, so or-ing q + 128 gives
+// 1152 + q.
+__device__ __forceinline__ uint2 widen4(uint32_t w) {
+  const uint32_t u = w ^ 0x80808080u;
+  uint32_t v[2] = {__byte_perm(u, 0x64646464u, 0x4140), __byte_perm(u, 0x64646464u, 0x4342)};
+  const __half2 bias = __float2half2_rn(1152.f);
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&v[j]), bias);
+    v[j] = *reinterpret_cast<const uint32_t*>(&x);
+  }
+  return make_uint2(v[0], v[1]);
+}
+
+constexpr int kWidenAhead = 8;
+
+// Row m of X in fp16 (columns past K zero): a lane has eight columns at a time, so that a warp's stores
+// are one run of 512 bytes, eight loads ahead of their use.
+__device__ __forceinline__ void widen_row(const Prep& p, int64_t m, int lane) {
+  const int units = static_cast<int>(p.ldx16 / 8), whole = p.K / 8;
+  const int8_t* from = p.q + m * p.ldq;
+  uint4* to = reinterpret_cast<uint4*>(p.x16 + m * p.ldx16);
+  for (int u0 = lane; u0 < units; u0 += 32 * kWidenAhead) {
+    uint2 w[kWidenAhead];
+#pragma unroll
+    for (int i = 0; i < kWidenAhead; ++i) {
+      const int u = u0 + 32 * i;
+      w[i] = make_uint2(0u, 0u);
+      if (u < whole) {
+        w[i] = __ldcs(reinterpret_cast<const uint2*>(from) + u);
+      } else if (u < units) {
+        uint32_t x[2] = {0u, 0u};
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (u * 8 + j < p.K) x[j / 4] |= static_cast<uint32_t>(static_cast<uint8_t>(from[u * 8 + j])) << (8 * (j % 4));
+        w[i] = make_uint2(x[0], x[1]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kWidenAhead; ++i) {
+      const int u = u0 + 32 * i;
+      if (u >= units) break;
+      const uint2 a = widen4(w[i].x), b = widen4(w[i].y);
+      to[u] = make_uint4(a.x, a.y, b.x, b.y);
+    }
+  }
+}
+
+// Both operands, as one list of items: first dZ's (from its end: the last that column_top_kernel read are
+// still in L2), then X's rows, one a warp.
+constexpr int kWidenRows = kPrepThreads / 32;
+
+__global__ void __launch_bounds__(kPrepThreads) operands_kernel(const Prep p) {
+  __shared__ float s_top[kPrepThreads / 64][64];
+  __shared__ __align__(16) float s_up[64];
+  pdl_wait();
+  pdl_launch_dependents();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int dz_items = p.tiles * p.bands;
+  const int items = dz_items + static_cast<int>((static_cast<int64_t>(p.M) + kWidenRows - 1) / kWidenRows);
+  for (int item = blockIdx.x; item < items; item += gridDim.x) {
+    if (item >= dz_items) {
+      const int64_t m = static_cast<int64_t>(item - dz_items) * kWidenRows + warp;
+      if (m < p.M) widen_row(p, m, lane);
+      continue;
+    }
+    const int back_item = dz_items - 1 - item;
+    const int tile = back_item % p.tiles, band = back_item / p.tiles;
+    {
+      const int c = threadIdx.x & 63;
+      float t = 0.f;
+      for (int b = threadIdx.x >> 6; b < p.bands; b += kPrepThreads / 64)
+        t = fmaxf(t, __ldcg(p.top + (static_cast<int64_t>(b) * p.tiles + tile) * 64 + c));
+      s_top[threadIdx.x >> 6][c] = t;
+      __syncthreads();
+      if (threadIdx.x < 64) {
+#pragma unroll
+        for (int i = 1; i < kPrepThreads / 64; ++i) t = fmaxf(t, s_top[i][c]);
+        // Below 2^-112 the exponent stays there, so that both powers are normal numbers; fp16's last
+        // place is then 2^-150, beneath fp32's.
+        const int e = max(static_cast<int>(__float_as_uint(t) >> 23) - 127, -112);
+        s_up[c] = __uint_as_float(static_cast<uint32_t>(14 - e + 127) << 23);
+        if (band == 0) p.back[tile * 64 + c] = __uint_as_float(static_cast<uint32_t>(e - 14 + 127) << 23);
+      }
+      __syncthreads();
+    }
+    const int piece = lane & 7, n = tile * 64 + piece * 8;
+    const int64_t m1 = min(static_cast<int64_t>(p.M), static_cast<int64_t>(band + 1) * p.band_rows);
+    if (n < p.N) {
+      float2 up[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) up[j] = *reinterpret_cast<const float2*>(&s_up[piece * 8 + 2 * j]);
+      for_rows(p, static_cast<int64_t>(band) * p.band_rows + (threadIdx.x >> 3), m1, n,
+               [&](int64_t m, const uint4& w, float s) {
+                 float2 v[4];
+                 scaled8(w, s, v);
+                 uint32_t o[4];
+#pragma unroll
+                 for (int j = 0; j < 4; ++j) {
+                   const float2 x = mul2(v[j], up[j]);
+                   const __half2 h = __floats2half2_rn(x.x, x.y);
+                   o[j] = *reinterpret_cast<const uint32_t*>(&h);
+                 }
+                 *reinterpret_cast<uint4*>(p.z16 + m * p.ldz + n) = make_uint4(o[0], o[1], o[2], o[3]);
+               });
+    }
+    __syncthreads();  // the next item's maxima go to the same place
   }
 }
 
@@ -498,7 +500,7 @@ __global__ void __launch_bounds__(TN) add_pieces_kernel(const Params p) {
   __nv_bfloat16* out = p.out + static_cast<int64_t>(n0) * p.ldo + k;
 #pragma unroll
   for (int i = 0; i < kAddRows; ++i)
-    if (n0 + i < p.N) out[i * p.ldo] = __float2bfloat16_rn(sum[i]);
+    if (n0 + i < p.N) out[i * p.ldo] = __float2bfloat16_rn(sum[i] * __ldg(p.back + n0 + i));
 }
 
 }  // namespace ckpt

@@ -3,14 +3,18 @@
 // K blocks of a tile are split over a cluster, whose CTAs add their fp32 partial sums through distributed
 // shared memory, in the order of their ranks: one launch, no workspace, the same bits every time.
 //
-// A stage of the ring holds a K block's raw int8 (8 KB), the widened tile made of it (16 KB) and dZ. The
-// stage is free again when its MMAs are done, so a converter waits for nothing but the loads. What bounds
-// a long sum is the converters' arithmetic, 0.35 us a K block: rings of their own for loads and tiles
-// (0.40) and twice the converters (0.34) did not shorten it.
+// A stage of the ring holds a K block's raw int8 (8 KB), the widened tile made of it (16 KB), and dZ, which
+// the same warps replace by dZ * scale in two bf16 terms (8 KB each per 64 columns): head, the product
+// rounded to bf16, and tail, what that took from it. Their sum is the product to 2^-14 of it, at fp32's
+// range, and the MMA adds q * head and q * tail to the same accumulator; q itself is exact in bf16.
+// (One fp16 term needs the columns' largest first, i.e. two launches more.) The stage is free again when
+// its MMAs are done, so a converter waits for nothing but the loads. What bounds a long sum is the
+// converters' arithmetic.
 // Warps: 0 TMA, 1 MMA, 2..9 converters in two groups of four that take the K blocks in turn, and the
 // epilogue after them.
 #pragma once
 
+#include "ckpt_layout.h"
 #include "gemm_ckpt.cuh"
 #include "igemm.cuh"
 
@@ -18,23 +22,25 @@ namespace c3cu {
 namespace ckpt_narrow {
 
 using ckpt::BK;
-using ckpt::kConvGroups;
-using ckpt::kConvWarps;
 using ckpt::MN_CHUNK_BYTES;
-using ckpt::RAW_BYTES;
 using ckpt::UMMA_K;
-constexpr int COLS = ckpt::HN;  // columns of dW per CTA: the MMA's 128 rows
+constexpr int kConvWarps = 4;   // a group's warps
+constexpr int kConvGroups = 2;  // the groups take K blocks in turn
+constexpr int COLS = 128;       // columns of dW per CTA: the MMA's 128 rows
 constexpr int kThreads = 32 * (2 + kConvGroups * kConvWarps);
 constexpr int kMaxCluster = 8;
+constexpr uint32_t RAW_BYTES = BK * COLS;  // 64 rows (m) of 128 int8 (k)
 constexpr uint32_t WIDE_BYTES = 2 * MN_CHUNK_BYTES;
 __host__ __device__ constexpr int chunks(int T) { return (T + 63) / 64; }  // of 64 columns of dZ
+static_assert(MN_CHUNK_BYTES == ckpt::kChunkBytes && BK == 64, "ckpt_layout.h");
 
-template <int T>
+template <int T, bool READY>
 struct Ring {
-  static constexpr int kStages = T <= 64 ? 6 : 4;
-  static constexpr uint32_t kStage = WIDE_BYTES + chunks(T) * MN_CHUNK_BYTES + RAW_BYTES;
-  static constexpr uint32_t kSmem = kStages * kStage + (3 * kStages + 1) * 8 + 8 + 1024;
-  static_assert(kStages % kConvGroups == 0, "a stage belongs to one group, which so sees each of its phases");
+  static constexpr int kStages = !READY ? 4 : T <= 64 ? 8 : 6;
+  static constexpr uint32_t kZ = chunks(T) * MN_CHUNK_BYTES;  // dZ, then head; tail behind it
+  static constexpr uint32_t kStage = WIDE_BYTES + (READY ? kZ : 2 * kZ + RAW_BYTES);
+  static constexpr uint32_t kSmem = kStages * kStage + (3 * kStages + 2) * 8 + 8 + 1024;
+  static_assert(READY || kStages % kConvGroups == 0, "a stage belongs to one group, which so sees each of its phases");
   static_assert(kSmem <= 227 * 1024 && kStages * kStage >= T * COLS * 4, "shared memory");
 };
 
@@ -42,26 +48,135 @@ struct Params {
   int32_t M, N, K;  // dW is N x K, the sum runs over M
   __nv_bfloat16* out;
   int64_t ldo;
-  const float* scale;  // [M]
+  const float* scale;  // [M]; READY: 2^(e - 14) of each row of dW, padded to 64
   int32_t kb_per_cta;  // K blocks per CTA of a cluster
   int32_t k_tiles;     // tiles of 128 columns
 };
 
+__device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+
+__device__ __forceinline__ void st_shared_v4(uint32_t addr, const uint4& v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
+// dZ * scale is taken times 2^6 and q times 2^-6: what head and tail lose of a product at the bottom of
+// fp32's normal numbers then is no more than of any other (below, a product is held to 2^-138), and the
+// scale of a row of fp32's largest numbers, 2^128 / 127, times 2^6 is finite.
+constexpr float kUp = 64.f;
+
+// The two int8 in bits 0..7 and 16..23 of w times 2^-6 as two bf16, exactly. 0x4000 is 128 * 2^-6 in bf16,
+// with 2^-6 as its last place: or-ing the low seven bits gives (128 + low7) 2^-6, or-ing the sign bit
+// 128 or 256 times 2^-6, and the difference is the int8 times 2^-6.
+__device__ __forceinline__ uint32_t widen_pair(uint32_t w) {
+  const uint32_t a = (w & 0x007f007fu) | 0x40004000u;
+  const uint32_t b = (w & 0x00800080u) | 0x40004000u;
+  const __nv_bfloat162 q = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a),
+                                   *reinterpret_cast<const __nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&q);
+}
+
+// Eight int8 (two words) as one 16-byte piece of bf16. The middle two of each four trade places (the
+// pairs are bytes 0, 2 and 1, 3 of a word); the epilogue trades them back, where it costs nothing.
+__device__ __forceinline__ uint4 widen8(uint32_t w0, uint32_t w1) {
+  return make_uint4(widen_pair(w0), widen_pair(w0 >> 8), widen_pair(w1), widen_pair(w1 >> 8));
+}
+
+// The raw block at `raw` into the tile at `tile`: thread t's share.
+__device__ __forceinline__ void widen_x(uint32_t raw, uint32_t tile, int t) {
+  uint4 w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = ld_shared_v4(raw + ckpt::x_from(ckpt::x_unit(t, i)));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const ckpt::XUnit x = ckpt::x_unit(t, i);
+    const uint4 even = widen8(w[i].x, w[i].y), odd = widen8(w[i].z, w[i].w);
+    st_shared_v4(tile + ckpt::x_to(x, false), x.odd_first ? odd : even);
+    st_shared_v4(tile + ckpt::x_to(x, true), x.odd_first ? even : odd);
+  }
+}
+
+// A row's scale times kUp as two bf16, each twice: the sum is the scale to 2^-16 of it.
+struct Scale2 {
+  __nv_bfloat162 head, tail;
+};
+
+__device__ __forceinline__ Scale2 split_scale(float s) {
+  const float up = __fmul_rn(s, kUp);
+  const __nv_bfloat16 head = __float2bfloat16_rn(up);
+  return {__bfloat162bfloat162(head), __bfloat162bfloat162(__float2bfloat16_rn(__fsub_rn(up, __bfloat162float(head))))};
+}
+
+// Two bf16 (w) times s, as head and tail: head is the product with the scale's head, rounded; a fused
+// multiply-add gives what that rounding took, exactly (16 bits less their upper 8), and a second one adds
+// the product with the scale's tail. |tail| <= 2^-7 of the product, so its one rounding and the scale's
+// are 2^-15 + 2^-16 of it in all.
+__device__ __forceinline__ void split_pair(uint32_t w, const Scale2& s, uint32_t& head, uint32_t& tail) {
+  const __nv_bfloat162 z = *reinterpret_cast<const __nv_bfloat162*>(&w);
+  const __nv_bfloat162 h = __hmul2_rn(z, s.head);
+  const __nv_bfloat162 t = __hfma2(z, s.tail, __hfma2(z, s.head, __hneg2(h)));
+  head = *reinterpret_cast<const uint32_t*>(&h);
+  tail = *reinterpret_cast<const uint32_t*>(&t);
+}
+
+// What is infinite has no tail (infinity less infinity); NaN is NaN in the head.
+__device__ __noinline__ uint32_t finite_pair(uint32_t tail) {
+  if ((tail & 0x7f80u) == 0x7f80u) tail &= 0xffff0000u;
+  if ((tail & 0x7f800000u) == 0x7f800000u) tail &= 0xffffu;
+  return tail;
+}
+
+__device__ __forceinline__ void split8(const uint4& w, const Scale2& s, uint4& h, uint4& l) {
+  split_pair(w.x, s, h.x, l.x);
+  split_pair(w.y, s, h.y, l.y);
+  split_pair(w.z, s, h.z, l.z);
+  split_pair(w.w, s, h.w, l.w);
+  const uint32_t any = l.x | l.y | l.z | l.w;  // all ones in an exponent here: perhaps in one of the tails
+  if ((any & 0x7f80u) == 0x7f80u || (any & 0x7f800000u) == 0x7f800000u)
+    l = make_uint4(finite_pair(l.x), finite_pair(l.y), finite_pair(l.z), finite_pair(l.w));
+}
+
+// dZ's chunks at `z` become heads, their tails go `tail` bytes behind them: thread t's share. scale[i] is
+// that of the thread's i-th row.
 template <int T>
+__device__ __forceinline__ void split_dz(uint32_t z, uint32_t tail, int t, const float (&scale)[ckpt::DzUnits<T>::kRows]) {
+  using U = ckpt::DzUnits<T>;
+#pragma unroll
+  for (int c = 0; c < U::kChunks; ++c) {
+    uint4 w[U::kRows];
+#pragma unroll
+    for (int i = 0; i < U::kRows; ++i)
+      w[i] = ld_shared_v4(z + c * ckpt::kChunkBytes + ckpt::piece_at(U::row(t, i), U::piece(t)));
+#pragma unroll
+    for (int i = 0; i < U::kRows; ++i) {
+      const uint32_t at = z + c * ckpt::kChunkBytes + ckpt::piece_at(U::row(t, i), U::piece(t));
+      uint4 h, l;
+      split8(w[i], split_scale(scale[i]), h, l);
+      st_shared_v4(at, h);
+      st_shared_v4(at + tail, l);
+    }
+  }
+}
+
+template <int T, bool READY>
 __global__ void __launch_bounds__(kThreads)
     dw_narrow_kernel(const __grid_constant__ CUtensorMap tmz, const __grid_constant__ CUtensorMap tmx, const Params p) {
-  constexpr int STAGES = Ring<T>::kStages;
-  constexpr uint32_t STAGE = Ring<T>::kStage;
-  constexpr uint32_t Z_AT = WIDE_BYTES, RAW_AT = Z_AT + chunks(T) * MN_CHUNK_BYTES;
-  constexpr uint32_t TMEM = T < 32 ? 32 : T;
+  constexpr int STAGES = Ring<T, READY>::kStages;
+  constexpr uint32_t STAGE = Ring<T, READY>::kStage;
+  constexpr uint32_t Z_AT = WIDE_BYTES, TAIL = Ring<T, READY>::kZ, RAW_AT = Z_AT + 2 * TAIL;
+  __shared__ float s_back[T];  // READY
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE);  // dZ and the int8 block landed
-  uint64_t* wide = full + STAGES;                                       // widened
+  uint64_t* wide = full + STAGES;                                       // converted
   uint64_t* empty = wide + STAGES;                                      // read by the MMAs
   uint64_t* acc_full = empty + STAGES;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
+  uint64_t* drain = acc_full + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
 
   const uint32_t warp = warp_id_sync();
   const uint32_t lane = lane_id();
@@ -82,29 +197,38 @@ __global__ void __launch_bounds__(kThreads)
       mbar_init(&empty[s], 1);
     }
     mbar_init(acc_full, 1);
+    mbar_init(drain, 1);
     fence_mbarrier_init();
     tma_prefetch_desc(&tmz);
     tma_prefetch_desc(&tmx);
   }
   if (warp == 1) {
-    tmem_alloc(tmem_slot, TMEM);
+    tmem_alloc(tmem_slot, T);
     tmem_relinquish();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  if constexpr (READY) {
+    pdl_wait();
+    pdl_launch_dependents();
+  }
 
   if (warp == 0) {
     if (lane == 0) {
       int s = 0;
       uint32_t ph = 0, armed = 0u, armed_par = 0u;
-      bool ok = true;
       for (int kb = kb0; kb < kb1; ++kb) {
-        if (!mbar_wait(&empty[s], ph ^ 1u, kFaultWaitEmpty)) { ok = false; break; }
+        if (!mbar_wait(&empty[s], ph ^ 1u, kFaultWaitEmpty)) break;
         uint8_t* at = smem + s * STAGE;
-        mbar_arrive_expect_tx(&full[s], chunks(T) * MN_CHUNK_BYTES + RAW_BYTES);
-        tma_load_2d(at + RAW_AT, &tmx, &full[s], k0, kb * BK);
+        mbar_arrive_expect_tx(&full[s], chunks(T) * MN_CHUNK_BYTES + (READY ? WIDE_BYTES : RAW_BYTES));
+        if constexpr (READY) {
+          tma_load_2d(at, &tmx, &full[s], k0, kb * BK);
+          tma_load_2d(at + MN_CHUNK_BYTES, &tmx, &full[s], k0 + 64, kb * BK);
+        } else {
+          tma_load_2d(at + RAW_AT, &tmx, &full[s], k0, kb * BK);
+        }
 #pragma unroll
         for (int c = 0; c < chunks(T); ++c)
           tma_load_2d(at + Z_AT + c * MN_CHUNK_BYTES, &tmz, &full[s], n0 + 64 * c, kb * BK);
@@ -112,58 +236,69 @@ __global__ void __launch_bounds__(kThreads)
         armed_par = (armed_par & ~(1u << s)) | (ph << s);
         if (++s == STAGES) { s = 0; ph ^= 1u; }
       }
-      if (!ok || fault_raised())
-        for (int t = 0; t < STAGES; ++t)
-          if (armed & (1u << t)) gemm::drain_wait(&full[t], (armed_par >> t) & 1u);
+      // no copy outlives the CTA, also where another role gave up on a late one after this lane was done
+      for (int t = 0; t < STAGES; ++t)
+        if (armed & (1u << t)) gemm::drain_wait(&full[t], (armed_par >> t) & 1u);
     }
     __syncwarp();
   } else if (warp == 1) {
     if (lane == 0) {
-      constexpr uint32_t IDESC = make_idesc_bf16_f32(COLS, T, true, true);
+      constexpr uint32_t IDESC = READY ? make_idesc_f16_f32(COLS, T, true, true) : make_idesc_bf16_f32(COLS, T, true, true);
       int s = 0;
       uint32_t ph = 0;
+      bool ok = true;
       for (int kb = kb0; kb < kb1; ++kb) {
-        // dZ landed before the tile was widened, but that was seen by the converters, not by this thread
-        if (!mbar_wait(&full[s], ph, kFaultWaitFull) || !mbar_wait(&wide[s], ph, kFaultWaitFull)) break;
+        // dZ and the int8 block were there before they were converted, but the converters saw that, not
+        // this thread
+        ok = mbar_wait(&full[s], ph, kFaultWaitFull) && (READY || mbar_wait(&wide[s], ph, kFaultWaitFull));
+        if (!ok) break;
         tc_fence_after();
         const uint32_t x = smem_u32(smem + s * STAGE);
         const uint32_t z = x + Z_AT;
 #pragma unroll
-        for (int kk = 0; kk < BK / UMMA_K; ++kk)
-          umma_f16_ss(tmem, make_sw128_desc(x + kk * UMMA_K * 128, MN_CHUNK_BYTES, 1024),
-                      make_sw128_desc(z + kk * UMMA_K * 128, MN_CHUNK_BYTES, 1024), IDESC,
-                      (kb != kb0 || kk != 0) ? 1u : 0u);
+        for (int part = 0; part < (READY ? 1 : 2); ++part)
+#pragma unroll
+          for (int kk = 0; kk < BK / UMMA_K; ++kk)
+            umma_f16_ss(tmem, make_sw128_desc(x + kk * UMMA_K * 128, MN_CHUNK_BYTES, 1024),
+                        make_sw128_desc(z + part * TAIL + kk * UMMA_K * 128, MN_CHUNK_BYTES, 1024), IDESC,
+                        (kb != kb0 || kk != 0 || part != 0) ? 1u : 0u);
         umma_commit(&empty[s]);
         if (++s == STAGES) { s = 0; ph ^= 1u; }
       }
-      umma_commit(acc_full);  // also on a fault: completes when the MMAs issued so far have
-      gemm::drain_wait(acc_full, 0u);
+      // after a fault the epilogue is not told that the sums are there: it gives up as well
+      if (ok) umma_commit(acc_full);
+      umma_commit(drain);
+      gemm::drain_wait(drain, 0u);
     }
     __syncwarp();
+  } else if constexpr (READY) {
+    for (int t = static_cast<int>(threadIdx.x) - 64; t < T; t += kThreads - 64)
+      s_back[t] = n0 + t < p.N ? __ldg(p.scale + n0 + t) : 0.f;
   } else {
     const int group = static_cast<int>(warp - 2u) / kConvWarps;
-    const ckpt::Widener widen(static_cast<int>(warp - 2u) % kConvWarps, static_cast<int>(lane));
-    float next[4];
+    const int t = static_cast<int>((warp - 2u) % kConvWarps * 32u + lane);
+    using U = ckpt::DzUnits<T>;
+    float next[U::kRows];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int m = (kb0 + group) * BK + widen.r0 + 4 * j;
-      next[j] = m < p.M ? __ldg(p.scale + m) : 0.f;
+    for (int i = 0; i < U::kRows; ++i) {
+      const int m = (kb0 + group) * BK + U::row(t, i);
+      next[i] = m < p.M ? __ldg(p.scale + m) : 0.f;
     }
     int s = group;
     uint32_t ph = 0;
     for (int kb = kb0 + group; kb < kb1; kb += kConvGroups) {
       if (!__all_sync(0xffffffffu, mbar_wait(&full[s], ph, kFaultWaitFull))) break;
       const uint32_t at = smem_u32(smem + s * STAGE);
-      uint4 w[4], o[8];
-      widen.load(at + RAW_AT, w);
+      float scale[U::kRows];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        widen.convert(w[j], next[j], &o[2 * j]);
-        const int m = (kb + kConvGroups) * BK + widen.r0 + 4 * j;
-        next[j] = m < p.M ? __ldg(p.scale + m) : 0.f;
+      for (int i = 0; i < U::kRows; ++i) {
+        scale[i] = next[i];
+        const int m = (kb + kConvGroups) * BK + U::row(t, i);
+        next[i] = m < p.M ? __ldg(p.scale + m) : 0.f;
       }
-      widen.store(at, o);
-      fence_proxy_async_shared();  // the MMA reads the tile through the async proxy
+      widen_x(at + RAW_AT, at, t);
+      split_dz<T>(at + Z_AT, TAIL, t, scale);
+      fence_proxy_async_shared();  // the MMA reads the tiles through the async proxy
       __syncwarp();
       if (lane == 0) mbar_arrive(&wide[s]);
       s += kConvGroups;
@@ -172,9 +307,11 @@ __global__ void __launch_bounds__(kThreads)
   }
 
   // ------------------------------------------------------------ epilogue: one column per lane
+  if constexpr (READY) __syncthreads();  // s_back
+  const auto rounded = [&](float sum, int row) { return __float2bfloat16_rn(READY ? sum * s_back[row] : sum); };
   const uint32_t q = warp & 3u;               // the lane quarter of a warp
   const int half = warp >= 6 ? 1 : 0;         // the two warps of a quarter share the rows of dW
-  const uint32_t in_quarter = (lane + 1u) & 2u ? lane ^ 3u : lane;  // scale8 swapped the middle two of four
+  const uint32_t in_quarter = !READY && ((lane + 1u) & 2u) ? lane ^ 3u : lane;  // widen8 swapped the middle two of four
   const int k = k0 + static_cast<int>(q * 32 + in_quarter);
   const uint32_t t_row = tmem + ((q * 32u) << 16);
   const int rows = min(T, p.N - n0);
@@ -195,7 +332,7 @@ __global__ void __launch_bounds__(kThreads)
         if (k < p.K) {
 #pragma unroll
           for (int j = 0; j < 16; ++j)
-            if (c + j < rows) out[(c + j) * p.ldo] = __float2bfloat16_rn(__uint_as_float(r[j]));
+            if (c + j < rows) out[(c + j) * p.ldo] = rounded(__uint_as_float(r[j]), c + j);
         }
       }
       __syncwarp();
@@ -205,7 +342,7 @@ __global__ void __launch_bounds__(kThreads)
     // and each CTA adds up and stores its share of the rows.
     float* part = reinterpret_cast<float*>(smem);
     const bool any = kb0 < kb1;  // the last CTAs may have no K block: their sums are zero
-    if (warp >= 2) {
+    if (warp >= 2 && ok) {
 #pragma unroll 1
       for (int c = 16 * half; c < rows; c += 32) {
         uint32_t r[16];
@@ -235,7 +372,7 @@ __global__ void __launch_bounds__(kThreads)
         }
 #pragma unroll
         for (int j = 0; j < J; ++j)
-          if (t + j < last) out[(t + j) * p.ldo] = __float2bfloat16_rn(sum[j]);
+          if (t + j < last) out[(t + j) * p.ldo] = rounded(sum[j], t + j);
       }
     }
     __syncwarp();
@@ -246,7 +383,7 @@ __global__ void __launch_bounds__(kThreads)
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, TMEM);
+    tmem_dealloc(tmem, T);
   }
 }
 

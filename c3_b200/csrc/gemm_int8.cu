@@ -55,8 +55,8 @@ struct AtOnce {
 };
 
 int query_clusters(int split) {
-  auto kern = ckpt_narrow::dw_narrow_kernel<32>;
-  constexpr int kSmem = static_cast<int>(ckpt_narrow::Ring<32>::kSmem);
+  auto kern = ckpt_narrow::dw_narrow_kernel<32, false>;
+  constexpr int kSmem = static_cast<int>(ckpt_narrow::Ring<32, false>::kSmem);
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess) {
     cudaGetLastError();
     return 0;
@@ -96,6 +96,11 @@ AtOnce clusters_at_once() {  // asked once per device
   return r;
 }
 
+// The calling thread's choice of form (c3cu_set_int8_form): -1 none, 0 the persistent kernel, else tiles
+// of that many rows, split over clusters of g_form_split.
+thread_local int g_form_tile = -1, g_form_split = 1;
+thread_local bool g_form_ready = false;
+
 // How a forward runs: T = 0 for the pair kernel, else tiles of T tokens, each split along K over a
 // cluster of `split` CTAs.
 struct ForwardPlan {
@@ -120,9 +125,17 @@ ForwardPlan plan_forward(int64_t M, int64_t N, int64_t K) {
   const int64_t kb_pair = (K + igemm::pair::BK - 1) / igemm::pair::BK;
   const int64_t pairs = ((N + gemm2::TM - 1) / gemm2::TM) * ((M + gemm2::TN - 1) / gemm2::TN);
   ForwardPlan best{0, 1, 0, 0};
+  const int64_t kb = (K + igemm::narrow::BK - 1) / igemm::narrow::BK;
+  const auto tiled = [kb](int T, int split) {
+    const int64_t per = (kb + split - 1) / split;
+    int stages = static_cast<int>(igemm::narrow::kMaxRing / igemm::narrow::stage_bytes(T));
+    if (stages > igemm::narrow::kMaxStages) stages = igemm::narrow::kMaxStages;
+    if (stages > per) stages = static_cast<int>(per);
+    return ForwardPlan{T, split, static_cast<int>(per), stages};
+  };
+  if (g_form_tile >= 0) return g_form_tile == 0 ? best : tiled(g_form_tile, g_form_split);
   if (gemm_max_ctas() > 0) return best;  // the persistent kernel keeps to the caller's CTAs
   double least = 2.5 + waves(pairs, sms / 2) * (4.0 + 0.27 * static_cast<double>(kb_pair));
-  const int64_t kb = (K + igemm::narrow::BK - 1) / igemm::narrow::BK;
   const AtOnce at_once = clusters_at_once();
   const int64_t n_tiles = (N + igemm::narrow::BN - 1) / igemm::narrow::BN;
   for (const auto& kind : kinds) {
@@ -135,10 +148,7 @@ ForwardPlan plan_forward(int64_t M, int64_t N, int64_t K) {
       const double t = 3.2 + waves(tiles, at_once(split)) * tile;
       if (t < least) {
         least = t;
-        int stages = static_cast<int>(igemm::narrow::kMaxRing / igemm::narrow::stage_bytes(kind.T));
-        if (stages > igemm::narrow::kMaxStages) stages = igemm::narrow::kMaxStages;
-        if (stages > per) stages = static_cast<int>(per);
-        best = {kind.T, split, static_cast<int>(per), stages};
+        best = tiled(kind.T, split);
       }
     }
   }
@@ -196,6 +206,7 @@ int igemv_split(int64_t blocks, int64_t K) {
 // cores. Measured (us, igemv / narrow): one token, 4096 x 4096 5.2 / 7.3, 1397 x 777 2.4 / 4.7, 12288 x
 // 12288 26 / 34.5; two, 12288 x 4096 12.8 / 11.9; four, 4096 x 4096 7.1 / 7.7, 12288 x 4096 16 / 11.9.
 bool use_igemv(int64_t M, int64_t N, int64_t K) {
+  if (g_form_tile >= 0) return false;
   if (gemm_max_ctas() > 0) return false;  // the persistent kernel keeps to the caller's CTAs
   return M <= 2 || (M <= igemv::kMaxTokens && N * K <= 20'000'000);
 }
@@ -241,126 +252,203 @@ int check_gemm_sizes(const char* what, int64_t M, int64_t N, int64_t K) {
 }
 
 // How a weight gradient runs: in small tiles (T > 0) of T rows, each split over a cluster of `split`
-// CTAs, or in large ones: X widened in the kernel (raw) or once into the workspace, the tiles' plan,
-// and the workspace's parts (partial sums first, then the widened X).
+// CTAs, or in large ones: the operands' layout in the workspace and the tiles' plan.
 struct DwRun {
   int T, split, kb_per_cta;
-  bool raw;
+  bool ready;  // the operands are laid out in the workspace first (always for large tiles)
   int clusters;
   ckpt::Plan plan;
-  size_t partial_bytes, wide_bytes;
-  int64_t wide_ld;
+  ckpt::Prep prep;                           // sizes only
+  size_t top_at, back_at, z_at, x_at, bytes;  // the workspace's parts; partial sums first
 };
 
-template <bool RAW>
 int dw_clusters(int* clusters) {
-  auto kern = ckpt::dw_kernel<RAW>;
+  auto kern = ckpt::dw_kernel;
   static std::atomic<uint64_t> smem_set{0};
   int rc = C3CU_OK;
   if (sm_count() > 0)  // before the occupancy query, which depends on it
-    rc = set_max_dynamic_smem(reinterpret_cast<const void*>(kern), ckpt::Ring<RAW>::kSmem, smem_set,
+    rc = set_max_dynamic_smem(reinterpret_cast<const void*>(kern), ckpt::SMEM_BYTES, smem_set,
                               "gemm_dw_int8: set max dynamic shared memory");
-  *clusters = pair_clusters(kern, ckpt::Ring<RAW>::kSmem, ckpt::Ring<RAW>::kThreads);
+  *clusters = pair_clusters(kern, ckpt::SMEM_BYTES, ckpt::kThreads);
   return rc;
 }
 
 int dw_run(int64_t M, int64_t N, int64_t K, DwRun* r) {
   const int64_t tiles = ((N + ckpt::TM - 1) / ckpt::TM) * ((K + ckpt::TN - 1) / ckpt::TN);
+  if (tiles > (1 << 24)) {
+    set_error("gemm_dw_int8: dW is too large (N %lld, K %lld)", (long long)N, (long long)K);
+    return C3CU_ERR_INVALID;
+  }
   const int blocks = static_cast<int>((M + ckpt::BK - 1) / ckpt::BK);
-  // Widening X in the kernel slows each K block by about 0.2 us (0.6 instead of 0.4); widening it first
-  // costs a launch, about 2.5 us, and three bytes per element of X at 6 TB/s.
-  dw_clusters<true>(&r->clusters);
+  const int rc = dw_clusters(&r->clusters);
+  if (rc != C3CU_OK) return rc;
   r->plan = ckpt::make_plan(static_cast<int>(tiles), r->clusters, blocks);
-  const double rounds = static_cast<double>(r->plan.whole / r->clusters) * blocks +
-                        (r->plan.rest > 0 ? r->plan.kb_per_piece : 0);
-  const double whole_only = r->plan.rest > 0 ? rounds : static_cast<double>((tiles + r->clusters - 1) / r->clusters) * blocks;
-  const double widening = 3. * static_cast<double>(M) * static_cast<double>(K) / 6e6;
-  r->raw = 0.2 * whole_only < 2.5 + widening;
-  // The faster kernel by a model of both, fitted to B200 measurements (us; K blocks of 64 rows of X):
-  //   large  3.3 + waves * 2.6 + blocks (0.43 RAW, 0.36 else) + cut tiles 2.8 + 0.09 pieces + widening
-  //   small  1.3 + waves (blocks c(T) + e(T)), e for a split tile 3.5 + 0.021 T
-  // Over 57 random sizes it misses the fastest form by 0.8 % on average, large tiles alone by 29 %.
-  // Measured, small / large: 256 x 784 over 128 rows 4.1 / 6.5, 32 x 25 over 2908 6.9 / 11.1, 1024 x
-  // 1024 over 2048 13.8 / 15.9, 2176 x 4822 over 576 37 / 21.
+  // The fastest form by a model of all, fitted to B200 measurements (us in a graph; blocks: K blocks of 64
+  // rows of X that a CTA or pair goes through):
+  //   large            6.0 + waves * 2.06 + blocks 0.34 + cut tiles 2.0 + 0.1 pieces + prep
+  //   small, ready     3.9 + waves (blocks c(T) + e(T)) + prep, the operands' bytes: through L2, or HBM
+  //   small, converted 1.2 + waves (blocks c(T) + e(T)), e for a split tile 3.2 + 0.026 T
+  // Over 330 random sizes its choice takes 0.2 % longer than the fastest form on average. Measured, large /
+  // ready / converted: 256 x 784 over 128 rows 8.8 / 7.3 / 4.6, 1024 x 1024 over 2048 20.0 / 14.7 / 18.5,
+  // 512 x 512 over 4096 18.6 / 14.6 / 15.9, 2176 x 4822 over 576 24 / 39 / 50.
   r->T = 0;
-  if (gemm_max_ctas() == 0) {  // else the persistent kernel keeps to the caller's CTAs
+  r->ready = true;
+  if (g_form_tile > 0) {
+    if (g_form_tile < 32 || g_form_tile > 128) {
+      set_error("gemm_dw_int8: no tiles of %d rows", g_form_tile);
+      return C3CU_ERR_INVALID;
+    }
+    r->T = g_form_tile;
+    r->split = g_form_split;
+    r->kb_per_cta = (blocks + g_form_split - 1) / g_form_split;
+    r->ready = g_form_ready;
+  } else if (g_form_tile < 0 && gemm_max_ctas() == 0) {  // a cap: the persistent kernel keeps to it
+    const double rounds = r->plan.rest > 0
+                              ? static_cast<double>(r->plan.whole / r->clusters) * blocks + r->plan.kb_per_piece
+                              : static_cast<double>((tiles + r->clusters - 1) / r->clusters) * blocks;
     const double turns = static_cast<double>((tiles + r->clusters - 1) / r->clusters);
-    double least = 3.3 + 2.6 * turns + (r->raw ? 0.43 : 0.36) * whole_only +
-                   (r->plan.rest > 0 ? 2.8 + 0.09 * r->plan.rest * r->plan.pieces : 0.) + (r->raw ? 0. : 1. + widening);
+    const double bytes = static_cast<double>(M) * (6. * static_cast<double>(N) + 3. * static_cast<double>(K));
+    const double prep = bytes / 7.07e6 + (bytes > 42e6 ? (bytes - 42e6) / 12.9e6 : 0.);
+    double least = 6.0 + 2.06 * turns + 0.34 * rounds + (r->plan.rest > 0 ? 2.0 + 0.1 * r->plan.rest * r->plan.pieces : 0.) + prep;
     constexpr struct {
       int T;
       double c, e;
-    } kinds[] = {{32, 0.37, 2.6}, {64, 0.40, 2.9}, {128, 0.44, 3.8}};
+    } kinds[2][3] = {{{32, 0.38, 2.5}, {64, 0.515, 3.05}, {128, 0.655, 4.0}},
+                     {{32, 0.28, 2.3}, {64, 0.235, 2.6}, {128, 0.335, 3.85}}};
     const int64_t k_tiles = (K + ckpt_narrow::COLS - 1) / ckpt_narrow::COLS;
     const AtOnce at_once = clusters_at_once();
-    for (const auto& kind : kinds) {
-      if (kind.T > 32 && kind.T >= 2 * N) break;  // half of it would do
-      const int64_t small = k_tiles * ((N + kind.T - 1) / kind.T);
-      for (int split = 1; split <= ckpt_narrow::kMaxCluster && split <= blocks; split *= 2) {
-        const int per = (blocks + split - 1) / split;
-        const double t = 1.3 + static_cast<double>((small + at_once(split) - 1) / at_once(split)) *
-                                   (per * kind.c + (split > 1 ? 3.5 + 0.021 * kind.T : kind.e));
-        if (t < least) {
-          least = t;
-          r->T = kind.T;
-          r->split = split;
-          r->kb_per_cta = per;
+    for (int ready = 0; ready < 2; ++ready) {
+      for (const auto& kind : kinds[ready]) {
+        if (kind.T > 32 && kind.T >= 2 * N) break;  // half of it would do
+        const int64_t small = k_tiles * ((N + kind.T - 1) / kind.T);
+        for (int split = 1; split <= ckpt_narrow::kMaxCluster && split <= blocks; split *= 2) {
+          const int per = (blocks + split - 1) / split;
+          const double e = split == 1 ? kind.e : (ready ? 3.4 : 3.2) + 0.026 * kind.T;
+          const double t = (ready ? 3.9 + prep : 1.2) +
+                           static_cast<double>((small + at_once(split) - 1) / at_once(split)) * (per * kind.c + e);
+          if (t < least) {
+            least = t;
+            r->T = kind.T;
+            r->split = split;
+            r->kb_per_cta = per;
+            r->ready = ready == 1;
+          }
         }
       }
     }
   }
-  if (r->T > 0) {
-    r->partial_bytes = r->wide_bytes = 0;
-    return C3CU_OK;
-  }
-  const int rc = r->raw ? dw_clusters<true>(&r->clusters) : dw_clusters<false>(&r->clusters);
-  r->plan = ckpt::make_plan(static_cast<int>(tiles), r->clusters, blocks);
-  r->partial_bytes = static_cast<size_t>(r->plan.rest) * r->plan.pieces * ckpt::TM * ckpt::TN * sizeof(float);
-  r->wide_ld = (K + 7) / 8 * 8;
-  r->wide_bytes = r->raw ? 0 : static_cast<size_t>(M) * r->wide_ld * 2;
-  return rc;
+  r->bytes = 0;
+  if (!r->ready) return C3CU_OK;
+  ckpt::Prep& p = r->prep;
+  p = ckpt::Prep{};
+  p.M = static_cast<int32_t>(M);
+  p.N = static_cast<int32_t>(N);
+  p.K = static_cast<int32_t>(K);
+  p.tiles = static_cast<int32_t>((N + 63) / 64);
+  // as many items as blocks that run at once, four an SM, so that each streams its rows without a restart
+  int64_t bands = static_cast<int64_t>(sm_count() > 0 ? sm_count() : 148) * 4 / p.tiles;
+  bands = bands < 1 ? 1 : bands > ckpt::kMaxBands ? ckpt::kMaxBands : bands;
+  int64_t rows = (M + bands - 1) / bands;
+  rows = (rows + ckpt::kPrepRows - 1) / ckpt::kPrepRows * ckpt::kPrepRows;
+  if (rows < 128) rows = 128;
+  p.band_rows = static_cast<int32_t>(rows);
+  p.bands = static_cast<int32_t>((M + rows - 1) / rows);
+  p.ldz = (N + 7) / 8 * 8;
+  p.ldx16 = (K + 7) / 8 * 8;
+  const auto part = [r](size_t bytes) {  // parts start on 256 bytes
+    const size_t at = r->bytes;
+    r->bytes += (bytes + 255) / 256 * 256;
+    return at;
+  };
+  part(r->T > 0 ? 0 : static_cast<size_t>(r->plan.rest) * r->plan.pieces * ckpt::TM * ckpt::TN * sizeof(float));
+  r->top_at = part(static_cast<size_t>(p.bands) * p.tiles * 64 * sizeof(float));
+  r->back_at = part(static_cast<size_t>(p.tiles) * 64 * sizeof(float));
+  r->z_at = part(static_cast<size_t>(M) * p.ldz * sizeof(__half));
+  r->x_at = part(static_cast<size_t>(M) * p.ldx16 * sizeof(__half));
+  return C3CU_OK;
 }
 
-template <bool RAW>
-int launch_dw(const CUtensorMap& ta, const CUtensorMap& tx, const ckpt::Params& p, int clusters, cudaStream_t st) {
-  const int items = ckpt::item_count(p.plan);
-  if (items < clusters) clusters = items;
-  // not RAW: the kernel that widens X is before it
-  int rc = cuda_status(launch_serialized(!RAW || pdl_enabled(), ckpt::dw_kernel<RAW>, dim3(2 * clusters),
-                                         dim3(ckpt::Ring<RAW>::kThreads), ckpt::Ring<RAW>::kSmem, st, ta, tx, p),
+template <int T, bool READY>
+int launch_dw_narrow(const CUtensorMap& tz, const CUtensorMap& tx, const ckpt_narrow::Params& p, int split,
+                     cudaStream_t st) {
+  auto kern = ckpt_narrow::dw_narrow_kernel<T, READY>;
+  static std::atomic<uint64_t> smem_set{0};
+  const int rc = set_max_dynamic_smem(reinterpret_cast<const void*>(kern), ckpt_narrow::Ring<T, READY>::kSmem, smem_set,
+                                      "gemm_dw_int8: set max dynamic shared memory");
+  if (rc != C3CU_OK) return rc;
+  const int64_t grid = static_cast<int64_t>(p.k_tiles) * ((p.N + T - 1) / T) * split;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.blockDim = dim3(ckpt_narrow::kThreads);
+  cfg.dynamicSmemBytes = ckpt_narrow::Ring<T, READY>::kSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(split);
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // READY: after operands_kernel
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = READY ? 2 : 1;
+  return cuda_status(cudaLaunchKernelEx(&cfg, kern, tz, tx, p), "gemm_dw_int8: launch");
+}
+
+template <bool READY>
+int launch_dw_tiles(const DwRun& r, const CUtensorMap& tz, const CUtensorMap& tx, const ckpt_narrow::Params& p,
+                    cudaStream_t st) {
+  switch (r.T) {
+    case 32: return launch_dw_narrow<32, READY>(tz, tx, p, r.split, st);
+    case 64: return launch_dw_narrow<64, READY>(tz, tx, p, r.split, st);
+    default: return launch_dw_narrow<128, READY>(tz, tx, p, r.split, st);
+  }
+}
+
+// The product from the operands in the workspace.
+int launch_dw_ready(const DwRun& r, const ckpt::Prep& a, const ckpt::Params& p, cudaStream_t st) {
+  // a block an item, or as many as the caller's cap
+  const int64_t most = gemm_max_ctas() > 0 ? gemm_max_ctas() : INT32_MAX;
+  const auto grid = [most](int64_t items) { return dim3(static_cast<unsigned>(items < most ? items : most)); };
+  const int64_t dz_items = static_cast<int64_t>(a.tiles) * a.bands;
+  const int64_t x_items = (static_cast<int64_t>(a.M) + ckpt::kWidenRows - 1) / ckpt::kWidenRows;
+  int rc = cuda_status(launch_kernel(ckpt::column_top_kernel, grid(dz_items), dim3(ckpt::kPrepThreads), 0, st, a),
                        "gemm_dw_int8: launch");
+  if (rc != C3CU_OK) return rc;
+  rc = cuda_status(launch_next(ckpt::operands_kernel, grid(dz_items + x_items), dim3(ckpt::kPrepThreads), 0, st, a),
+                   "gemm_dw_int8: launch");
+  if (rc != C3CU_OK) return rc;
+  CUtensorMap tz, tx;  // fp16, which TMA moves like any two bytes
+  if ((rc = encode_bf16_2d_sw128(&tz, a.z16, p.M, p.N, a.ldz, 64, ckpt::BK)) != C3CU_OK) return rc;
+  if ((rc = encode_bf16_2d_sw128(&tx, a.x16, p.M, p.K, a.ldx16, 64, ckpt::BK)) != C3CU_OK) return rc;
+  if (r.T > 0) {
+    const ckpt_narrow::Params q{p.M, p.N, p.K, p.out, p.ldo, p.back, r.kb_per_cta, (p.K + ckpt_narrow::COLS - 1) / ckpt_narrow::COLS};
+    return launch_dw_tiles<true>(r, tz, tx, q, st);
+  }
+  const int items = ckpt::item_count(p.plan);
+  const int clusters = items < r.clusters ? items : r.clusters;
+  rc = cuda_status(launch_next(ckpt::dw_kernel, dim3(2 * clusters), dim3(ckpt::kThreads), ckpt::SMEM_BYTES, st, tz, tx, p),
+                   "gemm_dw_int8: launch");
   if (rc != C3CU_OK || p.plan.rest == 0) return rc;
   return cuda_status(launch_next(ckpt::add_pieces_kernel, dim3(ckpt::TM / ckpt::kAddRows, p.plan.rest), dim3(ckpt::TN),
                                  0, st, p),
                      "gemm_dw_int8: launch");
 }
 
-template <int T>
-int launch_dw_narrow(const CUtensorMap& tz, const CUtensorMap& tx, const ckpt_narrow::Params& p, int split,
-                     cudaStream_t st) {
-  auto kern = ckpt_narrow::dw_narrow_kernel<T>;
-  static std::atomic<uint64_t> smem_set{0};
-  const int rc = set_max_dynamic_smem(reinterpret_cast<const void*>(kern), ckpt_narrow::Ring<T>::kSmem, smem_set,
-                            "gemm_dw_int8: set max dynamic shared memory");
-  if (rc != C3CU_OK) return rc;
-  const int64_t grid = static_cast<int64_t>(p.k_tiles) * ((p.N + T - 1) / T) * split;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(grid));
-  cfg.blockDim = dim3(ckpt_narrow::kThreads);
-  cfg.dynamicSmemBytes = ckpt_narrow::Ring<T>::kSmem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = static_cast<unsigned>(split);
-  attr.val.clusterDim.y = 1;
-  attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return cuda_status(cudaLaunchKernelEx(&cfg, kern, tz, tx, p), "gemm_dw_int8: launch");
-}
-
 }  // namespace
 }  // namespace c3cu
+
+extern "C" int c3cu_set_int8_form(int tile, int split, int ready) {
+  using namespace c3cu;
+  const auto power = [](int v, int lo, int hi) { return v >= lo && v <= hi && (v & (v - 1)) == 0; };
+  if (tile > 0 ? !power(tile, 16, 256) || !power(split, 1, 8) : tile < -1) {
+    set_error("set_int8_form: tile %d, split %d", tile, split);
+    return C3CU_ERR_INVALID;
+  }
+  g_form_tile = tile;
+  g_form_split = tile > 0 ? split : 1;
+  g_form_ready = ready != 0;
+  return C3CU_OK;
+}
 
 extern "C" int c3cu_linear_int8_fwd(const int8_t* X, int64_t ldx, const float* x_scale, const int8_t* W, int64_t ldw,
                                     const float* w_scale, const float* bias, void* Y, int64_t ldy, int out_dtype,
@@ -421,8 +509,7 @@ extern "C" size_t c3cu_gemm_dw_int8_workspace(int64_t M, int64_t N, int64_t K) {
   using namespace c3cu;
   if (M < 1 || N < 1 || K < 1 || check_gemm_sizes("gemm_dw_int8", M, N, K) != C3CU_OK) return 0;
   DwRun r;
-  dw_run(M, N, K, &r);
-  return r.partial_bytes + r.wide_bytes;
+  return dw_run(M, N, K, &r) == C3CU_OK ? r.bytes : 0;
 }
 
 extern "C" int c3cu_gemm_dw_int8(const void* dZ, int64_t lddz, const int8_t* X, int64_t ldx, const float* x_scale,
@@ -450,47 +537,43 @@ extern "C" int c3cu_gemm_dw_int8(const void* dZ, int64_t lddz, const int8_t* X, 
     set_error("gemm_dw_int8: a pointer is not aligned to its type");
     return C3CU_ERR_ALIGN;
   }
-  ckpt::Params p{};
-  p.M = static_cast<int32_t>(M);
-  p.N = static_cast<int32_t>(N);
-  p.K = static_cast<int32_t>(K);
-  p.out = static_cast<__nv_bfloat16*>(dW);
-  p.ldo = lddw;
-  p.scale = x_scale;
-  p.partial = static_cast<float*>(workspace);
-  if (((N + 255) / 256) * ((K + 255) / 256) > (1 << 24)) {
-    set_error("gemm_dw_int8: dW is too large (N %lld, K %lld)", (long long)N, (long long)K);
-    return C3CU_ERR_INVALID;
-  }
+  // the same rule in both forms, of which one reads by TMA
+  if ((rc = check_bf16_rows(dZ, N, lddz)) != C3CU_OK) return rc;
+  if ((rc = check_int8_rows(X, K, ldx)) != C3CU_OK) return rc;
   DwRun r;
   if ((rc = dw_run(M, N, K, &r)) != C3CU_OK) return rc;
-  p.plan = r.plan;
-  const size_t need = r.partial_bytes + r.wide_bytes;
-  if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace))) {
-    set_error("gemm_dw_int8: workspace of %zu bytes (16-byte aligned), %zu needed", workspace ? workspace_bytes : 0, need);
+  if (r.bytes > 0 && (!workspace || workspace_bytes < r.bytes || !aligned16(workspace))) {
+    set_error("gemm_dw_int8: workspace of %zu bytes (16-byte aligned), %zu needed", workspace ? workspace_bytes : 0, r.bytes);
     return C3CU_ERR_WORKSPACE;
   }
-  CUtensorMap ta, tx;
-  if ((rc = encode_bf16_2d_sw128(&ta, dZ, M, N, lddz, 64, ckpt::BK)) != C3CU_OK) return rc;
-  // X's rows are checked by the same rule in both forms
-  if ((rc = encode_int8_2d(&tx, X, M, K, ldx, ckpt::HN, ckpt::BK, false)) != C3CU_OK) return rc;
-  if (r.T > 0) {
-    const ckpt_narrow::Params q{p.M, p.N, p.K, p.out, p.ldo, p.scale, r.kb_per_cta,
-                                (p.K + ckpt_narrow::COLS - 1) / ckpt_narrow::COLS};
-    switch (r.T) {
-      case 32: return launch_dw_narrow<32>(ta, tx, q, r.split, st);
-      case 64: return launch_dw_narrow<64>(ta, tx, q, r.split, st);
-      default: return launch_dw_narrow<128>(ta, tx, q, r.split, st);
-    }
+  if (!r.ready) {
+    CUtensorMap tz, tx;
+    if ((rc = encode_bf16_2d_sw128(&tz, dZ, M, N, lddz, 64, ckpt::BK)) != C3CU_OK) return rc;
+    if ((rc = encode_int8_2d(&tx, X, M, K, ldx, ckpt_narrow::COLS, ckpt::BK, false)) != C3CU_OK) return rc;
+    const ckpt_narrow::Params q{static_cast<int32_t>(M), static_cast<int32_t>(N), static_cast<int32_t>(K),
+                                static_cast<__nv_bfloat16*>(dW), lddw, x_scale, r.kb_per_cta,
+                                static_cast<int32_t>((K + ckpt_narrow::COLS - 1) / ckpt_narrow::COLS)};
+    return launch_dw_tiles<false>(r, tz, tx, q, st);
   }
-  if (r.raw) return launch_dw<true>(ta, tx, p, r.clusters, st);
-  __nv_bfloat16* wide = reinterpret_cast<__nv_bfloat16*>(static_cast<uint8_t*>(workspace) + r.partial_bytes);
-  const int64_t want = (M + ckpt::kWidenWarps - 1) / ckpt::kWidenWarps, most = static_cast<int64_t>(sm_count()) * 8;
-  rc = cuda_status(launch_kernel(ckpt::widen_kernel, dim3(static_cast<unsigned>(want < most ? want : most)),
-                                 dim3(32 * ckpt::kWidenWarps), 0, st, X, ldx, x_scale, wide, r.wide_ld,
-                                 static_cast<int>(M), static_cast<int>(K)),
-                   "gemm_dw_int8: launch");
-  if (rc != C3CU_OK) return rc;
-  if ((rc = encode_bf16_2d_sw128(&tx, wide, M, K, r.wide_ld, 64, ckpt::BK)) != C3CU_OK) return rc;
-  return launch_dw<false>(ta, tx, p, r.clusters, st);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  ckpt::Prep a = r.prep;
+  a.dz = static_cast<const __nv_bfloat16*>(dZ);
+  a.lddz = lddz;
+  a.q = X;
+  a.ldq = ldx;
+  a.scale = x_scale;
+  a.top = reinterpret_cast<float*>(ws + r.top_at);
+  a.back = reinterpret_cast<float*>(ws + r.back_at);
+  a.z16 = reinterpret_cast<__half*>(ws + r.z_at);
+  a.x16 = reinterpret_cast<__half*>(ws + r.x_at);
+  ckpt::Params p{};
+  p.M = a.M;
+  p.N = a.N;
+  p.K = a.K;
+  p.out = static_cast<__nv_bfloat16*>(dW);
+  p.ldo = lddw;
+  p.back = a.back;
+  p.partial = reinterpret_cast<float*>(ws);
+  p.plan = r.plan;
+  return launch_dw_ready(r, a, p, st);
 }

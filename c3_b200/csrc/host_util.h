@@ -44,8 +44,9 @@ int encode_bf16_2d_sw128(CUtensorMap* map, const void* base, uint64_t rows, uint
 int encode_int8_2d(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_cols,
                    uint32_t box_rows, bool swizzle);
 
-// The same rules (16-byte aligned base and stride) for int8 rows that a kernel reads without a map.
+// The same rules (16-byte aligned base and stride) for rows that a kernel reads without a map.
 int check_int8_rows(const void* base, uint64_t cols, uint64_t ld);
+int check_bf16_rows(const void* base, uint64_t cols, uint64_t ld);
 
 // Called by c3cu_fault_status when a kernel recorded a fault: a split-K GEMM whose adder gave
 // up waiting may leave its ticket and ready words non-zero (its partner publishes after the

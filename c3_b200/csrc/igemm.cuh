@@ -129,13 +129,6 @@ __device__ __forceinline__ void store_tokens(const Params& p, const uint32_t (&a
   }
 }
 
-// Counts an arrival on a barrier of the leader CTA without a release at cluster scope, which would
-// wait for the warp's stores to reach memory: what the arrival reports is that the accumulator has
-// been read, and the tcgen05 fence orders that.
-__device__ __forceinline__ void arrive_leader(uint64_t* bar) {
-  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(mapa_shared(smem_u32(bar), 0u)) : "memory");
-}
-
 // ================================================================ CTA pairs
 namespace pair {
 using gemm2::A_STAGE_BYTES;
@@ -304,7 +297,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::kThreads, 1)
         } else {
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) arrive_leader(&acc_empty[acc]);
+          if (lane == 0) mbar_arrive_leader(&acc_empty[acc]);
         }
         const int m = m0 + c * 32;
         my_xs[lane] = xs[c];

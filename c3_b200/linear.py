@@ -375,8 +375,8 @@ def grad_weight_int8(dZ: torch.Tensor, Xq: torch.Tensor, x_scale: torch.Tensor, 
     """dW = dZ^T (Xq * x_scale) as bf16 [N, K]: `grad_weight` ("nk") with the layer's input kept in 8
     bits (quant.quantize_rows of a bf16 activation, or the int8 rows that went into forward_int8).
 
-    dZ [M, N] bf16 and Xq [M, K] int8, rows starting on 16 bytes. Accumulation is fp32; Xq * x_scale
-    is rounded to bf16 on its way into the tensor cores."""
+    dZ [M, N] bf16 and Xq [M, K] int8, rows starting on 16 bytes. Xq takes part exactly, dZ * x_scale is
+    held to 2^-11 of itself at least, accumulation is fp32: the error is the output's rounding."""
     if dW is None and _on_gpu(Xq):
         r = _lib.fast().grad_weight_int8(dZ, Xq, x_scale)
         if r is not None:

@@ -311,11 +311,20 @@ int c3cu_rms_norm_bwd(const void* dY, int64_t ldy, const void* H, int64_t ldh, c
 int c3cu_linear_int8_fwd(const int8_t* X, int64_t ldx, const float* x_scale, const int8_t* W, int64_t ldw,
                          const float* w_scale, const float* bias, void* Y, int64_t ldy, int out_dtype, int relu,
                          uint32_t* mask, int64_t ldm, int64_t M, int64_t N, int64_t K, c3cu_stream_t stream);
-/* dW[N][K] = sum_m dZ[m][n] (X[m][k] x_scale[m]) as bf16: the weight gradient from an 8-bit
- * checkpoint of the layer's input (fp32 accumulation; X x_scale is rounded to bf16 on its way
- * into the tensor cores). dZ [M][N] bf16. Workspace: c3cu_gemm_dw_int8_workspace(M, N, K) bytes
- * of device memory (16-byte aligned) that no other call uses meanwhile; the size depends on the
- * calling thread's c3cu_set_gemm_max_ctas. */
+/* For tests and tuning: the form that the calling thread's calls of the two int8 GEMMs take whatever their
+ * size and the cap on CTAs. tile -1: chosen by size (the default); 0: the persistent kernel on CTA pairs;
+ * 16 to 256 (forward) or 32 to 128 (dW), powers of two: tiles of that many rows of X or of dW, the sum of
+ * each split over a cluster of `split` CTAs (1, 2, 4 or 8); dW's from operands laid out in the workspace
+ * first if `ready`, else converted in the kernel. A dW workspace is asked for with the same form. */
+int c3cu_set_int8_form(int tile, int split, int ready);
+/* dW[N][K] = sum_m (dZ[m][n] x_scale[m]) X[m][k] as bf16: the weight gradient from an 8-bit
+ * checkpoint of the layer's input. X takes part exactly; dZ x_scale is held to 2^-11 of itself at
+ * least (fp16 with a power of two for each row of dW, or two bf16 terms, by size), so that the
+ * error is that of the output's rounding; fp32 accumulation. dZ [M][N] bf16. A row with scale NaN
+ * makes all of dW NaN; dZ's infinities and NaN reach their row of dW. Workspace:
+ * c3cu_gemm_dw_int8_workspace(M, N, K) bytes of device memory (16-byte aligned) that no other call
+ * uses meanwhile: 0 for small dW, else both operands in fp16 and partial sums; the size depends on
+ * the calling thread's c3cu_set_gemm_max_ctas. */
 size_t c3cu_gemm_dw_int8_workspace(int64_t M, int64_t N, int64_t K);
 int c3cu_gemm_dw_int8(const void* dZ, int64_t lddz, const int8_t* X, int64_t ldx, const float* x_scale, void* dW,
                       int64_t lddw, int64_t M, int64_t N, int64_t K, void* workspace, size_t workspace_bytes,

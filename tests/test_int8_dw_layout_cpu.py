@@ -1,0 +1,106 @@
+"""The converters' addresses of the small-tile weight gradient (csrc/ckpt_layout.h), compiled for the
+host: every piece of both operands is converted once, lands where the 128-byte swizzle puts it, and
+threads that go together touch every bank once."""
+import subprocess
+
+import pytest
+
+from c3_b200.build import CSRC
+
+_LAYOUT = r"""
+#include <cstdio>
+#include <cstring>
+#include "ckpt_layout.h"
+using namespace c3cu::ckpt;
+
+// byte offset of 16-byte piece p (of a chunk's eight) of row r under the 128-byte swizzle: address bits
+// 4..6 are xored with bits 7..9
+static unsigned swizzled(unsigned r, unsigned p) {
+  unsigned a = r * 128 + p * 16;
+  return a ^ ((a >> 3) & 0x70);
+}
+
+static bool banks_once(const unsigned* at) {  // eight 16-byte accesses
+  unsigned seen = 0;
+  for (int i = 0; i < 8; ++i) seen |= 1u << (at[i] / 16 % 8);
+  return seen == 0xff;
+}
+
+static int x_tile() {
+  static char written[16384 / 16], read[8192 / 16];
+  for (int i = 0; i < 4; ++i)
+    for (int t = 0; t < 128; ++t) {
+      const XUnit x = x_unit(t, i);
+      if (x_from(x) % 16 || x_from(x) >= 8192 || read[x_from(x) / 16]++) return 1;
+      const unsigned row = x_from(x) / 128, unit = x_from(x) % 128 / 16;  // columns 16 unit .. 16 unit + 15
+      for (int second = 0; second < 2; ++second) {
+        const bool odd = x.odd_first != (second != 0);  // which half of the unit the kernel stores there
+        const unsigned piece = 2 * unit + (odd ? 1 : 0);
+        const unsigned want = piece / 8 * kChunkBytes + swizzled(row, piece % 8);
+        if (x_to(x, second != 0) != want || written[want / 16]++) return 2;
+      }
+    }
+  for (int i = 0; i < 4; ++i)
+    for (int t = 0; t < 128; t += 8)
+      for (int second = 0; second < 2; ++second) {
+        unsigned from[8], to[8];
+        for (int j = 0; j < 8; ++j) {
+          from[j] = x_from(x_unit(t + j, i));
+          to[j] = x_to(x_unit(t + j, i), second != 0);
+        }
+        if (!banks_once(from) || !banks_once(to)) return 3;
+      }
+  for (char c : read)
+    if (c != 1) return 4;
+  for (char c : written)
+    if (c != 1) return 5;
+  return 0;
+}
+
+template <int T>
+static int dz_tile() {
+  using U = DzUnits<T>;
+  static char seen[U::kChunks][8192 / 16];
+  std::memset(seen, 0, sizeof seen);
+  for (int c = 0; c < U::kChunks; ++c)
+    for (int i = 0; i < U::kRows; ++i) {
+      for (int t = 0; t < 128; ++t) {
+        const int row = U::row(t, i), piece = U::piece(t);
+        if (row < 0 || row >= 64 || piece < 0 || piece >= 8 || 64 * c + 8 * piece >= T) return 1;
+        if (piece_at(row, piece) != swizzled(row, piece)) return 2;
+        if (seen[c][piece_at(row, piece) / 16]++) return 3;
+      }
+      for (int t = 0; t < 128; t += 8) {
+        unsigned at[8];
+        for (int j = 0; j < 8; ++j) at[j] = piece_at(U::row(t + j, i), U::piece(t + j));
+        if (!banks_once(at)) return 4;
+      }
+    }
+  for (int row = 0; row < 64; ++row)
+    for (int col = 0; col < T; col += 8)
+      if (seen[col / 64][swizzled(row, col % 64 / 8) / 16] != 1) return 5;
+  return 0;
+}
+
+int main() {
+  if (const int e = x_tile()) return 10 + e;
+  if (const int e = dz_tile<32>()) return 20 + e;
+  if (const int e = dz_tile<64>()) return 30 + e;
+  if (const int e = dz_tile<128>()) return 40 + e;
+  return 0;
+}
+"""
+
+
+@pytest.fixture(scope="module")
+def compiled(tmp_path_factory):
+    d = tmp_path_factory.mktemp("layout")
+    (d / "layout.cpp").write_text(_LAYOUT)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", f"-I{CSRC}", str(d / "layout.cpp"), "-o", str(d / "layout")],
+                   check=True)
+    return d / "layout"
+
+
+def test_each_piece_is_converted_once_and_lands_in_its_place(compiled):
+    r = subprocess.run([str(compiled)])
+    assert r.returncode == 0, f"check {r.returncode} failed"
