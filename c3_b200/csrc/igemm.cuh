@@ -224,13 +224,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::kThreads, 1)
           if (++s == STAGES) { s = 0; ph ^= 1u; }
         }
       }
-      if (!ok) {
-        if (leader) {
-          for (int t = 0; t < STAGES; ++t)
-            if (armed & (1u << t)) gemm::drain_wait(&full[t], (armed_par >> t) & 1u);
-        }
-        gemm2::settle_inflight_copies();
+      // No copy outlives the CTA, also where the MMA issuer gave up on a late one after this lane was done
+      // (the leader's barriers count both CTAs' copies, and the pair leaves together).
+      if (leader) {
+        for (int t = 0; t < STAGES; ++t)
+          if (armed & (1u << t)) gemm::drain_wait(&full[t], (armed_par >> t) & 1u);
       }
+      if (!ok) gemm2::settle_inflight_copies();
     }
     __syncwarp();
   } else if (warp == 1) {
@@ -330,7 +330,7 @@ constexpr int kThreads = 320;    // TMA, MMA, eight epilogue warps: two a schedu
 constexpr int kMaxStages = 8;
 constexpr int kMaxCluster = 8;
 constexpr uint32_t W_BYTES = BN * BK;
-constexpr uint32_t BAR_BYTES = (2 * kMaxStages + 1) * 8 + 8;
+constexpr uint32_t BAR_BYTES = (2 * kMaxStages + 2) * 8 + 8;
 constexpr uint32_t kMaxRing = 200 * 1024;
 constexpr int kMaxSmem = static_cast<int>(kMaxRing) + 4096;  // barriers and alignment besides
 __host__ __device__ constexpr uint32_t stage_bytes(int T) { return W_BYTES + static_cast<uint32_t>(T) * BK; }
@@ -363,7 +363,8 @@ __global__ void __launch_bounds__(narrow::kThreads)
   uint64_t* full = bars;
   uint64_t* empty = bars + kMaxStages;
   uint64_t* acc_full = bars + 2 * kMaxStages;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kMaxStages + 1);
+  uint64_t* drain = acc_full + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
 
   const uint32_t warp = warp_id_sync();
   const uint32_t lane = lane_id();
@@ -383,6 +384,7 @@ __global__ void __launch_bounds__(narrow::kThreads)
       mbar_init(&empty[s], 1);
     }
     mbar_init(acc_full, 1);
+    mbar_init(drain, 1);
     fence_mbarrier_init();
     tma_prefetch_desc(&tmw);
     tma_prefetch_desc(&tmx);
@@ -402,9 +404,8 @@ __global__ void __launch_bounds__(narrow::kThreads)
     if (lane == 0) {
       int s = 0;
       uint32_t ph = 0, armed = 0u, armed_par = 0u;
-      bool ok = true;
       for (int kb = kb0; kb < kb1; ++kb) {
-        if (!mbar_wait(&empty[s], ph ^ 1u, kFaultWaitEmpty)) { ok = false; break; }
+        if (!mbar_wait(&empty[s], ph ^ 1u, kFaultWaitEmpty)) break;
         mbar_arrive_expect_tx(&full[s], STAGE);
         tma_load_2d(smem + s * STAGE, &tmw, &full[s], kb * BK, n0);
         tma_load_2d(smem + s * STAGE + W_BYTES, &tmx, &full[s], kb * BK, m0);
@@ -412,9 +413,9 @@ __global__ void __launch_bounds__(narrow::kThreads)
         armed_par = (armed_par & ~(1u << s)) | (ph << s);
         if (++s == p.stages) { s = 0; ph ^= 1u; }
       }
-      if (!ok)
-        for (int t = 0; t < p.stages; ++t)
-          if (armed & (1u << t)) gemm::drain_wait(&full[t], (armed_par >> t) & 1u);
+      // no copy outlives the CTA, also where the MMA issuer gave up on a late one after this lane was done
+      for (int t = 0; t < p.stages; ++t)
+        if (armed & (1u << t)) gemm::drain_wait(&full[t], (armed_par >> t) & 1u);
     }
     __syncwarp();
   } else if (warp == 1) {
@@ -422,8 +423,9 @@ __global__ void __launch_bounds__(narrow::kThreads)
       constexpr uint32_t IDESC = make_idesc_s8_s32(BN, T);
       int s = 0;
       uint32_t ph = 0;
+      bool ok = true;
       for (int kb = kb0; kb < kb1; ++kb) {
-        if (!mbar_wait(&full[s], ph, kFaultWaitFull)) break;
+        if (!mbar_wait(&full[s], ph, kFaultWaitFull)) { ok = false; break; }
         tc_fence_after();
         const uint32_t w = smem_u32(smem + s * STAGE);
         const uint32_t x = w + W_BYTES;
@@ -434,8 +436,10 @@ __global__ void __launch_bounds__(narrow::kThreads)
         umma_commit(&empty[s]);
         if (++s == p.stages) { s = 0; ph ^= 1u; }
       }
-      umma_commit(acc_full);  // also on a fault: completes when the MMAs issued so far have
-      gemm::drain_wait(acc_full, 0u);
+      // after a fault the epilogue is not told that the sums are there: it gives up as well
+      if (ok) umma_commit(acc_full);
+      umma_commit(drain);
+      gemm::drain_wait(drain, 0u);
     }
     __syncwarp();
   }
@@ -471,7 +475,7 @@ __global__ void __launch_bounds__(narrow::kThreads)
     // [token][channel], and each CTA adds up and stores its share of the tokens.
     uint32_t* part = reinterpret_cast<uint32_t*>(smem);
     const bool any = kb0 < kb1;  // the last CTAs may have no K block: their sums are zero
-    if (warp >= 2) {
+    if (warp >= 2 && ok) {
 #pragma unroll 1
       for (int c = 16 * half; c < tokens; c += 32) {
         uint32_t r[16];
