@@ -39,7 +39,7 @@ struct Ring {
   static constexpr int kStages = !READY ? 4 : T <= 64 ? 8 : 6;
   static constexpr uint32_t kZ = chunks(T) * MN_CHUNK_BYTES;  // dZ, then head; tail behind it
   static constexpr uint32_t kStage = WIDE_BYTES + (READY ? kZ : 2 * kZ + RAW_BYTES);
-  static constexpr uint32_t kSmem = kStages * kStage + (3 * kStages + 2) * 8 + 8 + 1024;
+  static constexpr uint32_t kSmem = kStages * kStage + (3 * kStages + 2) * 8 + 16 + 1024;
   static_assert(READY || kStages % kConvGroups == 0, "a stage belongs to one group, which so sees each of its phases");
   static_assert(kSmem <= 227 * 1024 && kStages * kStage >= T * COLS * 4, "shared memory");
 };
@@ -177,6 +177,8 @@ __global__ void __launch_bounds__(kThreads)
   uint64_t* acc_full = empty + STAGES;
   uint64_t* drain = acc_full + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  uint32_t* gave_up = tmem_slot + 1;  // set by the MMA lane
+  uint32_t* asked = tmem_slot + 2;    // the TMA lane's stages that were asked for, and their phases
 
   const uint32_t warp = warp_id_sync();
   const uint32_t lane = lane_id();
@@ -191,6 +193,7 @@ __global__ void __launch_bounds__(kThreads)
   const int kb1 = min(kb0 + p.kb_per_cta, blocks);
 
   if (warp == 0 && lane == 0) {
+    *gave_up = 0u;
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&wide[s], kConvWarps);
@@ -236,9 +239,8 @@ __global__ void __launch_bounds__(kThreads)
         armed_par = (armed_par & ~(1u << s)) | (ph << s);
         if (++s == STAGES) { s = 0; ph ^= 1u; }
       }
-      // no copy outlives the CTA, also where another role gave up on a late one after this lane was done
-      for (int t = 0; t < STAGES; ++t)
-        if (armed & (1u << t)) gemm::drain_wait(&full[t], (armed_par >> t) & 1u);
+      asked[0] = armed;
+      asked[1] = armed_par;
     }
     __syncwarp();
   } else if (warp == 1) {
@@ -265,10 +267,11 @@ __global__ void __launch_bounds__(kThreads)
         umma_commit(&empty[s]);
         if (++s == STAGES) { s = 0; ph ^= 1u; }
       }
-      // after a fault the epilogue is not told that the sums are there: it gives up as well
-      if (ok) umma_commit(acc_full);
-      umma_commit(drain);
-      gemm::drain_wait(drain, 0u);
+      // After a fault the epilogue is not told that the sums are there: it gives up as well.
+      if (!ok) *gave_up = 1u;
+      uint64_t* done = ok ? acc_full : drain;
+      umma_commit(done);
+      gemm::drain_wait(done, 0u);
     }
     __syncwarp();
   } else if constexpr (READY) {
@@ -381,6 +384,11 @@ __global__ void __launch_bounds__(kThreads)
 
   tc_fence_before();
   __syncthreads();
+  // No copy outlives the CTA. Where the MMA lane went through all blocks, it saw each of them land; where it
+  // gave up on a late one, the TMA lane, which may have been done long before, waits for them here.
+  if (threadIdx.x == 0 && *gave_up != 0u)
+    for (int t = 0; t < STAGES; ++t)
+      if (asked[0] & (1u << t)) gemm::drain_wait(&full[t], (asked[1] >> t) & 1u);
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, T);

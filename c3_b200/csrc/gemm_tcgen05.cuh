@@ -106,6 +106,7 @@ __device__ __forceinline__ void issue_stage_loads(const CUtensorMap* tma, const 
 // Bounded wait used only while draining after a fault: ignores the fault word so that the
 // drain itself runs to completion (or to its own limit).
 __device__ __forceinline__ bool drain_wait(uint64_t* bar, uint32_t parity) {
+  if (mbar_try_wait(bar, parity)) return true;  // reading the clock first costs more than the usual wait
   const uint64_t t0 = globaltimer_ns();
   while (!mbar_try_wait(bar, parity)) {
     if (globaltimer_ns() - t0 > C3CU_WAIT_LIMIT_NS / 4) {

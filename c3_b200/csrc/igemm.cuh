@@ -330,7 +330,7 @@ constexpr int kThreads = 320;    // TMA, MMA, eight epilogue warps: two a schedu
 constexpr int kMaxStages = 8;
 constexpr int kMaxCluster = 8;
 constexpr uint32_t W_BYTES = BN * BK;
-constexpr uint32_t BAR_BYTES = (2 * kMaxStages + 2) * 8 + 8;
+constexpr uint32_t BAR_BYTES = (2 * kMaxStages + 2) * 8 + 16;
 constexpr uint32_t kMaxRing = 200 * 1024;
 constexpr int kMaxSmem = static_cast<int>(kMaxRing) + 4096;  // barriers and alignment besides
 __host__ __device__ constexpr uint32_t stage_bytes(int T) { return W_BYTES + static_cast<uint32_t>(T) * BK; }
@@ -365,6 +365,8 @@ __global__ void __launch_bounds__(narrow::kThreads)
   uint64_t* acc_full = bars + 2 * kMaxStages;
   uint64_t* drain = acc_full + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  uint32_t* gave_up = tmem_slot + 1;  // set by the MMA lane
+  uint32_t* asked = tmem_slot + 2;    // the TMA lane's stages that were asked for, and their phases
 
   const uint32_t warp = warp_id_sync();
   const uint32_t lane = lane_id();
@@ -379,6 +381,7 @@ __global__ void __launch_bounds__(narrow::kThreads)
   const int kb1 = min(kb0 + p.kb_per_cta, k_blocks);
 
   if (warp == 0 && lane == 0) {
+    *gave_up = 0u;
     for (int s = 0; s < p.stages; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
@@ -413,9 +416,8 @@ __global__ void __launch_bounds__(narrow::kThreads)
         armed_par = (armed_par & ~(1u << s)) | (ph << s);
         if (++s == p.stages) { s = 0; ph ^= 1u; }
       }
-      // no copy outlives the CTA, also where the MMA issuer gave up on a late one after this lane was done
-      for (int t = 0; t < p.stages; ++t)
-        if (armed & (1u << t)) gemm::drain_wait(&full[t], (armed_par >> t) & 1u);
+      asked[0] = armed;
+      asked[1] = armed_par;
     }
     __syncwarp();
   } else if (warp == 1) {
@@ -436,10 +438,11 @@ __global__ void __launch_bounds__(narrow::kThreads)
         umma_commit(&empty[s]);
         if (++s == p.stages) { s = 0; ph ^= 1u; }
       }
-      // after a fault the epilogue is not told that the sums are there: it gives up as well
-      if (ok) umma_commit(acc_full);
-      umma_commit(drain);
-      gemm::drain_wait(drain, 0u);
+      // After a fault the epilogue is not told that the sums are there: it gives up as well.
+      if (!ok) *gave_up = 1u;
+      uint64_t* done = ok ? acc_full : drain;
+      umma_commit(done);
+      gemm::drain_wait(done, 0u);
     }
     __syncwarp();
   }
@@ -512,6 +515,11 @@ __global__ void __launch_bounds__(narrow::kThreads)
 
   tc_fence_before();
   __syncthreads();
+  // No copy outlives the CTA. Where the MMA lane went through all blocks, it saw each of them land; where it
+  // gave up on a late one, the TMA lane, which may have been done long before, waits for them here.
+  if (threadIdx.x == 0 && *gave_up != 0u)
+    for (int t = 0; t < p.stages; ++t)
+      if (asked[0] & (1u << t)) gemm::drain_wait(&full[t], (asked[1] >> t) & 1u);
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, COLS);

@@ -77,26 +77,40 @@ def test_each_decision_is_needed():
     assert any(run(late, s, n, True, False)[0] for s, n, late in CASES)
 
 
-KERNELS = [("igemm.cuh", "igemm_pair_kernel"), ("igemm.cuh", "igemm_narrow_kernel"), ("gemm_ckpt.cuh", "dw_kernel"),
-           ("gemm_ckpt_narrow.cuh", "dw_narrow_kernel")]
-
-
-@pytest.mark.parametrize("file,kernel", KERNELS)
-def test_the_kernels_decide_so(file, kernel):
+def _kernel(file, kernel):
     text = (CSRC / file).read_text()
     start = text.index(f"    {kernel}(const __grid_constant__")
     end = text.find("__global__", start)
-    body = re.sub(r"//[^\n]*", "", text[start:end if end > 0 else len(text)])
+    return re.sub(r"//[^\n]*", "", text[start:end if end > 0 else len(text)])
+
+
+def _roles(body):
+    """The TMA lane's code, the MMA lane's, and what comes after all roles' loops."""
     producer = body[body.index("if (warp == 0) {"):body.index("else if (warp == 1) {")]
-    before, drain = producer.split("drain_wait", 1)
-    loop = before[before.rindex("for (int t = 0;"):]
-    guard = before[:before.rindex("for (int t = 0;")].rstrip()
-    assert "armed" in loop
-    # behind no condition but the pair's leadership
-    assert guard.removesuffix("if (leader) {").rstrip().endswith("}"), guard[-60:]
     mma = body[body.index("else if (warp == 1) {"):]
-    mma = mma[:mma.index("} else") if "} else" in mma else len(mma)]
-    says = [m for m in re.finditer(r"umma_commit(_pair_mc)?\(&?acc_full", mma)]
-    assert len(says) == 1
-    lead = mma[:says[0].start()].rstrip()
-    assert lead.endswith("if (ok)") or lead.endswith("if (!ok) break;"), lead[-40:]
+    return producer, mma[:mma.index("__syncwarp();")], body[body.rindex("tc_fence_before();"):]
+
+
+def _drain(armed, phases):
+    return rf"if \({armed} & \(1u << t\)\) gemm::drain_wait\(&full\[t\], \({phases} >> t\) & 1u\);"
+
+
+@pytest.mark.parametrize("file,kernel", [("igemm.cuh", "igemm_pair_kernel"), ("gemm_ckpt.cuh", "dw_kernel")])
+def test_the_pair_kernels_decide_so(file, kernel):
+    """The leader's TMA lane drains behind no condition of its own; the sums are announced after a break."""
+    producer, mma, _end = _roles(_kernel(file, kernel))
+    assert re.search(r"\}\s*if \(leader\) \{\s*for \(int t = 0; t < STAGES; \+\+t\)\s*" + _drain("armed", "armed_par"), producer)
+    assert mma.count("acc_full") == 1
+    assert re.search(r"if \(!ok\) break;\s*umma_commit_pair_mc\(&acc_full", mma)
+
+
+@pytest.mark.parametrize("file,kernel", [("igemm.cuh", "igemm_narrow_kernel"), ("gemm_ckpt_narrow.cuh", "dw_narrow_kernel")])
+def test_the_small_tile_kernels_decide_so(file, kernel):
+    """The drain is at the end, where the MMA lane gave up: otherwise that lane saw every copy land. The CTA
+    meets at a barrier between the two."""
+    producer, mma, end = _roles(_kernel(file, kernel))
+    assert re.search(r"if \(!ok\) \*gave_up = 1u;\s*uint64_t\* done = ok \? acc_full : drain;\s*umma_commit\(done\);", mma)
+    assert mma.count("acc_full") == 1
+    assert re.search(r"__syncthreads\(\);\s*if \(threadIdx.x == 0 && \*gave_up != 0u\)\s*for \(int t = 0; t < \S+; \+\+t\)\s*"
+                     + _drain(r"asked\[0\]", r"asked\[1\]"), end)
+    assert re.search(r"asked\[0\] = armed;\s*asked\[1\] = armed_par;\s*\}\s*__syncwarp", producer)
