@@ -367,6 +367,11 @@ struct RowRing {
   uint64_t full[kMaxStages];
 };
 
+// A warp gives up as a whole: the reductions below shuffle between all of its lanes.
+__device__ __forceinline__ bool wait_row(RowRing& ring, int s, uint32_t ph) {
+  return __all_sync(0xffffffffu, mbar_wait(&ring.full[s], ph, kFaultWaitFull));
+}
+
 // Fault path: the copies of the row whose wait gave up and of those after it land (or not, which
 // is bounded) before the block's shared memory is given back.
 __device__ __forceinline__ void settle_rows(RowRing& ring, int stages, int s, uint32_t ph, int64_t row, int64_t M) {
@@ -522,7 +527,7 @@ __global__ void __launch_bounds__(1024) ring_rows_kernel(const FwdArgs p) {
   uint32_t ph = 0;
   int64_t row = blockIdx.x;
   for (; row < p.M; row += gridDim.x) {
-    if (!mbar_wait(&ring.full[s], ph, kFaultWaitFull)) break;
+    if (!wait_row(ring, s, ph)) break;
     const uint8_t* at = rows + s * stage;
     Run<V> a[N];
     float2 squares = make_float2(0.f, 0.f);
@@ -721,7 +726,7 @@ __global__ void __launch_bounds__(512) norm_bwd_kernel(const BwdArgs p) {
     const T* from[3] = {static_cast<const T*>(p.dy) + row * p.ldy, static_cast<const T*>(p.h) + row * p.ldhh,
                         p.dh ? static_cast<const T*>(p.dh) + row * p.lddh : nullptr};
     if constexpr (RING) {
-      if (!mbar_wait(&ring.full[s], ph, kFaultWaitFull)) break;
+      if (!wait_row(ring, s, ph)) break;
     }
     auto read = [&](int k, const void* base, int64_t ld, Run<V>(&v)[N]) {
       bool buffered = RING;
@@ -858,7 +863,7 @@ __global__ void __launch_bounds__(kWideThreads) norm_bwd_wide_kernel(const BwdAr
   int64_t row = blockIdx.x;
   for (; row < p.M; row += gridDim.x) {
     const float rs = __ldg(p.rstd + row);
-    if (!mbar_wait(&ring.full[s], ph, kFaultWaitFull)) break;
+    if (!wait_row(ring, s, ph)) break;
     // where the k-th input's row is: in its buffer, or (off the grid, the first and last) where it was
     auto source = [&](int k, const void* base, int64_t ld) {
       const uint8_t* at = rows + s * stage + k * pitch;

@@ -114,3 +114,12 @@ def test_the_small_tile_kernels_decide_so(file, kernel):
     assert re.search(r"__syncthreads\(\);\s*if \(threadIdx.x == 0 && \*gave_up != 0u\)\s*for \(int t = 0; t < \S+; \+\+t\)\s*"
                      + _drain(r"asked\[0\]", r"asked\[1\]"), end)
     assert re.search(r"asked\[0\] = armed;\s*asked\[1\] = armed_par;\s*\}\s*__syncwarp", producer)
+
+
+def test_a_warp_gives_up_as_a_whole():
+    """Where all lanes of a warp wait, one that gave up alone would leave the others in a shuffle or vote that
+    names it: such waits are put to the vote themselves. The TMA and MMA roles are one lane each."""
+    for file, roles in (("quant.cu", 0), ("igemm.cuh", 5), ("gemm_ckpt.cuh", 3), ("gemm_ckpt_narrow.cuh", 3)):
+        text = re.sub(r"//[^\n]*", "", (CSRC / file).read_text())
+        voted = len(re.findall(r"__all_sync\(0xffffffffu, mbar_wait\(", text))
+        assert voted > 0 and len(re.findall(r"mbar_wait\(", text)) == voted + roles, file
