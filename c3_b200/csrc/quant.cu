@@ -318,8 +318,11 @@ __device__ __forceinline__ void row_reduce(float& sum, uint32_t& top, RowSums* s
   if constexpr (TOP) top = __reduce_max_sync(0xffffffffu, lane < warps ? s->top[flip][lane] : 0u);
 }
 
+// 0 for a row of zeros with eps 0, not infinity, which times the row's zeros would be NaN in the scale, in
+// the gradient and so in all of dweight and dW.
 __device__ __forceinline__ float rstd_of(float sum_squares, int K, float eps) {
-  return __fdiv_rn(1.f, __fsqrt_rn(__fadd_rn(__fdiv_rn(sum_squares, static_cast<float>(K)), eps)));
+  const float mean = __fadd_rn(__fdiv_rn(sum_squares, static_cast<float>(K)), eps);
+  return mean == 0.f ? 0.f : __fdiv_rn(1.f, __fsqrt_rn(mean));
 }
 
 // ---------------------------------------------------------------- rows through shared memory

@@ -24,7 +24,9 @@ def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, resi
     weight: fp32 [K]. With a residual (x's shape and type), h = x + residual rounded to x's type is
     the new residual stream; it may be written over either (h=residual or h=x). Without one, h is x.
     h and rstd are what `rms_norm_backward` needs. Rows may be slices of wider ones (unit column
-    stride). A row of h with an infinity or a NaN gets q = 0 and scale NaN."""
+    stride). A row of h with an infinity or a NaN gets q = 0 and scale NaN. A row of zeros has scale 0;
+    with eps = 0 (or one that is 0 in fp32) its rstd is 0 too, so that its gradients are those of a constant.
+    Squares are summed in fp32: |h| up to about 1e18, beyond which rstd and scale are 0."""
     if q is None and scale is None and h is None and rstd is None and _on_gpu(x):
         r = _lib.fast().rms_norm_int8(x, weight, eps, residual)
         if r is not None:

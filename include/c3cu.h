@@ -288,7 +288,10 @@ int c3cu_quantize_rows(const void* X, int64_t ldx, int dtype, int8_t* Q, int64_t
  *   h = x + r (rounded to dtype; R and H may be NULL together: then h is x),
  *   rstd = 1 / sqrt(mean_k h^2 + eps), y = h * rstd * weight,
  *   q = nearest integer to 127 a / A with a = fl32(h * weight), A = max_k |a|; scale = A rstd / 127.
- * Squares are summed in fp32 (|h| up to about 1e18). H may be X or R itself (same stride). */
+ * Where mean_k h^2 + eps is 0 in fp32 (a row of zeros with eps 0), rstd is 0: the row's scale is 0 and its
+ * gradients are those of a constant. Squares are summed in fp32: beyond |h| of about 1e18 the sum is
+ * infinite, rstd and scale 0; below about 1e-19 they vanish beside any eps that is not 0.
+ * H may be X or R itself (same stride). */
 int c3cu_rms_norm_int8(const void* X, int64_t ldx, const void* R, int64_t ldr, int dtype, const float* weight,
                        float eps, void* H, int64_t ldh, int8_t* Q, int64_t ldq, float* scale, float* rstd, int64_t M,
                        int64_t K, c3cu_stream_t stream);
