@@ -110,18 +110,36 @@ def _vector_of(t: torch.Tensor, name: str, dtype: torch.dtype, n: int, dev: int)
         _same_device(t, name, dev)
 
 
-def _require_apart(out: torch.Tensor, name: str, *inputs) -> None:
-    """Refuses a given output (2-D, unit column stride) whose memory reaches into an input's: other
-    rows of that input may still be read when it is written. `inputs` are (tensor, name) pairs."""
-    if out.numel() == 0:
-        return
-    a = out.data_ptr()
-    end = a + ((out.shape[0] - 1) * out.stride(0) + out.shape[1]) * out.element_size()
-    for t, other in inputs:
-        if t is None or t.numel() == 0:
-            continue
-        b = t.data_ptr()
-        if a < b + ((t.shape[0] - 1) * t.stride(0) + t.shape[1]) * t.element_size() and b < end:
+def _rows_span(t: torch.Tensor) -> tuple[int, int, int, int]:
+    """(first byte, rows, bytes from row to row, bytes in a row) of a vector or a matrix with unit column
+    stride."""
+    size = t.element_size()
+    if t.dim() == 1:
+        return t.data_ptr(), 1, 0, t.numel() * size
+    return t.data_ptr(), t.shape[0], t.stride(0) * size, t.shape[1] * size
+
+
+def _overlap(p: torch.Tensor, q: torch.Tensor) -> bool:
+    """Whether two operands share a byte. Other columns of one buffer do not; rows of different strides
+    that lie among each other are taken to."""
+    if p.numel() == 0 or q.numel() == 0:
+        return False
+    a, m, lda, wa = _rows_span(p)
+    b, n, ldb, wb = _rows_span(q)
+    if a >= b + (n - 1) * ldb + wb or b >= a + (m - 1) * lda + wa:
+        return False
+    if m > 1 and n > 1 and lda != ldb:
+        return True
+    ld = lda if m > 1 else ldb if n > 1 else 0
+    off = (b - a) % ld if ld else 0
+    return off < wa or off + wb > ld
+
+
+def _require_apart(out: torch.Tensor, name: str, *others) -> None:
+    """Refuses a given output that shares memory with an input, parts of which may still be read when it is
+    written, or with another output. `others` are (tensor or None, name) pairs."""
+    for t, other in others:
+        if t is not None and _overlap(out, t):
             raise _lib.C3CUError(-1, name, f"overlaps {other}")
 
 
@@ -357,11 +375,15 @@ def forward_int8(Xq: torch.Tensor, x_scale: torch.Tensor, Wq: torch.Tensor, w_sc
     ldy, ldm = N, words
     if Y is not None:
         ldy = _rows_of(Y, "Y", out_dtype, M, N, dev)
-        _require_apart(Y, "Y", (Xq, "Xq"), (Wq, "Wq"))
     if mask is not None:
         if not (relu and save_mask):
             raise _lib.C3CUError(-1, "mask", "a mask belongs to the ReLU output (relu and save_mask)")
         ldm = _rows_of(mask, "mask", torch.int32, M, words, dev)
+    inputs = ((Xq, "Xq"), (x_scale, "x_scale"), (Wq, "Wq"), (w_scale, "w_scale"), (b, "b"))
+    if Y is not None:
+        _require_apart(Y, "Y", *inputs)
+    if mask is not None:
+        _require_apart(mask, "mask", *inputs, (Y, "Y"))
     if Y is None:
         Y = torch.empty(M, N, dtype=out_dtype, device=Xq.device)
     if mask is None and relu and save_mask:
@@ -393,7 +415,7 @@ def grad_weight_int8(dZ: torch.Tensor, Xq: torch.Tensor, x_scale: torch.Tensor, 
     lddw = K
     if dW is not None:
         lddw = _rows_of(dW, "dW", torch.bfloat16, N, K, dev)
-        _require_apart(dW, "dW", (dZ, "dZ"), (Xq, "Xq"))
+        _require_apart(dW, "dW", (dZ, "dZ"), (Xq, "Xq"), (x_scale, "x_scale"))
     else:
         dW = torch.empty(N, K, dtype=torch.bfloat16, device=dZ.device)
     # the workspace is of this call alone: a graph that captures it keeps its own

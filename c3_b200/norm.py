@@ -50,21 +50,28 @@ def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, resi
         if h is not None:
             ldh = _rows_of(h, "h", dtype, M, K, dev)
             _require_same_rows_or_apart(h, ldh, "h", ((x, ldx, "x"), (residual, ldr, "residual")))
+            _require_apart(h, "h", (weight, "weight"))
         else:
             h = torch.empty(M, K, dtype=dtype, device=x.device)
+    # what a given output has to stay clear of: the inputs, h and the outputs before it
+    taken = [(x, "x"), (residual, "residual"), (weight, "weight"), (h, "h")]
     if q is None:
         q, ldq = empty_rows(M, K, x.device), row_stride(K)
     else:
         ldq = _rows_of(q, "q", torch.int8, M, K, dev)
-        _require_apart(q, "q", (x, "x"), (residual, "residual"), (h, "h"))
+        _require_apart(q, "q", *taken)
+        taken.append((q, "q"))
     if scale is None:
         scale = torch.empty(M, dtype=torch.float32, device=x.device)
     else:
         _vector_of(scale, "scale", torch.float32, M, dev)
+        _require_apart(scale, "scale", *taken)
+        taken.append((scale, "scale"))
     if rstd is None:
         rstd = torch.empty(M, dtype=torch.float32, device=x.device)
     else:
         _vector_of(rstd, "rstd", torch.float32, M, dev)
+        _require_apart(rstd, "rstd", *taken)
     _call("c3cu_rms_norm_int8", dev, x.data_ptr(), ldx, _ptr(residual), ldr, code, weight.data_ptr(), eps, _ptr(h), ldh,
           q.data_ptr(), ldq, scale.data_ptr(), rstd.data_ptr(), M, K)
     return q, scale, x if h is None else h, rstd
@@ -119,12 +126,15 @@ def rms_norm_backward(dy: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, r
     if dx is not None:
         lddx = _rows_of(dx, "dx", dtype, M, K, dev)
         _require_same_rows_or_apart(dx, lddx, "dx", ((dy, ldy, "dy"), (h, ldh, "h"), (dh, lddh, "dh")))
+        _require_apart(dx, "dx", (weight, "weight"), (rstd, "rstd"))
     else:
         dx = torch.empty(M, K, dtype=dtype, device=h.device)
     if dweight is None:
         dweight = torch.empty(K, dtype=torch.float32, device=h.device)
     else:
         _vector_of(dweight, "dweight", torch.float32, K, dev)
+        _require_apart(dweight, "dweight", (dy, "dy"), (h, "h"), (dh, "dh"), (weight, "weight"), (rstd, "rstd"),
+                       (dx, "dx"))
     # the workspace is of this call alone: a graph that captures it keeps its own
     if dev == _current_device():
         nb = _lib.load().c3cu_rms_norm_bwd_workspace(M, K)

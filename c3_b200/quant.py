@@ -59,5 +59,6 @@ def quantize_rows(x: torch.Tensor, q: torch.Tensor | None = None, scale: torch.T
         scale = torch.empty(M, dtype=torch.float32, device=x.device)
     else:
         _vector_of(scale, "scale", torch.float32, M, dev)
+        _require_apart(scale, "scale", (x, "x"), (q, "q"))
     _call("c3cu_quantize_rows", dev, x.data_ptr(), ldx, code, q.data_ptr(), ldq, scale.data_ptr(), M, K)
     return q, scale
