@@ -85,8 +85,8 @@ def _ld(t: torch.Tensor) -> int:
 # time for one token: linear 7.5 there, 11.3 through the helpers below, norm 10.2 and 16.1). Everything
 # else goes through the helpers, which leave saying what is wrong with an operand to _require and
 # _require_rows. `dev` is the first operand's device index.
-_current_device = torch._C._cuda_getDevice
-_raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = getattr(torch._C, "_cuda_getDevice", None)  # a torch without CUDA has neither: the module
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # imports, and calls refuse CPU tensors
 
 
 def _rows_of(t: torch.Tensor, name: str, dtype: torch.dtype, rows: int, cols: int, dev: int) -> int:
