@@ -191,6 +191,17 @@ def _cuda_device(values, found: int) -> int:
     return found
 
 
+def _all_devices(values) -> set:
+    """Every CUDA device of the tensors in `values`."""
+    found: set = set()
+    for v in values:
+        if isinstance(v, torch.Tensor):
+            found |= {v.get_device()} - {-1}
+        elif isinstance(v, (list, tuple)):
+            found |= _all_devices(v)
+    return found
+
+
 def on_tensor_device(fn):
     """Runs a wrapper of the C ABI on the device of its CUDA tensor arguments. The library
     launches on the current device with that device's stream, so the call is made with the
@@ -206,7 +217,8 @@ def on_tensor_device(fn):
         if idx == -1:
             return fn(*args, **kwargs)
         if idx == -2:
-            raise C3CUError(-1, fn.__name__, "tensors on different devices")
+            devices = sorted(_all_devices((args, tuple(kwargs.values()))))
+            raise C3CUError(-1, fn.__name__, f"tensors on different devices: cuda:{devices}")
         if idx == current():  # the common case: no device switch
             return fn(*args, **kwargs)
         with torch.cuda.device(idx):
