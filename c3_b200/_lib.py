@@ -1,13 +1,16 @@
 """Loads libc3cu.so (the C-ABI of include/c3cu.h) and declares its signatures.
 
 The product path has no fallback: if the library is missing and cannot be built, or if
-the current device is not an sm_100 part, every entry point raises C3CUError."""
+the current device is not an sm_100 part, every entry point raises C3CUError. (`fast`, a shorter way to
+the same entry points, has one: ctypes.)"""
 from __future__ import annotations
 
 import ctypes
 import functools
+import importlib.util
 import re
 import threading
+import warnings
 from pathlib import Path
 
 import torch
@@ -134,8 +137,23 @@ _FAST_ENTRIES = ("c3cu_quantize_rows", "c3cu_rms_norm_int8", "c3cu_rms_norm_bwd_
 _fast = None
 
 
+class _Ctypes:
+    """In the binding's place where there is none: leaves every call to the Python wrapper."""
+
+    def __getattr__(self, name):
+        return lambda *args: None
+
+
+def _load_fast_calls(path: Path):
+    spec = importlib.util.spec_from_file_location(f"{__package__}._fast_calls", path)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    return module
+
+
 def fast():
-    """The module of csrc/torch/fast_calls.cpp, bound to this library's entry points."""
+    """The module of csrc/torch/fast_calls.cpp for this torch, bound to this library's entry points. Where
+    it can be neither built nor loaded, a stand-in that leaves the calls to Python, with a warning."""
     global _fast
     if _fast is not None:
         return _fast
@@ -143,11 +161,17 @@ def fast():
     with _lock:
         if _fast is None:
             from . import build as _build
-            if not _build.FAST_CALLS.exists():
-                _build.build_fast_calls()
-            from . import _fast_calls
-            _fast_calls.bind(*(ctypes.cast(getattr(L, n), _vp).value for n in _FAST_ENTRIES))
-            _fast = _fast_calls
+            path = _build.fast_calls_path()
+            found = _Ctypes()
+            if path.exists() or _build.try_build_fast_calls() is not None:
+                try:
+                    module = _load_fast_calls(path)
+                    module.bind(*(ctypes.cast(getattr(L, n), _vp).value for n in _FAST_ENTRIES))
+                    found = module
+                except ImportError as e:
+                    warnings.warn(f"the C++ binding of the 8-bit calls does not load, they go through ctypes: {e}",
+                                  RuntimeWarning, stacklevel=2)
+            _fast = found
     return _fast
 
 

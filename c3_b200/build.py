@@ -1,15 +1,20 @@
 """Builds libc3cu.so in-tree: every CUDA translation unit for sm_100a plus the C++ host
 mirror of the C3 API, linked with the static CUDA runtime so that the library loads on
-machines without a GPU driver (calls then report C3CU_ERR_UNSUPPORTED); and _fast_calls.so, the
-binding of the 8-bit path's calls against torch's C++ headers (csrc/torch)."""
+machines without a GPU driver (calls then report C3CU_ERR_UNSUPPORTED); and _fast_calls.<torch>.so, the
+binding of the 8-bit path's calls against the C++ headers of the torch that is installed (csrc/torch).
+The binding only shortens a call's time on the host: where it cannot be built, the calls go through
+ctypes."""
 from __future__ import annotations
 
 import concurrent.futures as cf
+import hashlib
 import os
+import re
 import shutil
 import subprocess
 import sys
 import sysconfig
+import warnings
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -18,7 +23,6 @@ CSRC = PKG / "csrc"
 HOST = CSRC / "host"
 OUT_DIR = PKG / "_build"
 LIB = PKG / "libc3cu.so"
-FAST_CALLS = PKG / "_fast_calls.so"
 
 NVCC = os.environ.get("NVCC", shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc")
 GENCODE = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -58,13 +62,28 @@ def _compile(src: Path) -> Path:
     return obj
 
 
+def _fast_calls_sources() -> tuple[Path, Path]:
+    return CSRC / "torch" / "fast_calls.cpp", ROOT / "include" / "c3cu.h"
+
+
+def fast_calls_path() -> Path:
+    """The binding's file, named for the torch and the Python that it is compiled against and for what it is
+    compiled from: another torch's classes are laid out differently, and another c3cu.h may declare other
+    arguments, so that a binding of theirs must not be loaded."""
+    import torch
+    tag = re.sub(r"[^0-9A-Za-z]+", "_", f"torch{torch.__version__}_{sys.implementation.cache_tag}")
+    text = hashlib.sha256(b"".join(f.read_bytes() for f in _fast_calls_sources())).hexdigest()
+    return PKG / f"_fast_calls.{tag}.{text[:12]}.so"
+
+
 def build_fast_calls() -> Path:
     import torch
-    src, header = CSRC / "torch" / "fast_calls.cpp", ROOT / "include" / "c3cu.h"
-    if FAST_CALLS.exists() and FAST_CALLS.stat().st_mtime >= max(f.stat().st_mtime for f in (src, header)):
-        return FAST_CALLS
+    out = fast_calls_path()
+    if out.exists():
+        return out
+    src = _fast_calls_sources()[0]
     home = Path(torch.__file__).resolve().parent
-    tmp = FAST_CALLS.with_suffix(f".{os.getpid()}.tmp")
+    tmp = out.with_suffix(f".{os.getpid()}.tmp")
     cmd = [os.environ.get("CXX", "g++"), "-std=c++17", "-O2", "-fPIC", "-shared", "-Wall",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{ROOT / 'include'}",
            f"-isystem{home / 'include'}", f"-isystem{home / 'include/torch/csrc/api/include'}",
@@ -73,15 +92,29 @@ def build_fast_calls() -> Path:
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"compile failed: {' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
-    os.replace(tmp, FAST_CALLS)
-    return FAST_CALLS
+    os.replace(tmp, out)
+    for old in PKG.glob("_fast_calls*.so"):
+        if old.name == "_fast_calls.so" or (old != out and old.name.split(".")[1] == out.name.split(".")[1]):
+            old.unlink(missing_ok=True)  # from other sources
+    return out
+
+
+def try_build_fast_calls() -> Path | None:
+    """None, with a warning, where the binding cannot be built (no C++ compiler, a torch without its
+    headers)."""
+    try:
+        return build_fast_calls()
+    except (OSError, RuntimeError) as e:
+        warnings.warn(f"the C++ binding of the 8-bit calls was not built, they go through ctypes: {str(e)[-600:]}",
+                      RuntimeWarning, stacklevel=2)
+        return None
 
 
 def build(verbose: bool = False) -> Path:
     OUT_DIR.mkdir(exist_ok=True)
     cu, cpp = _sources()
     with cf.ThreadPoolExecutor(max_workers=os.cpu_count() or 4) as ex:
-        fast = ex.submit(build_fast_calls)
+        fast = ex.submit(try_build_fast_calls)
         objs = list(ex.map(_compile, cu + cpp))
         fast.result()
     if LIB.exists() and all(LIB.stat().st_mtime >= o.stat().st_mtime for o in objs):
