@@ -222,6 +222,23 @@ class StepEvents:
     allreduce: list
 
 
+class _Marks:
+    """Timing events of one step by phase, where it is recorded."""
+
+    def __init__(self, record: bool, stream):
+        self.record, self.stream = record, stream
+        self.phases: dict = {}
+
+    def __call__(self, name: str) -> None:
+        self.on(name, self.stream)
+
+    def on(self, name: str, stream) -> None:
+        if self.record:
+            e = torch.cuda.Event(enable_timing=True)
+            e.record(stream)
+            self.phases.setdefault(name, []).append(e)
+
+
 class LinearReluTrainStep:
     """The data-parallel captured step of Y = relu(X Wᵀ + b) on one rank's rows.
 
@@ -230,10 +247,15 @@ class LinearReluTrainStep:
     `reserve_sms` SMs are left to the collective while the dX GEMM overlaps it. With the
     "fused" collective: forward → pre-pass → dW GEMM that sums dW and db over the ranks → dX.
 
-    `x_checkpoint="int8"` keeps the layer's input between forward and dW as int8 rows with a scale
-    each (`Xq`, `x_scale`, half of X's bytes): dW then comes from them (linear.grad_weight_int8), so
-    a model of many layers can let each X go after its forward. It needs a bf16 dW that is not
-    summed by the GEMM itself."""
+    A call is the whole step; `forward` and `backward` are its two halves, for a model whose other layers
+    lie between them.
+
+    `x_checkpoint="int8"` keeps the layer's input between the halves as int8 rows with a scale each
+    (`Xq`, `x_scale`, half of X's bytes; the phase "fwd" holds their making): dW then comes from them
+    (linear.grad_weight_int8), and `backward` does without X, which may go after `forward`. In one call
+    X is there all along, and the checkpoint costs its time and bytes for nothing. dW from the
+    checkpoint lays both operands out anew for each of `chunks` bands. It needs a bf16 dW that is not summed
+    by the GEMM itself."""
 
     PHASES = ("fwd", "prepass", "dw", "dx")
 
@@ -293,22 +315,36 @@ class LinearReluTrainStep:
             linear.gemm(dZ, X, True, True, self.epi, dW, M=dZ.shape[1], N=self.k, K=self.m)
 
     def __call__(self, X, W, b, dY, record: bool = False) -> StepEvents | None:
-        from . import _lib, linear, quant
+        marks = _Marks(record, torch.cuda.current_stream(self.device))
+        self._forward(X, W, b, marks)
+        return self._backward(W, dY, X, marks)
+
+    def forward(self, X, W, b) -> torch.Tensor:
+        """Y (`self.Y`) and what `backward` needs beside W, dY and, without an int8 checkpoint, X."""
+        self._forward(X, W, b, _Marks(False, None))
+        return self.Y
+
+    def backward(self, W, dY, X=None) -> torch.Tensor:
+        """dX (`self.dX`), and dW and db summed over the ranks. X: the forward's, unless its int8 checkpoint
+        was kept."""
+        if self.Xq is None and X is None:
+            raise ValueError("without an int8 checkpoint backward needs the forward's X")
+        self._backward(W, dY, X, _Marks(False, torch.cuda.current_stream(self.device)))
+        return self.dX
+
+    def _forward(self, X, W, b, marks: _Marks) -> None:
+        from . import linear, quant
+        marks("fwd")
+        linear.forward(X, W, b, "nk", self.Y, self.mask)
+        if self.Xq is not None:
+            quant.quantize_rows(X, self.Xq, self.x_scale)
+        marks("fwd")
+
+    def _backward(self, W, dY, X, marks: _Marks) -> StepEvents | None:
+        from . import _lib, linear
         comp = torch.cuda.current_stream(self.device)
-        phases: dict = {}
+        record, mark, phases, mark_on = marks.record, marks, marks.phases, marks.on
         ar: list = []
-
-        def mark(name):
-            if record:
-                e = torch.cuda.Event(enable_timing=True)
-                e.record(comp)
-                phases.setdefault(name, []).append(e)
-
-        def mark_on(name, stream):
-            if record:
-                e = torch.cuda.Event(enable_timing=True)
-                e.record(stream)
-                phases.setdefault(name, []).append(e)
 
         def events():
             out = {p: (phases[p][0], phases[p][1]) for p in self.PHASES}
@@ -316,9 +352,6 @@ class LinearReluTrainStep:
                 out["dwdx"] = (phases["dwdx"][0], phases["dwdx"][1])
             return StepEvents(out, ar)
 
-        mark("fwd"); linear.forward(X, W, b, "nk", self.Y, self.mask); mark("fwd")
-        if self.Xq is not None:
-            quant.quantize_rows(X, self.Xq, self.x_scale)
         mark("prepass"); linear.relu_mask_db(dY, self.mask, self.dZ, self.db); mark("prepass")
         if self.overlap_dx:
             # dW (with its sum over the ranks when fused) on the compute stream, dX beside it;

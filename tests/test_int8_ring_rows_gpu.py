@@ -14,7 +14,7 @@ def _kernels(call):
     """Names of the kernels that a call launches, or None where the profiler sees no GPU."""
     from torch.profiler import ProfilerActivity, profile
     torch.cuda.synchronize()
-    with profile(activities=[ProfilerActivity.CUDA]) as p:
+    with profile(activities=[ProfilerActivity.CUDA], acc_events=True) as p:
         call()
         torch.cuda.synchronize()
     names = [e.key for e in p.key_averages() if "kernel" in e.key]
