@@ -203,8 +203,9 @@ int igemv_split(int64_t blocks, int64_t K) {
 }
 
 // Up to two tokens always, up to four while their multiplications do not outweigh a tile on the tensor
-// cores. Measured (us, igemv / narrow): one token, 4096 x 4096 5.2 / 7.3, 1397 x 777 2.4 / 4.7, 12288 x
-// 12288 26 / 34.5; two, 12288 x 4096 12.8 / 11.9; four, 4096 x 4096 7.1 / 7.7, 12288 x 4096 16 / 11.9.
+// cores. Measured (us in a graph, igemv / the best narrow form): one token, 4096 x 4096 5.0 / 7.4, 1024 x
+// 1024 2.0 / 4.4, 12288 x 12288 25.5 / 27.9; two, 12288 x 4096 11.1 / 11.8, 16384 x 16384 44.6 / 45.7; four,
+// 4096 x 4096 6.3 / 7.5, 12288 x 4096 16 / 11.8.
 bool use_igemv(int64_t M, int64_t N, int64_t K) {
   if (g_form_tile >= 0) return false;
   if (gemm_max_ctas() > 0) return false;  // the persistent kernel keeps to the caller's CTAs

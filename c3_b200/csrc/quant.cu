@@ -202,7 +202,7 @@ __device__ __forceinline__ void store_sums(float* out, int t, int i, int G, int 
 // ---------------------------------------------------------------- rounding to int8
 struct RowScale {
   float big;   // A
-  float inv;   // 127 / A, within 2^-24 of it
+  float inv;   // 127 / A, within 2^-24 of it: an approximate reciprocal and one step of Newton's method
   float safe;  // largest |a inv - round(a inv)| at which a inv rounds like the real quotient
   bool finite, tame;
 };
@@ -661,6 +661,32 @@ struct BwdArgs {
   int stages;      // ring form
 };
 
+// Asks for a row of dy, h and dh, `pitch` apart from `to` on, and arms `bar` with their bytes. Off the
+// 16-byte grid the rows that would reach past their matrix are left out.
+template <typename T, int SG>
+__device__ __forceinline__ void fill_bwd_row(const BwdArgs& p, uint8_t* to, uint64_t* bar, int64_t row, uint32_t bytes,
+                                             uint32_t pitch) {
+  if constexpr (SG == 0) {
+    mbar_arrive_expect_tx(bar, (p.dh ? 3u : 2u) * pitch);
+    bulk_load(to, static_cast<const T*>(p.dy) + row * p.ldy, bytes, bar);
+    bulk_load(to + pitch, static_cast<const T*>(p.h) + row * p.ldhh, bytes, bar);
+    if (p.dh) bulk_load(to + 2 * pitch, static_cast<const T*>(p.dh) + row * p.lddh, bytes, bar);
+  } else {
+    Span sp[3];
+    sp[0] = row_span<T>(p.dy, p.ldy, p.M, row, bytes);
+    sp[1] = row_span<T>(p.h, p.ldhh, p.M, row, bytes);
+    sp[2] = row_span<T>(p.dh, p.lddh, p.M, row, bytes);
+    if (!p.dh) sp[2].direct = true;
+    uint32_t tx = 0u;
+#pragma unroll
+    for (int k = 0; k < 3; ++k) tx += sp[k].direct ? 0u : sp[k].size;
+    mbar_arrive_expect_tx(bar, tx);
+#pragma unroll
+    for (int k = 0; k < 3; ++k)
+      if (!sp[k].direct) bulk_load(to + k * pitch, sp[k].from, sp[k].size, bar);
+  }
+}
+
 // g = w dy, xhat = h rstd: dx = rstd (g - xhat mean(g xhat)) + dh, dweight = sum_rows dy xhat.
 // A block walks over rows (grid-strided); a thread owns the same N runs of columns in each, so
 // dweight's share of the block stays in registers until the end. RING: rows come through the ring
@@ -678,28 +704,7 @@ __global__ void __launch_bounds__(512) norm_bwd_kernel(const BwdArgs p) {
   const uint32_t pitch = row_pitch(bytes, SG == 0);
   const uint32_t stage = (p.dh ? 3u : 2u) * pitch;
   pdl_launch_dependents();
-  auto fill = [&](int s, int64_t row) {
-    uint8_t* to = rows + s * stage;
-    if constexpr (SG == 0) {
-      mbar_arrive_expect_tx(&ring.full[s], stage);
-      bulk_load(to, static_cast<const T*>(p.dy) + row * p.ldy, bytes, &ring.full[s]);
-      bulk_load(to + pitch, static_cast<const T*>(p.h) + row * p.ldhh, bytes, &ring.full[s]);
-      if (p.dh) bulk_load(to + 2 * pitch, static_cast<const T*>(p.dh) + row * p.lddh, bytes, &ring.full[s]);
-    } else {
-      Span sp[3];
-      sp[0] = row_span<T>(p.dy, p.ldy, p.M, row, bytes);
-      sp[1] = row_span<T>(p.h, p.ldhh, p.M, row, bytes);
-      sp[2] = row_span<T>(p.dh, p.lddh, p.M, row, bytes);
-      if (!p.dh) sp[2].direct = true;
-      uint32_t tx = 0u;
-#pragma unroll
-      for (int k = 0; k < 3; ++k) tx += sp[k].direct ? 0u : sp[k].size;
-      mbar_arrive_expect_tx(&ring.full[s], tx);
-#pragma unroll
-      for (int k = 0; k < 3; ++k)
-        if (!sp[k].direct) bulk_load(to + k * pitch, sp[k].from, sp[k].size, &ring.full[s]);
-    }
-  };
+  auto fill = [&](int s, int64_t row) { fill_bwd_row<T, SG>(p, rows + s * stage, &ring.full[s], row, bytes, pitch); };
   if constexpr (RING) {
     if (t == 0) {
       for (int s = 0; s < p.stages; ++s) mbar_init(&ring.full[s], 1);
@@ -821,28 +826,7 @@ __global__ void __launch_bounds__(kWideThreads) norm_bwd_wide_kernel(const BwdAr
   const uint32_t pitch = row_pitch(bytes, SG == 0);
   const uint32_t stage = (p.dh ? 3u : 2u) * pitch;
   pdl_launch_dependents();
-  auto fill = [&](int s, int64_t row) {
-    uint8_t* to = rows + s * stage;
-    if constexpr (SG == 0) {
-      mbar_arrive_expect_tx(&ring.full[s], stage);
-      bulk_load(to, static_cast<const T*>(p.dy) + row * p.ldy, bytes, &ring.full[s]);
-      bulk_load(to + pitch, static_cast<const T*>(p.h) + row * p.ldhh, bytes, &ring.full[s]);
-      if (p.dh) bulk_load(to + 2 * pitch, static_cast<const T*>(p.dh) + row * p.lddh, bytes, &ring.full[s]);
-    } else {
-      Span sp[3];
-      sp[0] = row_span<T>(p.dy, p.ldy, p.M, row, bytes);
-      sp[1] = row_span<T>(p.h, p.ldhh, p.M, row, bytes);
-      sp[2] = row_span<T>(p.dh, p.lddh, p.M, row, bytes);
-      if (!p.dh) sp[2].direct = true;
-      uint32_t tx = 0u;
-#pragma unroll
-      for (int k = 0; k < 3; ++k) tx += sp[k].direct ? 0u : sp[k].size;
-      mbar_arrive_expect_tx(&ring.full[s], tx);
-#pragma unroll
-      for (int k = 0; k < 3; ++k)
-        if (!sp[k].direct) bulk_load(to + k * pitch, sp[k].from, sp[k].size, &ring.full[s]);
-    }
-  };
+  auto fill = [&](int s, int64_t row) { fill_bwd_row<T, SG>(p, rows + s * stage, &ring.full[s], row, bytes, pitch); };
   if (t == 0) {
     for (int s = 0; s < p.stages; ++s) mbar_init(&ring.full[s], 1);
     fence_mbarrier_init();
@@ -1116,9 +1100,10 @@ cudaError_t launch_rows(const FwdArgs& p, bool vec, cudaStream_t st) {
   }
   constexpr int V = Runs<T, 0>::V;
   // The ring pays where a block per row has too little in flight or too few blocks fit: wide rows
-  // (us, ring / block per row, bf16: quantise 16384 x 4096 41 / 49, 5461 x 12288 42 / 69, norm
-  // 16384 x 4096 77 / 81; but quantise 65536 x 1024 51 / 43 and fp32 8192 x 4096 33 / 25), and once
-  // its blocks have several rows each.
+  // (us, ring / block per row, bf16, 64 Mi elements: quantise at K 4096 41 / 49, 12288 42 / 69, norm at 4096
+  // 77 / 81; but fp32 8192 x 4096 33 / 25), and once its blocks have several rows each. Below 4096 it is
+  // either: quantise at K 3584 44 / 49, 2560 49 / 47, 2048 43 / 45, 1536 47 / 45, 1024 55 / 44, norm 74 / 81,
+  // 76 / 80, 75 / 77, 80 / 78, 82 / 78.
   if (p.K >= (sizeof(T) == 2 ? 4096 : 8200)) {
     // Elements per thread: quantising alone is short of issue slots, and twice the elements halve
     // what a row costs besides them.
@@ -1174,8 +1159,9 @@ size_t bwd_partial_rows(int64_t M, int64_t K, bool vec, int cols) {
     const int sms = sm_count();
     const int64_t most = static_cast<int64_t>(sms > 0 ? sms : 148) * bwd_blocks_per_sm(bwd_threads(K, vec));
     // A row more for a block costs about 0.65 us; a block's share of dweight, written and added up, 1.3 us
-    // per MB. Measured (us) with 1, 2, 3, 4 rows a block: 1000 x 1024 bf16 9.4, 7.9, 7.4, 8.1; 333 x 2048
-    // 8.6, 7.5, 6.9, 7.7; 333 x 512 4.3, 4.8, 6.3, 7.0.
+    // per MB; the square root weighs the two. Measured (us) with 1, 2, 3, 4 rows a block: 1000 x 1024 bf16 9.3,
+    // 8.1, 7.4, 7.9; 600 x 2048 10.5, 8.7, 8.0, 8.4; 333 x 512 4.3, 4.5, 6.2, 6.9; 4000 x 256 9.2, 9.9, 8.6, 8.0.
+    // Over 16 sizes (200 to 4000 rows of 256 to 8192) it takes 3 % longer than the best count, 23 % at the last.
     const int64_t each = static_cast<int64_t>(std::sqrt(8e-6 * static_cast<double>(M) * static_cast<double>(K)) + 0.1);
     const int64_t blocks = each > 1 ? (M + each - 1) / each : M;
     return static_cast<size_t>(blocks < most ? blocks : most);

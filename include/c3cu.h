@@ -155,7 +155,10 @@ int c3cu_set_split_wait_ns(uint64_t ns);
 /* Programmatic dependent launch for the GEMM and pre-pass kernels (process-wide; 0 = off, the
  * default): each such kernel may be scheduled while the previous kernel on its stream drains,
  * runs its prologue (barrier initialisation, TMEM allocation, descriptor prefetch) and then
- * waits for that kernel's completion before it touches global memory. Results are unchanged. */
+ * waits for that kernel's completion before it touches global memory. Results are unchanged. Of the
+ * 8-bit path it reaches the persistent int8 GEMM, the Linear of one to four tokens and the first kernel of
+ * a dW with a workspace; the small-tile GEMMs and the row kernels start when the kernel before them has
+ * ended. The second and third kernels of a call overlap the one before them whatever this is set to. */
 int c3cu_set_launch_overlap(int enable);
 /* Per-shape variant table filled by a tuner (the B200 counterpart of the reference's tile
  * auto-tuner, include/C3/AutoTuner.h:42-63, src/C3/C3Engine.cpp:1577-1651): calls of exactly

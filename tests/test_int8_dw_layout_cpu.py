@@ -4,6 +4,7 @@ threads that go together touch every bank once."""
 import subprocess
 
 import pytest
+import torch
 
 from c3_b200.build import CSRC
 
@@ -104,3 +105,35 @@ def compiled(tmp_path_factory):
 def test_each_piece_is_converted_once_and_lands_in_its_place(compiled):
     r = subprocess.run([str(compiled)])
     assert r.returncode == 0, f"check {r.returncode} failed"
+
+
+def test_two_bf16_terms_hold_the_product():
+    """head and tail of dZ * scale as gemm_ckpt_narrow.cuh makes them (split_scale, split_pair), in fp64 with
+    each rounding to bf16: within 2^-14 of the product, worst and over random scales, and their first
+    multiply-add is exact."""
+    g = torch.Generator().manual_seed(1)
+
+    def bf16(v):
+        return v.to(torch.float32).to(torch.bfloat16).double()  # exact in fp32 or far from a tie of both
+    z = bf16(torch.randn(400000, generator=g).double())
+    s = (torch.rand(400000, generator=g) * torch.exp(4 * torch.randn(400000, generator=g))).double() * 64
+    s = s.float().double()
+    s_head = bf16(s)
+    s_tail = bf16(s - s_head)
+    assert float(((s - s_head - s_tail).abs() / s).max()) <= 2.0 ** -16
+    head = bf16(z * s_head)
+    left = z * s_head - head
+    assert torch.equal(bf16(left), left)
+    tail = bf16(z * s_tail + left)
+    p = z * s
+    ok = p.abs() > 1e-30
+    assert float(((head + tail - p).abs()[ok] / p.abs()[ok]).max()) <= 2.0 ** -14
+
+
+def test_workspace_of_a_dw_too_large():
+    """More tiles than an int counts: refused, where the count used to wrap around."""
+    from c3_b200 import _lib
+    lib = _lib.load()
+    huge = 2 ** 31 - 1000
+    assert lib.c3cu_gemm_dw_int8_workspace(64, huge, huge) == 0 and "too large" in _lib.last_error()
+    assert lib.c3cu_gemm_dw_int8_workspace(16384, 4096, 4096) >= 2 * 16384 * (4096 + 4096)
