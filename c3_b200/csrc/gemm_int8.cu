@@ -286,10 +286,10 @@ int dw_run(int64_t M, int64_t N, int64_t K, DwRun* r) {
   r->plan = ckpt::make_plan(static_cast<int>(tiles), r->clusters, blocks);
   // The fastest form by a model of all, fitted to B200 measurements (us in a graph; blocks: K blocks of 64
   // rows of X that a CTA or pair goes through):
-  //   large            6.0 + waves * 2.06 + blocks 0.34 + cut tiles 2.0 + 0.1 pieces + prep
-  //   small, ready     3.9 + waves (blocks c(T) + e(T)) + prep, the operands' bytes: through L2, or HBM
+  //   large            6.0 + waves * 2.2 + blocks 0.34 + cut tiles 2.1 + 0.107 pieces + prep
+  //   small, ready     3.8 + waves (blocks c(T) + e(T)) + prep, the operands' bytes: through L2, or HBM
   //   small, converted 1.2 + waves (blocks c(T) + e(T)), e for a split tile 3.2 + 0.026 T
-  // Over 330 random sizes its choice takes 0.2 % longer than the fastest form on average. Measured, large /
+  // Over 390 random sizes its choice takes 0.3 % longer than the fastest form on average, 20 % at worst. Measured, large /
   // ready / converted: 256 x 784 over 128 rows 8.8 / 7.3 / 4.6, 1024 x 1024 over 2048 20.0 / 14.7 / 18.5,
   // 512 x 512 over 4096 18.6 / 14.6 / 15.9, 2176 x 4822 over 576 24 / 39 / 50.
   r->T = 0;
@@ -310,7 +310,7 @@ int dw_run(int64_t M, int64_t N, int64_t K, DwRun* r) {
     const double turns = static_cast<double>((tiles + r->clusters - 1) / r->clusters);
     const double bytes = static_cast<double>(M) * (6. * static_cast<double>(N) + 3. * static_cast<double>(K));
     const double prep = bytes / 7.07e6 + (bytes > 42e6 ? (bytes - 42e6) / 12.9e6 : 0.);
-    double least = 6.0 + 2.06 * turns + 0.34 * rounds + (r->plan.rest > 0 ? 2.0 + 0.1 * r->plan.rest * r->plan.pieces : 0.) + prep;
+    double least = 6.0 + 2.2 * turns + 0.34 * rounds + (r->plan.rest > 0 ? 2.1 + 0.107 * r->plan.rest * r->plan.pieces : 0.) + prep;
     constexpr struct {
       int T;
       double c, e;
@@ -325,7 +325,7 @@ int dw_run(int64_t M, int64_t N, int64_t K, DwRun* r) {
         for (int split = 1; split <= ckpt_narrow::kMaxCluster && split <= blocks; split *= 2) {
           const int per = (blocks + split - 1) / split;
           const double e = split == 1 ? kind.e : (ready ? 3.4 : 3.2) + 0.026 * kind.T;
-          const double t = (ready ? 3.9 + prep : 1.2) +
+          const double t = (ready ? 3.8 + prep : 1.2) +
                            static_cast<double>((small + at_once(split) - 1) / at_once(split)) * (per * kind.c + e);
           if (t < least) {
             least = t;
