@@ -54,6 +54,17 @@ struct DzUnits {
     return T >= 64 ? (t >> 3) + 16 * i : 8 * (t >> 5) + ((t >> 3) & 3) + 4 * ((t >> 2) & 1) + 32 * i;
   }
   static C3CU_HD constexpr int piece(int t) { return T >= 64 ? t & 7 : t & 3; }
+
+  // Where dZ lies in chunk c of its tile, and later head; and where tail goes, so that the MMA sees one tile
+  // of 2 T columns, all of head's before all of tail's: in chunks behind head's, or (32 columns) in the second
+  // half of the one chunk.
+  static C3CU_HD constexpr uint32_t head_at(int t, int i, int c) {
+    return static_cast<uint32_t>(c) * kChunkBytes + piece_at(row(t, i), piece(t));
+  }
+  static C3CU_HD constexpr uint32_t tail_at(int t, int i, int c) {
+    return T >= 64 ? head_at(t, i, c + kChunks) : piece_at(row(t, i), piece(t) + 4);
+  }
+  static constexpr uint32_t kBytes = T >= 64 ? 2 * kChunks * kChunkBytes : kChunkBytes;  // head and tail
 };
 
 }  // namespace ckpt

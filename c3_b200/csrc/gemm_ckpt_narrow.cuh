@@ -6,10 +6,12 @@
 // A stage of the ring holds a K block's raw int8 (8 KB), the widened tile made of it (16 KB), and dZ, which
 // the same warps replace by dZ * scale in two bf16 terms (8 KB each per 64 columns): head, the product
 // rounded to bf16, and tail, what that took from it. Their sum is the product to 2^-14 of it, at fp32's
-// range, and the MMA adds q * head and q * tail to the same accumulator; q itself is exact in bf16.
+// range; q itself is exact in bf16. The MMA takes both as one tile of 2 T columns, so that X's tile is read
+// once for the two, and the epilogue adds their sums.
 // (One fp16 term needs the columns' largest first, i.e. two launches more.) The stage is free again when
-// its MMAs are done, so a converter waits for nothing but the loads. What bounds a long sum is the
-// converters' arithmetic.
+// its MMAs are done, so a converter waits for nothing but the loads. What bounds a long sum is shared
+// memory: of a K block of 128 x 128 a copy writes 24 KB, the converters read those and write 48, and the MMAs
+// read 48 (about 0.65 us, where twice the converters changed nothing).
 // Warps: 0 TMA, 1 MMA, 2..9 converters in two groups of four that take the K blocks in turn, and the
 // epilogue after them.
 #pragma once
@@ -36,9 +38,9 @@ static_assert(MN_CHUNK_BYTES == ckpt::kChunkBytes && BK == 64, "ckpt_layout.h");
 
 template <int T, bool READY>
 struct Ring {
-  static constexpr int kStages = !READY ? 4 : T <= 64 ? 8 : 6;
-  static constexpr uint32_t kZ = chunks(T) * MN_CHUNK_BYTES;  // dZ, then head; tail behind it
-  static constexpr uint32_t kStage = WIDE_BYTES + (READY ? kZ : 2 * kZ + RAW_BYTES);
+  static constexpr int kStages = READY ? (T <= 64 ? 8 : 6) : T == 32 ? 6 : 4;
+  static constexpr uint32_t kZ = READY ? chunks(T) * MN_CHUNK_BYTES : ckpt::DzUnits<T>::kBytes;
+  static constexpr uint32_t kStage = WIDE_BYTES + kZ + (READY ? 0 : RAW_BYTES);
   static constexpr uint32_t kSmem = kStages * kStage + (3 * kStages + 2) * 8 + 16 + 1024;
   static_assert(READY || kStages % kConvGroups == 0, "a stage belongs to one group, which so sees each of its phases");
   static_assert(kSmem <= 227 * 1024 && kStages * kStage >= T * COLS * 4, "shared memory");
@@ -139,25 +141,40 @@ __device__ __forceinline__ void split8(const uint4& w, const Scale2& s, uint4& h
     l = make_uint4(finite_pair(l.x), finite_pair(l.y), finite_pair(l.z), finite_pair(l.w));
 }
 
-// dZ's chunks at `z` become heads, their tails go `tail` bytes behind them: thread t's share. scale[i] is
-// that of the thread's i-th row.
+// dZ at `z` becomes head and tail: thread t's share. scale[i] is that of the thread's i-th row.
 template <int T>
-__device__ __forceinline__ void split_dz(uint32_t z, uint32_t tail, int t, const float (&scale)[ckpt::DzUnits<T>::kRows]) {
+__device__ __forceinline__ void split_dz(uint32_t z, int t, const float (&scale)[ckpt::DzUnits<T>::kRows]) {
   using U = ckpt::DzUnits<T>;
 #pragma unroll
   for (int c = 0; c < U::kChunks; ++c) {
     uint4 w[U::kRows];
 #pragma unroll
-    for (int i = 0; i < U::kRows; ++i)
-      w[i] = ld_shared_v4(z + c * ckpt::kChunkBytes + ckpt::piece_at(U::row(t, i), U::piece(t)));
+    for (int i = 0; i < U::kRows; ++i) w[i] = ld_shared_v4(z + U::head_at(t, i, c));
 #pragma unroll
     for (int i = 0; i < U::kRows; ++i) {
-      const uint32_t at = z + c * ckpt::kChunkBytes + ckpt::piece_at(U::row(t, i), U::piece(t));
       uint4 h, l;
       split8(w[i], split_scale(scale[i]), h, l);
-      st_shared_v4(at, h);
-      st_shared_v4(at + tail, l);
+      st_shared_v4(z + U::head_at(t, i, c), h);
+      st_shared_v4(z + U::tail_at(t, i, c), l);
     }
+  }
+}
+
+// Sixteen sums of a lane's column from row c on. Converted tiles have head's and tail's beside each other.
+template <int T, bool READY>
+__device__ __forceinline__ void load_sums(uint32_t t_row, int c, float (&sum)[16]) {
+  uint32_t r[16];
+  tmem_ld_32x32b_x16(t_row + c, r);
+  if constexpr (READY) {
+    tmem_wait_ld();
+#pragma unroll
+    for (int j = 0; j < 16; ++j) sum[j] = __uint_as_float(r[j]);
+  } else {
+    uint32_t l[16];
+    tmem_ld_32x32b_x16(t_row + T + c, l);
+    tmem_wait_ld();
+#pragma unroll
+    for (int j = 0; j < 16; ++j) sum[j] = __uint_as_float(r[j]) + __uint_as_float(l[j]);
   }
 }
 
@@ -166,7 +183,8 @@ __global__ void __launch_bounds__(kThreads)
     dw_narrow_kernel(const __grid_constant__ CUtensorMap tmz, const __grid_constant__ CUtensorMap tmx, const Params p) {
   constexpr int STAGES = Ring<T, READY>::kStages;
   constexpr uint32_t STAGE = Ring<T, READY>::kStage;
-  constexpr uint32_t Z_AT = WIDE_BYTES, TAIL = Ring<T, READY>::kZ, RAW_AT = Z_AT + 2 * TAIL;
+  constexpr uint32_t Z_AT = WIDE_BYTES, RAW_AT = Z_AT + Ring<T, READY>::kZ;
+  constexpr uint32_t SUMS = READY ? T : 2 * T;  // columns of the accumulator
   __shared__ float s_back[T];  // READY
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
@@ -206,7 +224,7 @@ __global__ void __launch_bounds__(kThreads)
     tma_prefetch_desc(&tmx);
   }
   if (warp == 1) {
-    tmem_alloc(tmem_slot, T);
+    tmem_alloc(tmem_slot, SUMS);
     tmem_relinquish();
   }
   tc_fence_before();
@@ -245,7 +263,7 @@ __global__ void __launch_bounds__(kThreads)
     __syncwarp();
   } else if (warp == 1) {
     if (lane == 0) {
-      constexpr uint32_t IDESC = READY ? make_idesc_f16_f32(COLS, T, true, true) : make_idesc_bf16_f32(COLS, T, true, true);
+      constexpr uint32_t IDESC = READY ? make_idesc_f16_f32(COLS, SUMS, true, true) : make_idesc_bf16_f32(COLS, SUMS, true, true);
       int s = 0;
       uint32_t ph = 0;
       bool ok = true;
@@ -258,12 +276,10 @@ __global__ void __launch_bounds__(kThreads)
         const uint32_t x = smem_u32(smem + s * STAGE);
         const uint32_t z = x + Z_AT;
 #pragma unroll
-        for (int part = 0; part < (READY ? 1 : 2); ++part)
-#pragma unroll
-          for (int kk = 0; kk < BK / UMMA_K; ++kk)
-            umma_f16_ss(tmem, make_sw128_desc(x + kk * UMMA_K * 128, MN_CHUNK_BYTES, 1024),
-                        make_sw128_desc(z + part * TAIL + kk * UMMA_K * 128, MN_CHUNK_BYTES, 1024), IDESC,
-                        (kb != kb0 || kk != 0 || part != 0) ? 1u : 0u);
+        for (int kk = 0; kk < BK / UMMA_K; ++kk)
+          umma_f16_ss(tmem, make_sw128_desc(x + kk * UMMA_K * 128, MN_CHUNK_BYTES, 1024),
+                      make_sw128_desc(z + kk * UMMA_K * 128, MN_CHUNK_BYTES, 1024), IDESC,
+                      (kb != kb0 || kk != 0) ? 1u : 0u);
         umma_commit(&empty[s]);
         if (++s == STAGES) { s = 0; ph ^= 1u; }
       }
@@ -300,7 +316,7 @@ __global__ void __launch_bounds__(kThreads)
         next[i] = m < p.M ? __ldg(p.scale + m) : 0.f;
       }
       widen_x(at + RAW_AT, at, t);
-      split_dz<T>(at + Z_AT, TAIL, t, scale);
+      split_dz<T>(at + Z_AT, t, scale);
       fence_proxy_async_shared();  // the MMA reads the tiles through the async proxy
       __syncwarp();
       if (lane == 0) mbar_arrive(&wide[s]);
@@ -328,14 +344,13 @@ __global__ void __launch_bounds__(kThreads)
     if (warp >= 2 && ok) {
 #pragma unroll 1
       for (int c = 16 * half; c < rows; c += 32) {
-        uint32_t r[16];
+        float sum[16];
         __syncwarp();  // lanes past the last column skip the stores
-        tmem_ld_32x32b_x16(t_row + c, r);
-        tmem_wait_ld();
+        load_sums<T, READY>(t_row, c, sum);
         if (k < p.K) {
 #pragma unroll
           for (int j = 0; j < 16; ++j)
-            if (c + j < rows) out[(c + j) * p.ldo] = rounded(__uint_as_float(r[j]), c + j);
+            if (c + j < rows) out[(c + j) * p.ldo] = rounded(sum[j], c + j);
         }
       }
       __syncwarp();
@@ -348,11 +363,10 @@ __global__ void __launch_bounds__(kThreads)
     if (warp >= 2 && ok) {
 #pragma unroll 1
       for (int c = 16 * half; c < rows; c += 32) {
-        uint32_t r[16];
-        tmem_ld_32x32b_x16(t_row + c, r);
-        tmem_wait_ld();
+        float sum[16];
+        load_sums<T, READY>(t_row, c, sum);
 #pragma unroll
-        for (int j = 0; j < 16; ++j) part[(c + j) * COLS + q * 32u + lane] = any ? __uint_as_float(r[j]) : 0.f;
+        for (int j = 0; j < 16; ++j) part[(c + j) * COLS + q * 32u + lane] = any ? sum[j] : 0.f;
       }
     }
     cluster_sync_all();
@@ -391,7 +405,7 @@ __global__ void __launch_bounds__(kThreads)
       if (asked[0] & (1u << t)) gemm::drain_wait(&full[t], (asked[1] >> t) & 1u);
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, T);
+    tmem_dealloc(tmem, SUMS);
   }
 }
 

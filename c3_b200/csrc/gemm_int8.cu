@@ -289,7 +289,8 @@ int dw_run(int64_t M, int64_t N, int64_t K, DwRun* r) {
   //   large            6.0 + waves * 2.2 + blocks 0.34 + cut tiles 2.1 + 0.107 pieces + prep
   //   small, ready     3.8 + waves (blocks c(T) + e(T)) + prep, the operands' bytes: through L2, or HBM
   //   small, converted 1.2 + waves (blocks c(T) + e(T)), e for a split tile 3.2 + 0.026 T
-  // Over 390 random sizes its choice takes 0.3 % longer than the fastest form on average, 20 % at worst. Measured, large /
+  // Over 120 random sizes that it was not fitted to its choice takes 0.5 % longer than the fastest form on
+  // average, 18 % at worst. Measured, large /
   // ready / converted: 256 x 784 over 128 rows 8.8 / 7.3 / 4.6, 1024 x 1024 over 2048 20.0 / 14.7 / 18.5,
   // 512 x 512 over 4096 18.6 / 14.6 / 15.9, 2176 x 4822 over 576 24 / 39 / 50.
   r->T = 0;

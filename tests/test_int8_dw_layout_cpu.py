@@ -63,6 +63,8 @@ static int dz_tile() {
   using U = DzUnits<T>;
   static char seen[U::kChunks][8192 / 16];
   std::memset(seen, 0, sizeof seen);
+  static char both[U::kBytes / 16];  // head and tail, as the MMA reads them: column n, then T + n
+  std::memset(both, 0, sizeof both);
   for (int c = 0; c < U::kChunks; ++c)
     for (int i = 0; i < U::kRows; ++i) {
       for (int t = 0; t < 128; ++t) {
@@ -70,13 +72,23 @@ static int dz_tile() {
         if (row < 0 || row >= 64 || piece < 0 || piece >= 8 || 64 * c + 8 * piece >= T) return 1;
         if (piece_at(row, piece) != swizzled(row, piece)) return 2;
         if (seen[c][piece_at(row, piece) / 16]++) return 3;
+        for (int tail = 0; tail < 2; ++tail) {
+          const int col = tail * T + 64 * c + 8 * piece;
+          const unsigned want = col / 64 * kChunkBytes + swizzled(row, col % 64 / 8);
+          if ((tail ? U::tail_at(t, i, c) : U::head_at(t, i, c)) != want || both[want / 16]++) return 6;
+        }
       }
       for (int t = 0; t < 128; t += 8) {
-        unsigned at[8];
-        for (int j = 0; j < 8; ++j) at[j] = piece_at(U::row(t + j, i), U::piece(t + j));
-        if (!banks_once(at)) return 4;
+        unsigned at[8], behind[8];
+        for (int j = 0; j < 8; ++j) {
+          at[j] = U::head_at(t + j, i, c);
+          behind[j] = U::tail_at(t + j, i, c);
+        }
+        if (!banks_once(at) || !banks_once(behind)) return 4;
       }
     }
+  for (char b : both)
+    if (b != 1) return 7;
   for (int row = 0; row < 64; ++row)
     for (int col = 0; col < T; col += 8)
       if (seen[col / 64][swizzled(row, col % 64 / 8) / 16] != 1) return 5;
