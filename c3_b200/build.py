@@ -100,11 +100,11 @@ def build_fast_calls() -> Path:
 
 
 def try_build_fast_calls() -> Path | None:
-    """None, with a warning, where the binding cannot be built (no C++ compiler, a torch without its
-    headers)."""
+    """None, with a warning, where the binding cannot be built (no C++ compiler, a torch without its headers
+    or of another making)."""
     try:
         return build_fast_calls()
-    except (OSError, RuntimeError) as e:
+    except Exception as e:
         warnings.warn(f"the C++ binding of the 8-bit calls was not built, they go through ctypes: {str(e)[-600:]}",
                       RuntimeWarning, stacklevel=2)
         return None

@@ -67,7 +67,7 @@ __device__ __forceinline__ void st_shared_v4(uint32_t addr, const uint4& v) {
 
 // dZ * scale is taken times 2^6 and q times 2^-6: what head and tail lose of a product at the bottom of
 // fp32's normal numbers then is no more than of any other (below, a product is held to 2^-138), and the
-// scale of a row of fp32's largest numbers, 2^128 / 127, times 2^6 is finite.
+// scale of a row of fp32's largest numbers, 2^128 / 127, times 2^6 is finite. Products from 2^122 on are not.
 constexpr float kUp = 64.f;
 
 // The two int8 in bits 0..7 and 16..23 of w times 2^-6 as two bf16, exactly. 0x4000 is 128 * 2^-6 in bf16,

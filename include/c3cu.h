@@ -325,8 +325,9 @@ int c3cu_linear_int8_fwd(const int8_t* X, int64_t ldx, const float* x_scale, con
 int c3cu_set_int8_form(int tile, int split, int ready);
 /* dW[N][K] = sum_m (dZ[m][n] x_scale[m]) X[m][k] as bf16: the weight gradient from an 8-bit
  * checkpoint of the layer's input. X takes part exactly; dZ x_scale is held to 2^-11 of itself at
- * least (fp16 with a power of two for each row of dW, or two bf16 terms, by size), so that the
- * error is that of the output's rounding; fp32 accumulation. dZ [M][N] bf16. A row with scale NaN
+ * least (fp16 with a power of two for each row of dW, or two bf16 terms, by size; products far
+ * below their row's largest to 2^-39 of that, and all below 2^-126 to 2^-138 or better; products
+ * from 2^122 on count as infinite), so that the error is that of the output's rounding; fp32 accumulation. dZ [M][N] bf16. A row with scale NaN
  * makes all of dW NaN; dZ's infinities and NaN reach their row of dW. Workspace:
  * c3cu_gemm_dw_int8_workspace(M, N, K) bytes of device memory (16-byte aligned) that no other call
  * uses meanwhile: 0 for small dW, else both operands in fp16 and partial sums; the size depends on

@@ -177,3 +177,21 @@ def test_what_is_not_finite_stays_so_and_where_it_is(cuda_device, form):
     dz[7, 3] = dz[9, 4] = clean[7, 3] * 0
     rest = [i for i in range(n) if i not in (3, 4)]
     _check(dw[rest], dz[:, rest], q, s)
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_large_products(cuda_device, form):
+    """Products of dZ and scale up to 2^121 (small tiles take them times 2^6), in sums that fp32 holds."""
+    dev = cuda_device
+    m, n, k = 66, 16, 24
+    dz = torch.zeros((m, n), dtype=BF16, device=dev)
+    dz[3], dz[65] = 1.5 * 2.0 ** 100, -2.0 ** 100
+    q = quant.empty_rows(m, k, dev)
+    q.fill_(127)
+    q[3] = (torch.arange(k, device=dev) % 7 - 3).to(torch.int8)
+    q[65] = 2
+    s = torch.full((m,), 2.0 ** 20, device=dev)
+    with _form(*form):
+        dw = linear.grad_weight_int8(dz, q, s)
+    want = (1.5 * q[3].double() - 2) * 2.0 ** 120  # exact in bf16
+    assert torch.equal(dw.double(), want.expand(n, k))

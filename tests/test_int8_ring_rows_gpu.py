@@ -14,9 +14,12 @@ def _kernels(call):
     """Names of the kernels that a call launches, or None where the profiler sees no GPU."""
     from torch.profiler import ProfilerActivity, profile
     torch.cuda.synchronize()
-    with profile(activities=[ProfilerActivity.CUDA], acc_events=True) as p:
-        call()
-        torch.cuda.synchronize()
+    try:
+        with profile(activities=[ProfilerActivity.CUDA], acc_events=True) as p:
+            call()
+            torch.cuda.synchronize()
+    except RuntimeError:  # the profiler's, where another tool holds the GPU's counters
+        return None
     names = [e.key for e in p.key_averages() if "kernel" in e.key]
     return names or None
 
