@@ -11,7 +11,7 @@
 //
 // fp16 has five bits of exponent where bf16 has eight, so each column of dZ * scale, i.e. each row of dW,
 // is brought into its range by a power of two of its own:
-//   column_top_kernel  the largest finite |dZ * scale| of each column (in bands of rows)
+//   column_top_kernel  the largest finite |dZ * scale| of each column (in bands of rows; not launched for one)
 //   operands_kernel    dZ * scale * 2^(14 - e) in fp16, e the exponent of the column's largest, and q in
 //                      fp16, both into the workspace
 //   dw_kernel          the product, gemm2_kernel's structure (256 x 256 tiles on CTA pairs, both operands
@@ -273,26 +273,31 @@ __device__ __forceinline__ uint4 load_ragged_dz(const Prep& p, int64_t m, int n)
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// f(row, dZ's eight columns from n on, scale) for the thread's rows of a band, eight loads ahead of their use.
-template <class F>
-__device__ __forceinline__ void for_rows(const Prep& p, int64_t m0, int64_t m1, int n, F f) {
-  constexpr int A = 8;
-  int64_t m = m0;
-  if (n + 8 <= p.N) {
-    for (; m + (A - 1) * kPrepRows < m1; m += A * kPrepRows) {
-      uint4 w[A];
-      float s[A];
+// f(row, dZ's eight columns from n on, scale) for A of the thread's rows at a time, whose loads go out
+// together, while there are A left before m1; returns the next row.
+template <int A, class F>
+__device__ __forceinline__ int64_t for_rows_by(const Prep& p, int64_t m, int64_t m1, int n, F& f) {
+  for (; m + (A - 1) * kPrepRows < m1; m += A * kPrepRows) {
+    uint4 w[A];
+    float s[A];
 #pragma unroll
-      for (int a = 0; a < A; ++a) {
-        w[a] = __ldg(reinterpret_cast<const uint4*>(p.dz + (m + a * kPrepRows) * p.lddz + n));
-        s[a] = __ldg(p.scale + m + a * kPrepRows);
-      }
-#pragma unroll
-      for (int a = 0; a < A; ++a) f(m + a * kPrepRows, w[a], s[a]);
+    for (int a = 0; a < A; ++a) {
+      w[a] = __ldg(reinterpret_cast<const uint4*>(p.dz + (m + a * kPrepRows) * p.lddz + n));
+      s[a] = __ldg(p.scale + m + a * kPrepRows);
     }
-#pragma unroll 4
-    for (; m < m1; m += kPrepRows)
-      f(m, __ldg(reinterpret_cast<const uint4*>(p.dz + m * p.lddz + n)), __ldg(p.scale + m));
+#pragma unroll
+    for (int a = 0; a < A; ++a) f(m + a * kPrepRows, w[a], s[a]);
+  }
+  return m;
+}
+
+// The same for all of the thread's rows of a band.
+template <class F>
+__device__ __forceinline__ void for_rows(const Prep& p, int64_t m, int64_t m1, int n, F f) {
+  if (n + 8 <= p.N) {
+    m = for_rows_by<8>(p, m, m1, n, f);
+    m = for_rows_by<4>(p, m, m1, n, f);
+    for_rows_by<1>(p, m, m1, n, f);
   } else {
     for (; m < m1; m += kPrepRows) f(m, load_ragged_dz(p, m, n), __ldg(p.scale + m));
   }
@@ -312,57 +317,67 @@ __device__ __forceinline__ float larger_finite(float top, float v) {
   return fabsf(v) < __builtin_huge_valf() ? larger(top, v) : top;
 }
 
+// The largest finite |dZ * scale| of the tile's column threadIdx.x (below 64) in rows m0.. of a band, by the
+// whole block.
+struct Tops {
+  float of[kPrepThreads / 32][64];
+};
+
+__device__ __forceinline__ float column_top(const Prep& p, int tile, int64_t m0, int64_t m1, Tops& s) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int piece = lane & 7, n = tile * 64 + piece * 8;
+  m0 += threadIdx.x >> 3;
+  float top[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (n < p.N) {
+    const auto walk = [&](auto pick) {
+      for_rows(p, m0, m1, n, [&](int64_t, const uint4& w, float scale) {
+        float2 v[4];
+        scaled8(w, scale, v);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          top[2 * j] = pick(top[2 * j], v[j].x);
+          top[2 * j + 1] = pick(top[2 * j + 1], v[j].y);
+        }
+      });
+    };
+    walk([](float t, float v) { return larger(t, v); });
+    bool infinite = false;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) infinite = infinite || top[j] == __builtin_huge_valf();
+    if (infinite) {  // again without what is infinite
+#pragma unroll
+      for (int j = 0; j < 8; ++j) top[j] = 0.f;
+      walk([](float t, float v) { return larger_finite(t, v); });
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    top[j] = fmaxf(top[j], __shfl_xor_sync(0xffffffffu, top[j], 8));
+    top[j] = fmaxf(top[j], __shfl_xor_sync(0xffffffffu, top[j], 16));
+  }
+  if (lane < 8) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s.of[warp][piece * 8 + j] = top[j];
+  }
+  __syncthreads();
+  float t = 0.f;
+  if (threadIdx.x < 64) {
+#pragma unroll
+    for (int w = 0; w < kPrepThreads / 32; ++w) t = fmaxf(t, s.of[w][threadIdx.x]);
+  }
+  return t;
+}
+
 __global__ void __launch_bounds__(kPrepThreads) column_top_kernel(const Prep p) {
-  __shared__ float s_top[kPrepThreads / 32][64];
+  __shared__ Tops s_top;
   pdl_wait();
   pdl_launch_dependents();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int piece = lane & 7;
   for (int item = blockIdx.x; item < p.tiles * p.bands; item += gridDim.x) {
     const int tile = item % p.tiles, band = item / p.tiles;
-    const int n = tile * 64 + piece * 8;
-    const int64_t m1 = min(static_cast<int64_t>(p.M), static_cast<int64_t>(band + 1) * p.band_rows);
-    const int64_t m0 = static_cast<int64_t>(band) * p.band_rows + (threadIdx.x >> 3);
-    float top[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (n < p.N) {
-      const auto walk = [&](auto pick) {
-        for_rows(p, m0, m1, n, [&](int64_t, const uint4& w, float s) {
-          float2 v[4];
-          scaled8(w, s, v);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            top[2 * j] = pick(top[2 * j], v[j].x);
-            top[2 * j + 1] = pick(top[2 * j + 1], v[j].y);
-          }
-        });
-      };
-      walk([](float t, float v) { return larger(t, v); });
-      bool infinite = false;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) infinite = infinite || top[j] == __builtin_huge_valf();
-      if (infinite) {  // again without what is infinite
-#pragma unroll
-        for (int j = 0; j < 8; ++j) top[j] = 0.f;
-        walk([](float t, float v) { return larger_finite(t, v); });
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      top[j] = fmaxf(top[j], __shfl_xor_sync(0xffffffffu, top[j], 8));
-      top[j] = fmaxf(top[j], __shfl_xor_sync(0xffffffffu, top[j], 16));
-    }
-    if (lane < 8) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) s_top[warp][piece * 8 + j] = top[j];
-    }
-    __syncthreads();
-    if (threadIdx.x < 64) {
-      float t = 0.f;
-#pragma unroll
-      for (int w = 0; w < kPrepThreads / 32; ++w) t = fmaxf(t, s_top[w][threadIdx.x]);
-      p.top[(static_cast<int64_t>(band) * p.tiles + tile) * 64 + threadIdx.x] = t;
-    }
-    __syncthreads();
+    const int64_t m0 = static_cast<int64_t>(band) * p.band_rows;
+    const float t = column_top(p, tile, m0, min(static_cast<int64_t>(p.M), m0 + p.band_rows), s_top);
+    if (threadIdx.x < 64) p.top[(static_cast<int64_t>(band) * p.tiles + tile) * 64 + threadIdx.x] = t;
+    __syncthreads();  // the next item's maxima go to the same place
   }
 }
 
@@ -419,7 +434,7 @@ __device__ __forceinline__ void widen_row(const Prep& p, int64_t m, int lane) {
 constexpr int kWidenRows = kPrepThreads / 32;
 
 __global__ void __launch_bounds__(kPrepThreads) operands_kernel(const Prep p) {
-  __shared__ float s_top[kPrepThreads / 64][64];
+  __shared__ Tops s_top;
   __shared__ __align__(16) float s_up[64];
   pdl_wait();
   pdl_launch_dependents();
@@ -434,31 +449,34 @@ __global__ void __launch_bounds__(kPrepThreads) operands_kernel(const Prep p) {
     }
     const int back_item = dz_items - 1 - item;
     const int tile = back_item % p.tiles, band = back_item / p.tiles;
-    {
-      const int c = threadIdx.x & 63;
-      float t = 0.f;
+    const int64_t m0 = static_cast<int64_t>(band) * p.band_rows;
+    const int64_t m1 = min(static_cast<int64_t>(p.M), m0 + p.band_rows);
+    const int c = threadIdx.x & 63;
+    float t = 0.f;
+    if (p.bands == 1) {  // no kernel before this one
+      t = column_top(p, tile, m0, m1, s_top);
+    } else {
       for (int b = threadIdx.x >> 6; b < p.bands; b += kPrepThreads / 64)
         t = fmaxf(t, __ldcg(p.top + (static_cast<int64_t>(b) * p.tiles + tile) * 64 + c));
-      s_top[threadIdx.x >> 6][c] = t;
+      s_top.of[threadIdx.x >> 6][c] = t;
       __syncthreads();
-      if (threadIdx.x < 64) {
 #pragma unroll
-        for (int i = 1; i < kPrepThreads / 64; ++i) t = fmaxf(t, s_top[i][c]);
-        // Below 2^-112 the exponent stays there, so that both powers are normal numbers; fp16's last
-        // place is then 2^-150, beneath fp32's.
-        const int e = max(static_cast<int>(__float_as_uint(t) >> 23) - 127, -112);
-        s_up[c] = __uint_as_float(static_cast<uint32_t>(14 - e + 127) << 23);
-        if (band == 0) p.back[tile * 64 + c] = __uint_as_float(static_cast<uint32_t>(e - 14 + 127) << 23);
-      }
-      __syncthreads();
+      for (int i = 1; i < kPrepThreads / 64; ++i) t = fmaxf(t, s_top.of[i][c]);
     }
+    if (threadIdx.x < 64) {
+      // Below 2^-112 the exponent stays there, so that both powers are normal numbers; fp16's last
+      // place is then 2^-150, beneath fp32's.
+      const int e = max(static_cast<int>(__float_as_uint(t) >> 23) - 127, -112);
+      s_up[c] = __uint_as_float(static_cast<uint32_t>(14 - e + 127) << 23);
+      if (band == 0) p.back[tile * 64 + c] = __uint_as_float(static_cast<uint32_t>(e - 14 + 127) << 23);
+    }
+    __syncthreads();
     const int piece = lane & 7, n = tile * 64 + piece * 8;
-    const int64_t m1 = min(static_cast<int64_t>(p.M), static_cast<int64_t>(band + 1) * p.band_rows);
     if (n < p.N) {
       float2 up[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) up[j] = *reinterpret_cast<const float2*>(&s_up[piece * 8 + 2 * j]);
-      for_rows(p, static_cast<int64_t>(band) * p.band_rows + (threadIdx.x >> 3), m1, n,
+      for_rows(p, m0 + (threadIdx.x >> 3), m1, n,
                [&](int64_t m, const uint4& w, float s) {
                  float2 v[4];
                  scaled8(w, s, v);

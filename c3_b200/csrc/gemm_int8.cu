@@ -274,6 +274,11 @@ int dw_clusters(int* clusters) {
   return rc;
 }
 
+// Up to this many rows dZ is one band, whose columns' maxima operands_kernel finds by itself: its blocks read
+// their rows twice in less time than a launch takes (us in a graph, one band / two kernels: 128 x 4096 x 4096 14.7
+// / 16.6, 300 x 12288 x 1024 17.5 / 19.1, 576 x 2176 x 4822 23.2 / 23.7, 640 x 2560 x 2048 17.4 / 16.6).
+constexpr int64_t kOneBand = 576;
+
 int dw_run(int64_t M, int64_t N, int64_t K, DwRun* r) {
   const int64_t tiles = ((N + ckpt::TM - 1) / ckpt::TM) * ((K + ckpt::TN - 1) / ckpt::TN);
   if (tiles > (1 << 24)) {
@@ -287,7 +292,8 @@ int dw_run(int64_t M, int64_t N, int64_t K, DwRun* r) {
   // The fastest form by a model of all, fitted to B200 measurements (us in a graph; blocks: K blocks of 64
   // rows of X that a CTA or pair goes through):
   //   large            6.0 + waves * 2.2 + blocks 0.34 + cut tiles 2.1 + 0.107 pieces + prep
-  //   small, ready     3.8 + waves (blocks c(T) + e(T)) + prep, the operands' bytes: through L2, or HBM
+  //   small, ready     3.8 + waves (blocks c(T) + e(T)) + prep, the operands' bytes: through L2, or HBM,
+  //                    less 1.0 for a launch that is not made (kOneBand)
   //   small, converted 1.2 + waves (blocks c(T) + e(T)), e for a split tile 3.2 + 0.026 T
   // Over 120 random sizes that it was not fitted to its choice takes 0.5 % longer than the fastest form on
   // average, 18 % at worst. Measured, large /
@@ -310,7 +316,7 @@ int dw_run(int64_t M, int64_t N, int64_t K, DwRun* r) {
                               : static_cast<double>((tiles + r->clusters - 1) / r->clusters) * blocks;
     const double turns = static_cast<double>((tiles + r->clusters - 1) / r->clusters);
     const double bytes = static_cast<double>(M) * (6. * static_cast<double>(N) + 3. * static_cast<double>(K));
-    const double prep = bytes / 7.07e6 + (bytes > 42e6 ? (bytes - 42e6) / 12.9e6 : 0.);
+    const double prep = bytes / 7.07e6 + (bytes > 42e6 ? (bytes - 42e6) / 12.9e6 : 0.) - (M <= kOneBand ? 1.0 : 0.);
     double least = 6.0 + 2.2 * turns + 0.34 * rounds + (r->plan.rest > 0 ? 2.1 + 0.107 * r->plan.rest * r->plan.pieces : 0.) + prep;
     constexpr struct {
       int T;
@@ -353,6 +359,7 @@ int dw_run(int64_t M, int64_t N, int64_t K, DwRun* r) {
   int64_t rows = (M + bands - 1) / bands;
   rows = (rows + ckpt::kPrepRows - 1) / ckpt::kPrepRows * ckpt::kPrepRows;
   if (rows < 128) rows = 128;
+  if (M <= kOneBand) rows = (M + 31) / 32 * 32;
   p.band_rows = static_cast<int32_t>(rows);
   p.bands = static_cast<int32_t>((M + rows - 1) / rows);
   p.ldz = (N + 7) / 8 * 8;
@@ -413,10 +420,14 @@ int launch_dw_ready(const DwRun& r, const ckpt::Prep& a, const ckpt::Params& p, 
   const auto grid = [most](int64_t items) { return dim3(static_cast<unsigned>(items < most ? items : most)); };
   const int64_t dz_items = static_cast<int64_t>(a.tiles) * a.bands;
   const int64_t x_items = (static_cast<int64_t>(a.M) + ckpt::kWidenRows - 1) / ckpt::kWidenRows;
-  int rc = cuda_status(launch_kernel(ckpt::column_top_kernel, grid(dz_items), dim3(ckpt::kPrepThreads), 0, st, a),
-                       "gemm_dw_int8: launch");
+  int rc = C3CU_OK;
+  if (a.bands > 1)
+    rc = cuda_status(launch_kernel(ckpt::column_top_kernel, grid(dz_items), dim3(ckpt::kPrepThreads), 0, st, a),
+                     "gemm_dw_int8: launch");
   if (rc != C3CU_OK) return rc;
-  rc = cuda_status(launch_next(ckpt::operands_kernel, grid(dz_items + x_items), dim3(ckpt::kPrepThreads), 0, st, a),
+  // with one band it is the call's first kernel
+  rc = cuda_status(launch_serialized(a.bands > 1 || pdl_enabled(), ckpt::operands_kernel, grid(dz_items + x_items),
+                                     dim3(ckpt::kPrepThreads), 0, st, a),
                    "gemm_dw_int8: launch");
   if (rc != C3CU_OK) return rc;
   CUtensorMap tz, tx;  // fp16, which TMA moves like any two bytes

@@ -126,12 +126,13 @@ def test_training_batch(cuda_device):
 FORMS = [(0, 1, 0), (32, 1, 0), (64, 2, 0), (128, 4, 0), (32, 2, 1), (64, 1, 1), (128, 2, 1)]
 
 
+@pytest.mark.parametrize("m", [300, 1300])
 @pytest.mark.parametrize("form", FORMS)
-def test_columns_and_rows_of_any_size(cuda_device, form):
+def test_columns_and_rows_of_any_size(cuda_device, form, m):
     """Columns of dZ from 1e-30 to 1e30 beside each other, one of zeros, rows of X from 1e-6 to 1e6: each
     row of dW is as exact as if it were alone."""
     dev = cuda_device
-    m, n, k = 300, 72, 200
+    n, k = 72, 200
     dz, q, s = _case(m, n, k, dev, 9)
     sizes = 10.0 ** torch.linspace(-30, 30, n, dtype=torch.float64, device=dev)
     dz.copy_((dz.double() * 1e3 * sizes[None, :]).to(BF16))
@@ -161,14 +162,15 @@ def test_products_at_the_ends_of_fp32(cuda_device, form):
     assert bool(((dw.double() - ref).abs() <= tol).all())
 
 
+@pytest.mark.parametrize("m", [130, 1300])
 @pytest.mark.parametrize("form", FORMS)
-def test_what_is_not_finite_stays_so_and_where_it_is(cuda_device, form):
+def test_what_is_not_finite_stays_so_and_where_it_is(cuda_device, form, m):
     dev = cuda_device
-    m, n, k = 130, 40, 96
+    n, k = 40, 96
     dz, q, s = _case(m, n, k, dev, 13)
     clean = dz.clone()
     q[q == 0] = 1
-    dz[7, 3] = float("inf")
+    dz[7, 3] = float("inf")  # the rows of a few blocks apart: one alone meets it
     dz[9, 4] = float("nan")
     with _form(*form):
         dw = linear.grad_weight_int8(dz, q, s)
